@@ -18,6 +18,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libi8f.so"
 I8F_BF16, I8F_F16, I8F_F32 = 0, 1, 2
 WSCALE_TENSOR, WSCALE_CHANNEL = 0, 1
 EPI_PYTORCH, EPI_SINGLE = 0, 1
+NORM_CODE = {None: 0, "rms": 1, "layer": 2}
 STATIC_WORKSPACE_BYTES = 16 * 1024 * 1024 + 256 * 1024
 
 DTYPE_CODE = {torch.bfloat16: I8F_BF16, torch.float16: I8F_F16, torch.float32: I8F_F32}
@@ -26,6 +27,14 @@ DTYPE_CODE = {torch.bfloat16: I8F_BF16, torch.float16: I8F_F16, torch.float32: I
 class NativeLibraryError(RuntimeError):
     """libi8f.so is missing, stale, or reported an error."""
 
+
+class RequestRowsStruct(ctypes.Structure):
+    """i8f_request_rows of the C header."""
+    _fields_ = [("rows", c_int64), ("row_adapter", c_void_p), ("row_request", c_void_p), ("chunks", c_void_p),
+                ("n_chunks", c_int64), ("max_adapter", ctypes.c_int32)]
+
+
+_ROWS = ctypes.POINTER(RequestRowsStruct)
 
 _PROTOTYPES = {
     "i8f_version": (c_int, []),
@@ -75,6 +84,20 @@ _PROTOTYPES = {
                             c_int64, c_void_p]),
     "i8f_lora_up_add": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64,
                                 c_int64, c_void_p]),
+    "i8f_lora_down_requests": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, _ROWS, c_void_p, c_int64, c_int, c_int64,
+                                       c_int64, c_void_p]),
+    "i8f_lora_requests_workspace_bytes": (c_size_t, [_ROWS, c_int64]),
+    "i8f_linear_w8a8_lora_requests": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int,
+                                              c_void_p, c_int64, c_void_p, c_int64, c_int64, _ROWS, c_void_p, c_int, c_int64,
+                                              c_int64, c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "i8f_linear_w8a16_small_lora_requests_workspace_bytes": (c_size_t, [_ROWS, c_int64, c_int64]),
+    "i8f_linear_w8a16_small_lora_requests": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int,
+                                                     c_void_p, c_void_p, c_int64, c_int64, _ROWS, c_void_p, c_int64, c_int64,
+                                                     c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
+    "i8f_gated_residual_norm": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                        c_int64, c_int, c_float, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+                                        c_int64, c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                        c_void_p]),
     "i8f_lora_merge_sr": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int,
                                   c_int64, c_int64, c_int64, c_float, c_int, c_void_p, c_uint64, c_void_p]),
     "i8f_lora_merge_max_rank": (c_int64, [c_int, c_int]),

@@ -46,6 +46,8 @@ constexpr int kStageRowBytes = 128; // one 128-byte swizzle span of K per stage
 
 enum Kind : int { kKindI8 = 0, kKindBF16 = 1, kKindF16 = 2 };
 enum EpiMode : int { kEpiI32 = 0, kEpiDequant = 1, kEpiCast = 2, kEpiAccum = 3 };
+// what joins the product in the epilogue (a template parameter, so that the plain kernels carry none of it)
+enum Extra : int { kExtraNone = 0, kExtraLora = 1, kExtraAddend = 2 };
 
 // status codes written by bounded waits
 enum : int { kStEmptyWait = 101, kStFullWait = 102, kStAccEmptyWait = 103, kStAccFullWait = 104 };
@@ -75,6 +77,10 @@ struct GemmParams {
     int out_col0; // column of the destination matrices at which this launch's block starts
     int k_split;  // 1, or 2: the two CTAs of a cluster each take half of K for the same tile (single-CTA kernels)
     int* status;
+    // kExtraAddend: fp32 [M, ld_addend], added before the rounding to rows whose row_adapter is not negative
+    const float* addend;
+    long long ld_addend;
+    const int* row_adapter;
 };
 
 constexpr int kMaxOutputs = 8;
@@ -92,8 +98,9 @@ struct alignas(64) LoraMaps {
     CUtensorMap b;   // lora_b [N, r], box 64 x (rows of B per CTA)
 };
 
-template <int BN, bool PAIR, bool LORA = false>
+template <int BN, bool PAIR, int EXTRA = kExtraNone>
 struct Cfg {
+    static constexpr bool LORA = EXTRA == kExtraLora;
     static constexpr int kBRows = PAIR ? BN / 2 : BN;  // rows of B this CTA stages
     static constexpr int kABytes = kBM * kStageRowBytes;
     static constexpr int kBBytes = kBRows * kStageRowBytes;
@@ -255,9 +262,9 @@ __device__ __forceinline__ void old_values(const GemmParams& p, long long row, i
 // term (bias, LoRA, previous output) is one packed add per pair.  The result goes either straight to global
 // memory or, when `stage` is non-zero, into this warp's shared-memory staging chunk (row = lane, 64 bytes per
 // row, 16-byte pieces XOR-swizzled with (row >> 1) & 3 as the TMA 64-byte swizzle expects).
-template <int OUT, bool LORA>
+template <int OUT, int EXTRA>
 __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, long long row, bool row_ok, int col,
-                                               const uint32_t (&v)[32], const uint32_t (&lv)[LORA ? 32 : 1], float row_scale,
+                                               const uint32_t (&v)[32], const uint32_t (&lv)[EXTRA != kExtraNone ? 32 : 1], float row_scale,
                                                float ws_scalar, const float* cs, const float* cb, const OldChunk& old,
                                                uint32_t stage, int lane, int wide_half = -1, const uint32_t* cg = nullptr) {
     uint32_t yp[16];
@@ -283,6 +290,12 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, long long ro
 #pragma unroll
             for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], cb[j]);
         }
+        if constexpr (EXTRA == kExtraAddend) {
+            if (single) {   // the low-rank term joins in fp32: one rounding in all
+#pragma unroll
+                for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], __uint_as_float(lv[j]));
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) yp[i] = pack2<OUT>(y[2 * i], y[2 * i + 1]);
         if (!single && p.bias != nullptr) {
@@ -290,11 +303,13 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, long long ro
 #pragma unroll
             for (int i = 0; i < 16; ++i) yp[i] = add2<OUT>(yp[i], cbp[i]);
         }
-        if constexpr (LORA) {
+        if constexpr (EXTRA != kExtraNone) {
             // y + lora_y.to(y.dtype): both terms are in the output type, as in the reference
+            if (EXTRA == kExtraLora || !single) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                yp[i] = add2<OUT>(yp[i], pack2<OUT>(__uint_as_float(lv[2 * i]), __uint_as_float(lv[2 * i + 1])));
+                for (int i = 0; i < 16; ++i)
+                    yp[i] = add2<OUT>(yp[i], pack2<OUT>(__uint_as_float(lv[2 * i]), __uint_as_float(lv[2 * i + 1])));
+            }
         }
         if (p.add_existing && row_ok) {
             uint32_t prev[16];
@@ -358,11 +373,12 @@ __device__ __forceinline__ void store_i32_row32(const GemmParams& p, long long r
     }
 }
 
-template <int KIND, int BN, bool PAIR, bool LORA>
-__global__ void __launch_bounds__((Cfg<BN, PAIR, LORA>::kThreads), 1)
+template <int KIND, int BN, bool PAIR, int EXTRA>
+__global__ void __launch_bounds__((Cfg<BN, PAIR, EXTRA>::kThreads), 1)
 gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ OutMaps outs, const __grid_constant__ LoraMaps lora, const GemmParams p) {
-    using C = Cfg<BN, PAIR, LORA>;
+    using C = Cfg<BN, PAIR, EXTRA>;
+    constexpr bool LORA = C::LORA;
     static_assert(!LORA || (KIND == kKindI8 && PAIR), "the fused LoRA accumulator exists for the paired int8 kernel");
     constexpr int kElemsPerStage = (KIND == kKindI8) ? kStageRowBytes : kStageRowBytes / 2;
     constexpr uint32_t kIdesc = (KIND == kKindI8)     ? make_idesc(kDFmtS32, kFmtS8, C::kTileM, BN)
@@ -643,6 +659,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const long long warp_row0 = row - lane;
             const bool row_ok = row < p.M;
             const float row_scale = (dequant && row_ok) ? __ldg(p.a_scale + row) : 0.f;
+            bool has_addend = false;
+            if constexpr (EXTRA == kExtraAddend) has_addend = row_ok && __ldg(p.row_adapter + row) >= 0;
             // this warp's share of the tile's 32-column chunks (all of them with four epilogue warps), cut at N
             constexpr int kChunksPerWarp = (BN / 32) / (C::kEpiWarps / 4);
             const int c_first = ((warp - 2) >> 2) * kChunksPerWarp;
@@ -689,8 +707,19 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 const int col = n_blk * BN + c * 32;
                 uint32_t v[32];
                 tmem_ld_32x32(t_addr + c * 32, v);
-                uint32_t lv[LORA ? 32 : 1];
+                uint32_t lv[EXTRA != kExtraNone ? 32 : 1];
                 if constexpr (LORA) tmem_ld_32x32(t_lora + c * 32, lv);
+                if constexpr (EXTRA == kExtraAddend) {   // ld_addend is a multiple of 32: a whole chunk is always there
+                    const uint4* src = reinterpret_cast<const uint4*>(p.addend + row * p.ld_addend + col);
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        const uint4 o = has_addend ? __ldg(src + g) : make_uint4(0u, 0u, 0u, 0u);
+                        lv[4 * g] = o.x;
+                        lv[4 * g + 1] = o.y;
+                        lv[4 * g + 2] = o.z;
+                        lv[4 * g + 3] = o.w;
+                    }
+                }
                 const OldChunk old_cur = old_next;
                 if (need_old && c + 1 < c_end) prefetch_old(p, row, row_ok, col + 32, old_next);
                 uint32_t stage = 0;
@@ -737,11 +766,11 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 if (p.epi_mode == kEpiI32) {
                     if (row_ok) store_i32_row32(p, row, col, v);
                 } else if (p.out_dtype == I8F_BF16) {
-                    epilogue_chunk<I8F_BF16, LORA>(p, row, row_ok, col, v, lv, row_scale, ws_scalar, col_scale + c * 32,
+                    epilogue_chunk<I8F_BF16, EXTRA>(p, row, row_ok, col, v, lv, row_scale, ws_scalar, col_scale + c * 32,
                                                    col_bias + c * bias_step, old_cur, stage, lane, wide_half,
                                                    has_gate ? reinterpret_cast<const uint32_t*>(col_bias) + BN / 2 + c * 16 : nullptr);
                 } else {
-                    epilogue_chunk<I8F_F16, LORA>(p, row, row_ok, col, v, lv, row_scale, ws_scalar, col_scale + c * 32,
+                    epilogue_chunk<I8F_F16, EXTRA>(p, row, row_ok, col, v, lv, row_scale, ws_scalar, col_scale + c * 32,
                                                   col_bias + c * bias_step, old_cur, stage, lane, wide_half,
                                                   has_gate ? reinterpret_cast<const uint32_t*>(col_bias) + BN / 2 + c * 16 : nullptr);
                 }
@@ -946,13 +975,13 @@ struct LoraOperands {
     int kind;             // kKindBF16 or kKindF16
 };
 
-template <int KIND, int BN, bool PAIR, bool LORA = false>
+template <int KIND, int BN, bool PAIR, int EXTRA = kExtraNone>
 int launch_gemm(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N, int64_t K, GemmParams p,
                 cudaStream_t st, const Scatter* scatter = nullptr, const LoraOperands* lo = nullptr, int k_split = 1) {
-    using C = Cfg<BN, PAIR, LORA>;
+    using C = Cfg<BN, PAIR, EXTRA>;
     CUtensorMap tmA, tmB;
     LoraMaps lmaps{};
-    if (LORA) {
+    if (C::LORA) {
         int rc_l = make_operand_map(&lmaps.t, lo->kind, lo->t, M, lo->r, lo->ldt, kBM);
         if (rc_l != I8F_OK) return rc_l;
         rc_l = make_operand_map(&lmaps.b, lo->kind, lo->b, N, lo->r, lo->ldb, C::kBRows);
@@ -998,7 +1027,7 @@ int launch_gemm(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t 
     p.tiles_n = static_cast<int>((N + BN - 1) / BN);
     p.status = device_status_word();
     I8F_REQUIRE(p.status != nullptr, I8F_ERR_CUDA, "device status word unavailable");
-    auto kern = gemm_tcgen05_kernel<KIND, BN, PAIR, LORA>;
+    auto kern = gemm_tcgen05_kernel<KIND, BN, PAIR, EXTRA>;
     static bool attr_done[64] = {false};
     static int max_clusters[64] = {0};
     const int dev = current_device();
@@ -1165,17 +1194,17 @@ GemmPlan plan_gemm(int64_t M, int64_t N, int64_t K, int elem_bytes, int64_t sms,
     return plan;
 }
 
-template <int KIND>
+template <int KIND, int EXTRA = kExtraNone>
 int launch_gemm_auto(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N, int64_t K,
                      const GemmParams& p, cudaStream_t st, const Scatter* scatter = nullptr) {
     const GemmPlan plan = plan_gemm(M, N, K, KIND == kKindI8 ? 1 : 2, sm_count(), scatter != nullptr, forced_tile(), ksplit_enabled());
     const int k_split = plan.k_split;
     switch (plan.choice) {
-        case 1: return launch_gemm<KIND, 256, true>(a, lda, b, ldb, M, N, K, p, st, scatter);
-        case 2: return launch_gemm<KIND, 256, false>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
-        case 3: return launch_gemm<KIND, 128, false>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
-        case 5: return launch_gemm<KIND, 32, false>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
-        default: return launch_gemm<KIND, 64, false>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
+        case 1: return launch_gemm<KIND, 256, true, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter);
+        case 2: return launch_gemm<KIND, 256, false, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
+        case 3: return launch_gemm<KIND, 128, false, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
+        case 5: return launch_gemm<KIND, 32, false, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
+        default: return launch_gemm<KIND, 64, false, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
     }
 }
 
@@ -1238,7 +1267,9 @@ int i8f_gemm_i8_i32(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw, 
 static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw,
                             const float* w_scale, int w_scale_mode, const void* bias, int bias_dtype, void* out,
                             int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int epilogue_order,
-                            int add_existing, void* stream, const Scatter* scatter = nullptr, const void* gate = nullptr) {
+                            int add_existing, void* stream, const Scatter* scatter = nullptr, const void* gate = nullptr,
+                            const float* addend = nullptr, int64_t ld_addend = 0, const int* row_adapter = nullptr,
+                            bool check_only = false) {
     int rc = check_operands(a, lda, w, ldw, 1, M, N, K);
     if (rc != I8F_OK) return rc;
     I8F_REQUIRE(a_scale != nullptr && w_scale != nullptr, I8F_ERR_INVALID_ARG, "NULL scale pointer");
@@ -1249,6 +1280,7 @@ static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, 
     I8F_REQUIRE(bias == nullptr || dtype_size(bias_dtype) != 0, I8F_ERR_INVALID_ARG, "unknown bias dtype %d", bias_dtype);
     I8F_REQUIRE(epilogue_order == I8F_EPI_PYTORCH || epilogue_order == I8F_EPI_SINGLE, I8F_ERR_INVALID_ARG,
                 "unknown epilogue_order %d", epilogue_order);
+    if (check_only) return I8F_OK;
     GemmParams p{};
     p.out = out;
     p.ldo = ldo;
@@ -1264,7 +1296,12 @@ static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, 
     p.gate = gate;
     p.vec_ok = aligned16(out) && (ldo % 8 == 0);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-
+    if (addend != nullptr) {
+        p.addend = addend;
+        p.ld_addend = ld_addend;
+        p.row_adapter = row_adapter;
+        return launch_gemm_auto<kKindI8, kExtraAddend>(a, lda, w, ldw, M, N, K, p, st);
+    }
     return launch_gemm_auto<kKindI8>(a, lda, w, ldw, M, N, K, p, st, scatter);
 }
 
@@ -1343,9 +1380,9 @@ int i8f_linear_w8a8_lora(const int8_t* a, int64_t lda, const float* a_scale, con
         return (v == 128 || v == 160) ? v : 256;
     }();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (bn == 160) return launch_gemm<kKindI8, 160, true, true>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
-    if (bn == 128) return launch_gemm<kKindI8, 128, true, true>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
-    return launch_gemm<kKindI8, 256, true, true>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
+    if (bn == 160) return launch_gemm<kKindI8, 160, true, kExtraLora>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
+    if (bn == 128) return launch_gemm<kKindI8, 128, true, kExtraLora>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
+    return launch_gemm<kKindI8, 256, true, kExtraLora>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
 }
 
 int i8f_linear_w8a8_scatter(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw,
@@ -1445,3 +1482,15 @@ int i8f_lora_up_add(const void* t, int64_t ldt, const void* lora_b, int64_t ldb,
 }
 
 }  // extern "C"
+
+namespace i8f {
+
+int linear_w8a8_addend(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
+                       int w_scale_mode, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M,
+                       int64_t N, int64_t K, int epilogue_order, const float* addend, int64_t ld_addend, const int* row_adapter,
+                       bool check_only, cudaStream_t stream) {
+    return linear_w8a8_impl(a, lda, a_scale, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, out_dtype, ldo, M, N, K,
+                            epilogue_order, 0, stream, nullptr, nullptr, addend, ld_addend, row_adapter, check_only);
+}
+
+}  // namespace i8f

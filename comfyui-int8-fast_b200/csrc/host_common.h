@@ -42,6 +42,18 @@ inline int check_launch(const char* what) {
 
 int* device_status_word();  // device address of the status word on the current device, or nullptr
 
+// i8f_linear_w8a8 with an fp32 addend [M, ld_addend] (ld_addend a multiple of 32, 16-byte aligned) on the rows whose
+// row_adapter is not negative; in gemm_tcgen05.cu.  With `check_only` the arguments are checked and nothing is launched, so
+// that a caller can refuse a bad call before it launches what comes first.
+int linear_w8a8_addend(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
+                       int w_scale_mode, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M,
+                       int64_t N, int64_t K, int epilogue_order, const float* addend, int64_t ld_addend, const int* row_adapter,
+                       bool check_only, cudaStream_t stream);
+// The same for at most 16 rows of unquantised activations; in linear_small_m.cu.
+int linear_small_addend(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
+                        const void* bias, int bias_dtype, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                        const float* addend, int64_t ld_addend, const int* row_adapter, bool check_only, cudaStream_t stream);
+
 }  // namespace i8f
 
 #define I8F_REQUIRE(cond, code, ...)                    \

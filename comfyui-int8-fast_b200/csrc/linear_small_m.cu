@@ -55,16 +55,22 @@ __device__ __forceinline__ float load_bias(const void* bias, int bias_dt, int64_
     return static_cast<const float*>(bias)[n];
 }
 
-// Four int8 in a word -> two packed 16-bit pairs of dt(fp32(w) * s).
-template <int DT>
+// Four int8 in a word -> two packed 16-bit pairs of dt(fp32(w) * s), or with SCALED false of w itself (exact in both types).
+template <int DT, bool SCALED>
 __device__ __forceinline__ void dequant4(uint32_t word, float s, uint32_t& lo, uint32_t& hi) {
     constexpr uint32_t kTwo23 = 0x4B000000u;      // 2^23: its low mantissa byte receives w + 128
     constexpr float kOffset = 8388736.0f;         // 2^23 + 128
     const uint32_t u = word ^ 0x80808080u;
-    const float f0 = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(u, kTwo23, 0x7440)), kOffset), s);
-    const float f1 = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(u, kTwo23, 0x7441)), kOffset), s);
-    const float f2 = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(u, kTwo23, 0x7442)), kOffset), s);
-    const float f3 = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(u, kTwo23, 0x7443)), kOffset), s);
+    float f0 = __fsub_rn(__uint_as_float(__byte_perm(u, kTwo23, 0x7440)), kOffset);
+    float f1 = __fsub_rn(__uint_as_float(__byte_perm(u, kTwo23, 0x7441)), kOffset);
+    float f2 = __fsub_rn(__uint_as_float(__byte_perm(u, kTwo23, 0x7442)), kOffset);
+    float f3 = __fsub_rn(__uint_as_float(__byte_perm(u, kTwo23, 0x7443)), kOffset);
+    if constexpr (SCALED) {
+        f0 = __fmul_rn(f0, s);
+        f1 = __fmul_rn(f1, s);
+        f2 = __fmul_rn(f2, s);
+        f3 = __fmul_rn(f3, s);
+    }
     lo = pack2<DT>(f0, f1);
     hi = pack2<DT>(f2, f3);
 }
@@ -107,14 +113,14 @@ __device__ __forceinline__ void load_x(XFrag& f, const uint16_t* xap, const uint
 // The weights are the A operand (16 features x 16 k, built in registers by the dequantisation, so the four
 // registers of a fragment need no shuffling), the activations the B operand (16 k x 8 tokens, whose register
 // pairs are consecutive words of the 128-bit loads).
-template <int DT, bool HI_ROWS>
+template <int DT, bool HI_ROWS, bool SCALED>
 __device__ __forceinline__ void consume_chunk(const uint4& wlo, const uint4& whi, const XFrag& x, float sc_lo, float sc_hi,
                                               float (&acc)[HI_ROWS ? 2 : 1][4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         uint32_t a0, a1, a2, a3;
-        dequant4<DT>(word_of(wlo, j), sc_lo, a0, a2);
-        dequant4<DT>(word_of(whi, j), sc_hi, a1, a3);
+        dequant4<DT, SCALED>(word_of(wlo, j), sc_lo, a0, a2);
+        dequant4<DT, SCALED>(word_of(whi, j), sc_hi, a1, a3);
         // x words 2j and 2j+1 of the lane's 8 (two elements each) = real k 4j..4j+3
         mma_16x8x16<DT>(acc[0], a0, a1, a2, a3, word_of(x.a[j >> 1], (2 * j) & 3), word_of(x.a[j >> 1], (2 * j + 1) & 3));
         if constexpr (HI_ROWS)
@@ -129,11 +135,21 @@ __device__ __forceinline__ void consume_chunk(const uint4& wlo, const uint4& whi
 // tokens are independent in the accumulator, so lanes whose feature or token is past the end read a valid
 // stand-in (the last feature / token 0) instead of carrying predicates; those results are never stored.
 // kDepth: weight chunks in flight per lane (a register ring); the activations (L1/L2 hits) are fetched per chunk.
-template <int DT, bool HI_ROWS, int kDepth>
+//
+// REQ: the form beside per-request adapters, y = dt(scale * (x . w^T) + bias + addend) with an fp32 addend [M, ld_addend] on
+// the rows whose row_adapter is not negative.  The weights enter the product as the integers they are (exact in bf16 and
+// fp16, and one multiply per weight less) and everything is rounded once, at the end; the plain form keeps the
+// reference's roundings of the scaled weight and of the bias.
+struct SmallAddend {
+    const float* addend;
+    int64_t ld;
+    const int* row_adapter;
+};
+template <int DT, bool HI_ROWS, int kDepth, bool REQ>
 __global__ void __launch_bounds__(kThreads, HI_ROWS ? 3 : 4)
 small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict__ w, int64_t ldw,
                const float* __restrict__ w_scale, int per_row, const void* __restrict__ bias, int bias_dt,
-               void* __restrict__ out, int64_t ldo, int M, int64_t N, int64_t K) {
+               void* __restrict__ out, int64_t ldo, int M, int64_t N, int64_t K, const SmallAddend req) {
     constexpr int kHalves = HI_ROWS ? 2 : 1;
     __shared__ float4 s_part[2][kWarps][kHalves][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -186,7 +202,7 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
                 if (i < my_chunks) {   // warp-uniform
                     XFrag xf;
                     load_x<HI_ROWS>(xf, xap, xbp, s * kStride);
-                    consume_chunk<DT, HI_ROWS>(ring_lo[s], ring_hi[s], xf, sc_lo, sc_hi, acc);
+                    consume_chunk<DT, HI_ROWS, !REQ>(ring_lo[s], ring_hi[s], xf, sc_lo, sc_hi, acc);
                     if (i + kDepth < my_chunks) {
                         ring_lo[s] = __ldg(reinterpret_cast<const uint4*>(wlo + (s + kDepth) * kStride));
                         ring_hi[s] = __ldg(reinterpret_cast<const uint4*>(whi + (s + kDepth) * kStride));
@@ -210,7 +226,7 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
                 load_x<HI_ROWS>(xf, xa0, xb0, k0);
             }
             // every lane of the warp executes the MMAs (mma.sync is a warp-wide operation); lanes past K feed zeros
-            consume_chunk<DT, HI_ROWS>(tlo, thi, xf, sc_lo, sc_hi, acc);
+            consume_chunk<DT, HI_ROWS, !REQ>(tlo, thi, xf, sc_lo, sc_hi, acc);
         }
 
         // the next block's first weights are in flight while this block's partial sums meet
@@ -240,7 +256,12 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
             for (int e = 0; e < 4; ++e) {
                 const int m = h * 8 + 2 * t + (e & 1);
                 const int64_t n = nb * 16 + g + (e >> 1) * 8;
-                if (m < M && n < N) {
+                if (REQ && m < M && n < N) {
+                    float r = v[e] * (per_row ? __ldg(w_scale + n) : __ldg(w_scale));
+                    if (bias != nullptr) r += load_bias(bias, bias_dt, n);
+                    if (__ldg(req.row_adapter + m) >= 0) r += __ldg(req.addend + m * req.ld + n);
+                    store_dt<DT>(out, static_cast<int64_t>(m) * ldo + n, r);
+                } else if (m < M && n < N) {
                     const float b = bias != nullptr ? round_dt<DT>(load_bias(bias, bias_dt, n)) : 0.0f;
                     store_dt<DT>(out, static_cast<int64_t>(m) * ldo + n, __fadd_rn(v[e], b));
                 }
@@ -253,16 +274,16 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
     }
 }
 
-template <int DT>
+template <int DT, bool REQ = false>
 int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int per_row,
                    const void* bias, int bias_dt, void* out, int64_t ldo, int M, int64_t N, int64_t K,
-                   cudaStream_t stream) {
+                   cudaStream_t stream, const SmallAddend& req = SmallAddend{}) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const int64_t blocks = (N + 15) / 16;
     const bool hi = M > 8;
-    auto kernel = hi ? small_m_kernel<DT, true, 2> : small_m_kernel<DT, false, 2>;
+    auto kernel = hi ? small_m_kernel<DT, true, 2, REQ> : small_m_kernel<DT, false, 2, REQ>;
     // persistent: as many CTAs as are resident at once, each walking feature blocks with a grid stride
     static int s_resident[2][2] = {};
     int& per_sm = s_resident[DT == I8F_BF16 ? 0 : 1][hi ? 1 : 0];
@@ -274,18 +295,18 @@ int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, con
     }
     const int64_t resident = static_cast<int64_t>(per_sm) * sms;
     const int grid = static_cast<int>(blocks < resident ? blocks : resident);
-    kernel<<<grid, kThreads, 0, stream>>>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K);
+    kernel<<<grid, kThreads, 0, stream>>>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, req);
     return check_launch("small_m_kernel");
 }
 
 }  // namespace
 }  // namespace i8f
 
-extern "C" int i8f_linear_w8a16_small(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw,
-                                      const float* w_scale, int w_scale_mode, const void* bias, int bias_dtype,
-                                      void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, void* stream_) {
+// Argument checks shared by the entry points; *empty is set where there is nothing to compute.
+static int check_small(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
+                       const void* bias, int bias_dtype, const void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, bool* empty) {
     using namespace i8f;
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    *empty = false;
     I8F_REQUIRE(x != nullptr && w != nullptr && w_scale != nullptr && out != nullptr, I8F_ERR_INVALID_ARG,
                 "x, w, w_scale and out must not be NULL");
     I8F_REQUIRE(x_dtype == I8F_BF16 || x_dtype == I8F_F16, I8F_ERR_UNSUPPORTED, "x_dtype must be bf16 or fp16");
@@ -298,7 +319,18 @@ extern "C" int i8f_linear_w8a16_small(const void* x, int x_dtype, int64_t ldx, c
     I8F_REQUIRE(ldx >= K && ldw >= K && ldo >= N, I8F_ERR_INVALID_ARG, "a pitch is smaller than its row");
     I8F_REQUIRE(K % 16 == 0 && ldw % 16 == 0 && ldx % 8 == 0 && aligned16(x) && aligned16(w), I8F_ERR_ALIGNMENT,
                 "K and ldw must be multiples of 16, ldx of 8, x and w 16-byte aligned");
-    if (M == 0 || N == 0) return I8F_OK;
+    *empty = M == 0 || N == 0;
+    return I8F_OK;
+}
+
+extern "C" int i8f_linear_w8a16_small(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw,
+                                      const float* w_scale, int w_scale_mode, const void* bias, int bias_dtype,
+                                      void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, void* stream_) {
+    using namespace i8f;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    bool empty;
+    const int rc = check_small(x, x_dtype, ldx, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, ldo, M, N, K, &empty);
+    if (rc != I8F_OK || empty) return rc;
     const int per_row = w_scale_mode == I8F_WSCALE_CHANNEL;
     if (x_dtype == I8F_BF16)
         return dispatch_small<I8F_BF16>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dtype, out, ldo, static_cast<int>(M), N,
@@ -306,3 +338,22 @@ extern "C" int i8f_linear_w8a16_small(const void* x, int x_dtype, int64_t ldx, c
     return dispatch_small<I8F_F16>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dtype, out, ldo, static_cast<int>(M), N, K,
                                    stream);
 }
+
+namespace i8f {
+
+int linear_small_addend(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
+                        const void* bias, int bias_dtype, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                        const float* addend, int64_t ld_addend, const int* row_adapter, bool check_only, cudaStream_t stream) {
+    bool empty;
+    const int rc = check_small(x, x_dtype, ldx, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, ldo, M, N, K, &empty);
+    if (rc != I8F_OK || empty || check_only) return rc;
+    const int per_row = w_scale_mode == I8F_WSCALE_CHANNEL;
+    const SmallAddend req{addend, ld_addend, row_adapter};
+    if (x_dtype == I8F_BF16)
+        return dispatch_small<I8F_BF16, true>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dtype, out, ldo, static_cast<int>(M), N,
+                                              K, stream, req);
+    return dispatch_small<I8F_F16, true>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dtype, out, ldo, static_cast<int>(M), N, K,
+                                         stream, req);
+}
+
+}  // namespace i8f

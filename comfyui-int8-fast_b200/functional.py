@@ -6,10 +6,13 @@ implementation.
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 from torch import Tensor
 
 from . import _native as nat
+from .adapters import RequestRows
 
 HADAMARD_GROUP = 128
 
@@ -34,6 +37,15 @@ def _code(dtype: torch.dtype) -> int:
         return nat.DTYPE_CODE[dtype]
     except KeyError:
         raise TypeError(f"unsupported dtype {dtype}; expected bf16, fp16 or fp32") from None
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Context in which `device` is the current one (the C ABI launches on the current device)."""
+    idx = device.index
+    return _SAME_DEVICE if idx is None or idx == torch.cuda.current_device() else torch.cuda.device(idx)
 
 
 _WORKSPACE_BYTES: dict = {}
@@ -411,6 +423,230 @@ def lora_up_add_(y: Tensor, t: Tensor, lora_b: Tensor) -> Tensor:
         nat.check(nat.load().i8f_lora_up_add(nat.ptr(t), _ld(t), nat.ptr(lora_b), _ld(lora_b), nat.ptr(y), _ld(y),
                                              _code(y.dtype), M, N, r, nat.current_stream(y.device)), "i8f_lora_up_add")
     return y
+
+
+def _check_requests(rows: RequestRows, x: Tensor, lora_a: Tensor | None, lora_b: Tensor | None, dtype: torch.dtype, K: int, N: int):
+    """The row plan and the bank of adapters against the call; returns (adapters, rank)."""
+    if rows.device != x.device:
+        raise ValueError(f"the row plan is on {rows.device}, the activations on {x.device}")
+    if rows.total != x.shape[0]:
+        raise ValueError(f"the row plan is for {rows.total} rows, the call has {x.shape[0]}")
+    n = r = None
+    for name, bank, inner in (("lora_a", lora_a, (1, K)), ("lora_b", lora_b, (2, N))):
+        if bank is None:
+            continue
+        if bank.dim() != 3 or bank.dtype != dtype or bank.device != x.device or not bank.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [adapters, ...] bank of {dtype} on {x.device}, got {bank.dtype} "
+                             f"{tuple(bank.shape)} on {bank.device}")
+        rank = bank.shape[1] if inner[0] == 1 else bank.shape[2]
+        other = bank.shape[2] if inner[0] == 1 else bank.shape[1]
+        if other != inner[1] or (n is not None and (bank.shape[0], rank) != (n, r)):
+            raise ValueError(f"{name} {tuple(bank.shape)} does not fit the layer [{N}, {K}] or the other factor")
+        n, r = bank.shape[0], rank
+    if rows.max_adapter >= n:
+        raise ValueError(f"the rows name adapter {rows.max_adapter}, the bank has {n}")
+    return n, r
+
+
+def lora_down_requests(x: Tensor, lora_a: Tensor, rows: RequestRows) -> Tensor:
+    """t [M,r]: row m of x (bf16 or fp16) times the transposed lora_a [adapters, r, K] of the row's adapter, in x's dtype;
+    zeros on rows without an adapter."""
+    nat.require_device(x.device)
+    x = _rows(x)
+    M, K = x.shape
+    n, r = _check_requests(rows, x, lora_a, None, x.dtype, K, 0)
+    t = torch.empty((M, r), dtype=x.dtype, device=x.device)
+    if M:
+        with _on(x.device):
+            nat.check(nat.load().i8f_lora_down_requests(x.data_ptr(), _ld(x), lora_a.data_ptr(), n, r, rows.native_ptr, t.data_ptr(), r,
+                                                        _code(x.dtype), M, K, nat.current_stream(x.device)),
+                      "i8f_lora_down_requests")
+    return t
+
+
+def linear_w8a8_lora_requests(q: Tensor, q_scale: Tensor, w: Tensor, w_scale, bias: Tensor | None, t: Tensor, lora_b: Tensor,
+                              rows: RequestRows, out_dtype: torch.dtype, order: int = nat.EPI_SINGLE) -> Tensor:
+    """Dequantising int8 GEMM from pre-quantised activations with the low-rank term t[m] @ lora_b[adapter(m)]^T of each
+    row's own adapter (lora_b [adapters, N, r], t from lora_down_requests; both in out_dtype).
+
+    The default order keeps everything in fp32 up to one rounding; EPI_PYTORCH has the roundings of linear_w8a8_lora."""
+    nat.require_device(q.device)
+    q, w, t = _rows(q), _rows(w), _rows(t)
+    M, K = q.shape
+    N = w.shape[0]
+    _check_weight(w, K)
+    n, r = _check_requests(rows, q, None, lora_b, out_dtype, K, N)
+    if t.shape != (M, r) or t.dtype != out_dtype or t.device != q.device:
+        raise ValueError(f"t must be [{M}, {r}] in {out_dtype} on {q.device}")
+    if q_scale.numel() != M or q_scale.dtype != torch.float32:
+        raise ValueError(f"q_scale must be fp32 with one entry per row ({M})")
+    ws, mode = _wscale_arg(w_scale, q.device, N)
+    bias = _bias_arg(bias, q.device, N)
+    out = torch.empty((M, N), dtype=out_dtype, device=q.device)
+    if M and N:
+        with _on(q.device):
+            lib = nat.load()
+            need = lib.i8f_lora_requests_workspace_bytes(rows.native_ptr, N)
+            workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+            nat.check(lib.i8f_linear_w8a8_lora_requests(q.data_ptr(), _ld(q), nat.ptr(q_scale.reshape(-1)), w.data_ptr(), _ld(w),
+                                                        ws.data_ptr(), mode, nat.ptr(bias), _code(bias.dtype) if bias is not None else 0,
+                                                        t.data_ptr(), _ld(t), lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(),
+                                                        _code(out_dtype), N, M, N, K, order, workspace.data_ptr(), need,
+                                                        nat.current_stream(q.device)), "i8f_linear_w8a8_lora_requests")
+    return out
+
+
+def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lora_a: Tensor, lora_b: Tensor, rows: RequestRows,
+                         out_dtype: torch.dtype, hadamard: bool = False, rotated_lora_input: bool = True,
+                         order: int = nat.EPI_SINGLE) -> Tensor:
+    """Quantised linear of a batch of requests: (rotate) -> quantise -> int8 GEMM shared by all rows, with the low-rank
+    adapter of each row's request (lora_a [adapters, r, K], lora_b [adapters, N, r], see adapters.stack_adapters) beside it.
+
+    x [M,K] bf16 or fp16, out_dtype the same type.  With `hadamard` the adapters see the rotated activations unless
+    `rotated_lora_input` is false, as in the single-adapter forward."""
+    if out_dtype != x.dtype:
+        raise ValueError(f"out_dtype must be the activations' type {x.dtype}, which the adapters share")
+    _check_requests(rows, x, lora_a, lora_b, out_dtype, x.shape[-1], w.shape[0])
+    with _on(x.device):
+        if hadamard and rotated_lora_input:
+            q, q_scale, lora_in = quantize_rowwise(x, hadamard=True, return_rotated=True)
+        else:
+            q, q_scale = quantize_rowwise(x, hadamard=hadamard)
+            lora_in = x
+        t = lora_down_requests(lora_in, lora_a, rows)
+        return linear_w8a8_lora_requests(q, q_scale, w, w_scale, bias, t, lora_b, rows, out_dtype, order=order)
+
+
+def linear_small_batch_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lora_a: Tensor, lora_b: Tensor,
+                                     rows: RequestRows) -> Tensor:
+    """M <= 16 rows (single tokens) of several requests: y = x @ (w * w_scale)^T + bias + (x @ lora_a[a]^T) @ lora_b[a]^T with
+    the adapter a of each row, activations not quantised, one rounding to x's dtype (bf16 or fp16)."""
+    nat.require_device(x.device)
+    x, w = _rows(x), _rows(w)
+    M, K = x.shape
+    N = w.shape[0]
+    _check_weight(w, K)
+    n, r = _check_requests(rows, x, lora_a, lora_b, x.dtype, K, N)
+    ws, mode = _wscale_arg(w_scale, x.device, N)
+    bias = _bias_arg(bias, x.device, N)
+    out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    if M and N:
+        with _on(x.device):
+            lib = nat.load()
+            need = lib.i8f_linear_w8a16_small_lora_requests_workspace_bytes(rows.native_ptr, N, r)
+            workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
+            nat.check(lib.i8f_linear_w8a16_small_lora_requests(x.data_ptr(), _code(x.dtype), _ld(x), w.data_ptr(), _ld(w), ws.data_ptr(), mode,
+                                                               nat.ptr(bias), _code(bias.dtype) if bias is not None else 0,
+                                                               lora_a.data_ptr(), lora_b.data_ptr(), n, r, rows.native_ptr,
+                                                               out.data_ptr(), N, M, N, K, workspace.data_ptr(), need,
+                                                               nat.current_stream(x.device)),
+                      "i8f_linear_w8a16_small_lora_requests")
+    return out
+
+
+def _bias_arg(bias: Tensor | None, device: torch.device, n: int) -> Tensor | None:
+    if bias is None:
+        return None
+    if bias.numel() != n:
+        raise ValueError(f"bias must have {n} elements, got {bias.numel()}")
+    return bias.to(device).contiguous()
+
+
+def _modulation(v: Tensor | None, name: str, y: Tensor, requests: int) -> Tensor | None:
+    """One row of K values per request ([requests, K]) or one for all ([K])."""
+    if v is None:
+        return None
+    if v.dim() == 1:
+        v = v[None]
+    if v.dim() != 2 or v.shape[1] != y.shape[1] or v.shape[0] not in (1, requests):
+        raise ValueError(f"{name} must be [{y.shape[1]}] or [{requests}, {y.shape[1]}], got {tuple(v.shape)}")
+    v = v.to(device=y.device, dtype=y.dtype)
+    if v.stride(1) != 1 and v.shape[1] > 1:
+        v = v.contiguous()
+    if v.shape[0] > 1 and v.stride(0) < v.shape[1]:
+        v = v.contiguous()
+    return v
+
+
+def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm, post_weight, norm, weight, scale, shift, eps,
+                         x_out, want_h, want_q):
+    nat.require_device(y.device)
+    if x.dim() != 2 or y.dim() != 2 or x.shape != y.shape or x.device != y.device:
+        raise ValueError(f"x and y must be 2-D tensors of one shape on one device, got {tuple(x.shape)} and {tuple(y.shape)}")
+    if y.dtype not in (torch.bfloat16, torch.float16) or x.dtype not in (y.dtype, torch.float32):
+        raise ValueError(f"y must be bf16 or fp16 and x of the same type or fp32, got {y.dtype} and {x.dtype}")
+    if post_norm not in nat.NORM_CODE or norm not in ("rms", "layer"):
+        raise ValueError("post_norm is None, 'rms' or 'layer'; norm is 'rms' or 'layer'")
+    M, K = y.shape
+    requests = 1
+    if rows is not None:
+        if rows.device != y.device or rows.total != M:
+            raise ValueError(f"the row plan is for {rows.total} rows on {rows.device}, the call has {M} on {y.device}")
+        requests = rows.requests
+    given = x
+    x, y = _rows(x), _rows(y)
+    vectors = [_modulation(v, name, y, requests) for v, name in ((gate, "gate"), (scale, "scale"), (shift, "shift"))]
+    weights = []
+    for v, name in ((post_weight, "post_weight"), (weight, "weight")):
+        if v is not None and v.numel() != K:
+            raise ValueError(f"{name} must have {K} elements")
+        weights.append(None if v is None else v.reshape(-1).to(device=y.device, dtype=y.dtype).contiguous())
+    if x_out is None:
+        x_out = torch.empty((M, K), dtype=x.dtype, device=x.device)
+    elif x_out.shape != (M, K) or x_out.dtype != x.dtype or x_out.device != x.device or (K > 1 and x_out.stride(1) != 1) or (
+            M > 1 and x_out.stride(0) < K):
+        raise ValueError("x_out must have x's shape, type and device, rows of unit inner stride that do not overlap")
+    elif x_out is given:
+        x = x_out
+    h = torch.empty((M, K), dtype=y.dtype, device=y.device) if want_h else None
+    q = torch.empty((M, K), dtype=torch.int8, device=y.device) if want_q else None
+    q_scale = torch.empty((M, 1), dtype=torch.float32, device=y.device) if want_q else None
+    if M and K:
+        # one vector for all rows: a pitch that the row plan's request index multiplies is not used with row_request NULL
+        shared = all(v is None or v.shape[0] == 1 for v in vectors)
+        if not shared:
+            vectors = [v if v is None or v.shape[0] == requests else v.expand(requests, K).contiguous() for v in vectors]
+        g, s, t = vectors
+        with _on(y.device):
+            nat.check(nat.load().i8f_gated_residual_norm(
+                x.data_ptr(), _code(x.dtype), _ld(x), y.data_ptr(), _code(y.dtype), _ld(y), M, K,
+                None if shared else rows.native.row_request, nat.ptr(g), _ld(g) if g is not None else 0, 1 if gate_tanh else 0,
+                float(residual_scale), nat.NORM_CODE[post_norm], nat.ptr(weights[0]), nat.NORM_CODE[norm], nat.ptr(weights[1]),
+                nat.ptr(s), _ld(s) if s is not None else 0, nat.ptr(t), _ld(t) if t is not None else 0, float(eps),
+                x_out.data_ptr(), _ld(x_out), nat.ptr(h), K, nat.ptr(q), K, nat.ptr(q_scale), nat.current_stream(y.device)),
+                "i8f_gated_residual_norm")
+    return x_out, h, q, q_scale
+
+
+def gated_residual_norm(x: Tensor, y: Tensor, gate: Tensor | None = None, *, rows: RequestRows | None = None, gate_tanh: bool = False,
+                        residual_scale: float = 1.0, post_norm: str | None = None, post_weight: Tensor | None = None,
+                        norm: str = "rms", weight: Tensor | None = None, scale: Tensor | None = None, shift: Tensor | None = None,
+                        eps: float = 1e-6, x_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """The residual stream after a block and the input of the next, in one pass over x and y [M,K]:
+
+        x_new = residual_scale * x + g * post_norm(y) * post_weight          g = gate, or tanh(gate) with `gate_tanh`
+        h     = norm(x_new) * weight * (1 + scale) + shift
+
+    post_norm: None, "rms" or "layer" (without affine part); norm: "rms" or "layer".  gate, scale and shift are [K] for all
+    rows or [requests, K] with the row plan `rows` (row slices of a wider matrix are read in place); they and the weights
+    [K] are taken in y's dtype (bf16 or fp16).  x is in y's dtype or fp32.  Everything in between is fp32 and h comes from
+    the unrounded x_new.  Returns (x_new, h); `x_out` (it may be x) receives x_new.  At most 16384 columns."""
+    x_new, h, _, _ = _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm, post_weight, norm, weight, scale,
+                                          shift, eps, x_out, True, False)
+    return x_new, h
+
+
+def quantize_rowwise_gated_residual_norm(x: Tensor, y: Tensor, gate: Tensor | None = None, *, rows: RequestRows | None = None,
+                                         gate_tanh: bool = False, residual_scale: float = 1.0, post_norm: str | None = None,
+                                         post_weight: Tensor | None = None, norm: str = "rms", weight: Tensor | None = None,
+                                         scale: Tensor | None = None, shift: Tensor | None = None, eps: float = 1e-6,
+                                         x_out: Tensor | None = None, return_h: bool = False):
+    """gated_residual_norm whose h is turned into per-token int8 for the quantised linear that follows, without being
+    rounded to 16 bits first.  Returns (x_new, q int8 [M,K], row_scale fp32 [M,1]) and, if asked, h in y's dtype as well
+    (the input of the adapters beside that linear)."""
+    x_new, h, q, q_scale = _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm, post_weight, norm, weight,
+                                                scale, shift, eps, x_out, return_h, True)
+    return (x_new, q, q_scale, h) if return_h else (x_new, q, q_scale)
 
 
 def lora_merge_sr_(w: Tensor, w_scale, up: Tensor, down: Tensor, lora_scale: float, hadamard: bool = False,

@@ -294,6 +294,75 @@ int i8f_lora_up(const void* t, int64_t ldt, const void* lora_b, int64_t ldb,
 int i8f_lora_up_add(const void* t, int64_t ldt, const void* lora_b, int64_t ldb,
                     void* y, int64_t ldy, int dtype, int64_t M, int64_t N, int64_t r, void* stream);
 
+/* ---- A batch whose rows belong to several requests ------------------------------------------------------------
+ * None of the entry points below has a counterpart in the reference, which has one LoRA composition and one set of
+ * modulation vectors for the whole batch.
+ *
+ * Which rows belong to which request and adapter.  The struct is host memory, read during the call only; the arrays are
+ * device memory.  Build it once per batch and hand it to every layer of the step (adapters.RequestRows of the package
+ * does).  The library trusts the arrays (they are on the device): they must describe exactly `rows` rows, and every
+ * adapter index must be -1 (none) or at most `max_adapter`. */
+typedef struct i8f_request_rows {
+    int64_t rows;               /* rows of the batch, M */
+    const int32_t* row_adapter; /* [rows]: index into the bank of adapters, -1: none */
+    const int32_t* row_request; /* [rows]: request of the row (gated_residual_norm) */
+    const int32_t* chunks;      /* [n_chunks][4]: first row, row count (1..4), adapter or -1, 0; the chunks cover every row once */
+    int64_t n_chunks;
+    int32_t max_adapter;        /* largest adapter index in use, -1 if none */
+} i8f_request_rows;
+
+/* Down projection, one adapter per request: t [M,r] = round(x[m] @ bank_a[adapter(m)]^T), zeros on rows without an
+ * adapter.  bank_a [adapters, r, K] contiguous; x, bank_a and t in `dtype` (I8F_BF16 or I8F_F16), fp32 accumulation.
+ * r a multiple of 8 up to 1024, K and the pitches multiples of 8, pointers 16-byte aligned. */
+int i8f_lora_down_requests(const void* x, int64_t ldx, const void* bank_a, int64_t adapters, int64_t r,
+                           const i8f_request_rows* rows, void* t, int64_t ldt, int dtype, int64_t M, int64_t K, void* stream);
+
+/* Shared int8 projection with one adapter per request:
+ *   I8F_EPI_SINGLE:  out = round(dequant (+bias) + t[m] @ bank_b[adapter(m)]^T), everything in fp32 up to one rounding
+ *   I8F_EPI_PYTORCH: out = round(round(dequant (+bias)) + round(t[m] @ bank_b[adapter(m)]^T)), the roundings of
+ *                    i8f_linear_w8a8_lora
+ * bank_b [adapters, N, r] contiguous in out_dtype, t from i8f_lora_down_requests; the other arguments as in
+ * i8f_linear_w8a8.  `workspace`: i8f_lora_requests_workspace_bytes of device memory, 16-byte aligned. */
+size_t i8f_lora_requests_workspace_bytes(const i8f_request_rows* rows, int64_t N);
+int i8f_linear_w8a8_lora_requests(const int8_t* a, int64_t lda, const float* a_scale,
+                                  const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
+                                  const void* bias, int bias_dtype, const void* t, int64_t ldt, const void* bank_b,
+                                  int64_t adapters, int64_t r, const i8f_request_rows* rows,
+                                  void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int epilogue_order,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* The form for at most 16 rows (single tokens), activations not quantised:
+ *   out = round(w_scale * (x @ w^T) + bias + round(x[m] @ bank_a[a]^T) @ bank_b[a]^T), a = adapter(m)
+ * in fp32 up to the one rounding of the result (and that of the low-rank intermediate).  Arguments as in
+ * i8f_linear_w8a16_small; the banks as above, in x_dtype. */
+size_t i8f_linear_w8a16_small_lora_requests_workspace_bytes(const i8f_request_rows* rows, int64_t N, int64_t r);
+int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw,
+                                         const float* w_scale, int w_scale_mode, const void* bias, int bias_dtype,
+                                         const void* bank_a, const void* bank_b, int64_t adapters, int64_t r,
+                                         const i8f_request_rows* rows, void* out, int64_t ldo,
+                                         int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Norm kinds: v / sqrt(mean(v^2) + eps) and (v - mean(v)) / sqrt(var(v) + eps) over a row. */
+#define I8F_NORM_NONE 0
+#define I8F_NORM_RMS 1
+#define I8F_NORM_LAYER 2
+
+/* Gated residual update between two norms, per row m of request q(m) = row_request[m] (NULL: 0 for every row):
+ *   x_out = residual_scale * x + g * post_norm(y) * post_weight       g = gate[q] or, with gate_tanh, tanh(gate[q])
+ *   h     = norm(x_out) * weight * (1 + scale[q]) + shift[q]
+ * fp32 throughout; h comes from the unrounded x_out, so each output is rounded once.  x, x_out [M,K] in x_dtype
+ * (y_dtype or I8F_F32); y, h and all vectors in y_dtype (I8F_BF16 or I8F_F16).  gate, scale, shift: [requests, K] with
+ * pitches ldg, lds, ldt, each may be NULL (1, 0, 0), as may the weights [K].  h [M,K] and the per-token int8 form of h
+ * (q [M,K], row_scale [M] as in i8f_quant_rowwise) may be asked for separately or both; NULL: not wanted.  x_out may be x.
+ * K at most 16384; rows of any length, pitch and alignment (16-byte aligned rows of a multiple of 8 elements are read
+ * and written in 16-byte pieces). */
+int i8f_gated_residual_norm(const void* x, int x_dtype, int64_t ldx, const void* y, int y_dtype, int64_t ldy,
+                            int64_t M, int64_t K, const int32_t* row_request, const void* gate, int64_t ldg, int gate_tanh,
+                            float residual_scale, int post_norm, const void* post_weight, int norm, const void* weight,
+                            const void* scale, int64_t lds, const void* shift, int64_t ldt, float eps,
+                            void* x_out, int64_t ldxo, void* h, int64_t ldh, int8_t* q, int64_t ldq, float* row_scale,
+                            void* stream);
+
 /* Stochastic-rounding merge of a low-rank update into int8 weights, in place:
  *   delta = (up [N,r] @ down [r,K]) * lora_scale            (fp32, j ascending)
  *   hadamard128: delta <- delta rotated per 128-block of K   (fp32)

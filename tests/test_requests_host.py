@@ -1,0 +1,140 @@
+"""The host side of a batch of requests: the row plan, the bank of adapters, and what the entry points refuse (no GPU)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+
+def tables(rows):
+    """row_adapter, row_request and chunks of a plan made on the CPU, read back through the struct the library gets."""
+    n = rows.native
+
+    def at(ptr, count):
+        return np.ctypeslib.as_array(ctypes.cast(ptr, ctypes.POINTER(ctypes.c_int32)), (count,)).copy() if count else np.zeros(0, np.int32)
+
+    return at(n.row_adapter, n.rows), at(n.row_request, n.rows), at(n.chunks, 4 * n.n_chunks).reshape(-1, 4)
+
+
+@pytest.mark.parametrize("lengths,adapters", [
+    ([1], None), ([1], [3]), ([0, 5, 0], [0, 1, 2]), ([1] * 9, [0, 0, 0, 0, 0, 1, -1, -1, 1]), ([257, 3, 0, 255], [2, -1, 5, 2]),
+    ([4, 4, 1, 300], [1, 1, 1, 0]), ([0, 0], [0, 0]), ([1000], [-1]),
+])
+def test_row_plan_describes_every_row_once(pkg, lengths, adapters):
+    rows = pkg.adapters.RequestRows(lengths, adapters, device="cpu")
+    want_adapter = [a for n, a in zip(lengths, adapters or [-1] * len(lengths)) for _ in range(n)]
+    want_request = [i for i, n in enumerate(lengths) for _ in range(n)]
+    row_adapter, row_request, chunks = tables(rows)
+    assert rows.total == rows.native.rows == sum(lengths) and rows.requests == len(lengths)
+    assert row_adapter.tolist() == want_adapter and row_request.tolist() == want_request
+    assert rows.native.max_adapter == max(want_adapter, default=-1)
+    covered = []
+    for first, count, adapter, _ in chunks.tolist():
+        assert 1 <= count <= 4 and all(want_adapter[first + i] == adapter for i in range(count))
+        covered += range(first, first + count)
+    assert covered == list(range(sum(lengths)))
+    for ptr in (rows.native.row_adapter, rows.native.row_request, rows.native.chunks):
+        assert ptr % 16 == 0
+
+
+@pytest.mark.parametrize("lengths,adapters", [([], None), ([-1], None), ([2, 3], [0]), ([2], [-2]), ([2], [1 << 20]), ([1 << 30, 1 << 30], None)])
+def test_row_plan_refuses(pkg, lengths, adapters):
+    with pytest.raises(ValueError):
+        pkg.adapters.RequestRows(lengths, adapters, device="cpu")
+
+
+def test_stack_adapters_pads_ranks_and_scales(pkg):
+    g = torch.Generator().manual_seed(1)
+    factors = [(torch.randn(r, 32, generator=g), torch.randn(24, r, generator=g), s) for r, s in ((3, 0.5), (8, 1.0), (11, 2.0))]
+    a, b = pkg.adapters.stack_adapters(factors + [(factors[0][0], factors[0][1])], torch.float32, "cpu")
+    assert a.shape == (4, 16, 32) and b.shape == (4, 24, 16) and a.is_contiguous() and b.is_contiguous()
+    for i, (down, up, s) in enumerate(factors):
+        torch.testing.assert_close(b[i] @ a[i], up @ down * s, rtol=0, atol=11 * 2 ** -22 * float((up.abs() @ down.abs()).max()) * s)
+        assert not a[i, down.shape[0]:].any() and not b[i, :, down.shape[0]:].any()
+    assert torch.equal(a[3, :3], factors[0][0])
+    with pytest.raises(ValueError):
+        pkg.adapters.stack_adapters([], torch.float32, "cpu")
+    with pytest.raises(ValueError):
+        pkg.adapters.stack_adapters([factors[0][:2], (torch.zeros(4, 31), torch.zeros(24, 4))], torch.float32, "cpu")
+    with pytest.raises(ValueError):
+        pkg.adapters.stack_adapters([(torch.zeros(4, 32), torch.zeros(24, 5))], torch.float32, "cpu")
+
+
+def test_cpu_tensors_are_rejected(pkg):
+    rows = pkg.adapters.RequestRows([4], [0], device="cpu")
+    F, E = pkg.functional, pkg._native.NativeLibraryError
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(32, 64, dtype=torch.int8)
+    a, b = torch.zeros(1, 8, 64, dtype=torch.bfloat16), torch.zeros(1, 32, 8, dtype=torch.bfloat16)
+    for call in (lambda: F.linear_lora_requests(x, w, 1.0, None, a, b, rows, torch.bfloat16),
+                 lambda: F.linear_small_batch_lora_requests(x, w, 1.0, None, a, b, rows),
+                 lambda: F.lora_down_requests(x, a, rows),
+                 lambda: F.gated_residual_norm(x, x), lambda: F.quantize_rowwise_gated_residual_norm(x, x)):
+        with pytest.raises(E, match="CUDA"):
+            call()
+
+
+P = ctypes.c_void_p(4096)        # an aligned address that no refused call ever reads
+ODD = ctypes.c_void_p(4098)
+
+
+def native_rows(pkg, rows=8, max_adapter=1, **kw):
+    s = pkg._native.RequestRowsStruct(rows=rows, row_adapter=4096, row_request=4096, chunks=4096, n_chunks=2, max_adapter=max_adapter)
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return ctypes.byref(s)
+
+
+def test_abi_refuses_bad_adapter_calls(pkg):
+    nat = pkg._native
+    lib = nat.load()
+
+    def down(x=P, ldx=64, bank=P, adapters=2, r=16, rows=None, t=P, ldt=16, dt=nat.I8F_BF16, M=8, K=64):
+        return lib.i8f_lora_down_requests(x, ldx, bank, adapters, r, rows or native_rows(pkg), t, ldt, dt, M, K, None)
+
+    for want, kw in ((-1, dict(M=9)), (-1, dict(rows=native_rows(pkg, chunks=None))), (-1, dict(rows=native_rows(pkg, n_chunks=0))),
+                     (-3, dict(dt=nat.I8F_F32)), (-1, dict(adapters=1)), (-1, dict(bank=None)), (-3, dict(r=12)), (-3, dict(r=0)),
+                     (-3, dict(r=1032, ldt=1032)), (-2, dict(bank=ODD)), (-1, dict(x=None)), (-1, dict(t=None)), (-1, dict(ldx=56)),
+                     (-1, dict(ldt=8)), (-2, dict(x=ODD)), (-2, dict(t=ODD)), (-2, dict(K=60)), (-2, dict(ldx=68)), (-2, dict(ldt=20))):
+        assert down(**kw) == want, kw
+        assert nat.last_error()
+    assert down(M=0, rows=native_rows(pkg, rows=0)) == 0
+
+    def gemm(t=P, ldt=16, bank=P, adapters=2, r=16, rows=None, dt=nat.I8F_BF16, M=8, N=64, K=64, order=1, ws=P, ws_bytes=1 << 20, a=P):
+        return lib.i8f_linear_w8a8_lora_requests(a, K, P, P, K, P, 0, None, 0, t, ldt, bank, adapters, r, rows or native_rows(pkg), P, dt, N,
+                                                 M, N, K, order, ws, ws_bytes, None)
+
+    for want, kw in ((-1, dict(M=9)), (-3, dict(dt=nat.I8F_F32)), (-1, dict(adapters=1)), (-3, dict(r=20)), (-1, dict(t=None)), (-1, dict(ldt=8)),
+                     (-2, dict(t=ODD)), (-2, dict(bank=ODD)), (-6, dict(ws=None)), (-6, dict(ws_bytes=64)), (-2, dict(ws=ODD))):
+        assert gemm(**kw) == want, kw
+        assert nat.last_error()
+    assert gemm(M=0, rows=native_rows(pkg, rows=0)) == 0
+    assert gemm(N=0) == 0
+
+    def small(x=P, dt=nat.I8F_BF16, ldx=64, bank_a=P, bank_b=P, adapters=2, r=16, rows=None, M=8, N=64, K=64, ws=P, ws_bytes=1 << 20):
+        return lib.i8f_linear_w8a16_small_lora_requests(x, dt, ldx, P, K, P, 0, None, 0, bank_a, bank_b, adapters, r,
+                                                        rows or native_rows(pkg, rows=M), P, N, M, N, K, ws, ws_bytes, None)
+
+    for want, kw in ((-1, dict(rows=native_rows(pkg, rows=7))), (-3, dict(M=17)), (-3, dict(dt=nat.I8F_F32)), (-1, dict(adapters=1)), (-3, dict(r=4)),
+                     (-1, dict(bank_a=None)), (-2, dict(bank_b=ODD)), (-2, dict(K=72, ldx=72)), (-6, dict(ws=None)), (-6, dict(ws_bytes=64)),
+                     (-1, dict(x=None))):
+        assert small(**kw) == want, kw
+        assert nat.last_error()
+
+
+def test_abi_refuses_bad_norm_calls(pkg):
+    nat = pkg._native
+    lib = nat.load()
+
+    def call(x=P, xdt=nat.I8F_BF16, ldx=64, y=P, ydt=nat.I8F_BF16, ldy=64, M=8, K=64, gate=P, ldg=64, post=1, norm=1, scale=None, lds=0,
+             shift=None, ldt=0, eps=1e-6, xo=P, ldxo=64, h=P, ldh=64, q=None, ldq=0, rs=None):
+        return lib.i8f_gated_residual_norm(x, xdt, ldx, y, ydt, ldy, M, K, None, gate, ldg, 0, 1.0, post, None, norm, None, scale, lds, shift,
+                                           ldt, eps, xo, ldxo, h, ldh, q, ldq, rs, None)
+
+    for want, kw in ((-3, dict(ydt=nat.I8F_F32)), (-3, dict(xdt=nat.I8F_F16)), (-1, dict(M=-1)), (-1, dict(K=-8)),
+                     (-3, dict(K=16392, ldx=16392, ldy=16392, ldg=16392, ldxo=16392, ldh=16392)), (-1, dict(post=3)), (-1, dict(norm=0)),
+                     (-1, dict(eps=-1.0)), (-1, dict(x=None)), (-1, dict(y=None)), (-1, dict(xo=None)), (-1, dict(h=None)),
+                     (-1, dict(h=None, q=P, ldq=64)), (-1, dict(ldx=63)), (-1, dict(ldy=63)), (-1, dict(ldxo=63)), (-1, dict(ldh=63)),
+                     (-1, dict(q=P, ldq=63, rs=P)), (-1, dict(ldg=63)), (-1, dict(scale=P, lds=63)), (-1, dict(shift=P, ldt=63))):
+        assert call(**kw) == want, kw
+        assert nat.last_error()
+    assert call(M=0) == 0 and call(K=0) == 0
