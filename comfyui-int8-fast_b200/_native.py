@@ -30,8 +30,9 @@ class NativeLibraryError(RuntimeError):
 
 class RequestRowsStruct(ctypes.Structure):
     """i8f_request_rows of the C header."""
-    _fields_ = [("rows", c_int64), ("row_adapter", c_void_p), ("row_request", c_void_p), ("chunks", c_void_p),
-                ("n_chunks", c_int64), ("max_adapter", ctypes.c_int32)]
+    _fields_ = [("rows", c_int64), ("row_adapter", c_void_p), ("row_request", c_void_p), ("tiles", c_void_p), ("slots", c_void_p),
+                ("chunks", c_void_p), ("n_dense", c_int64), ("n_chunks", c_int64), ("addend_rows", c_int64),
+                ("max_adapter", ctypes.c_int32)]
 
 
 _ROWS = ctypes.POINTER(RequestRowsStruct)
@@ -90,6 +91,10 @@ _PROTOTYPES = {
     "i8f_linear_w8a8_lora_requests": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int,
                                               c_void_p, c_int64, c_void_p, c_int64, c_int64, _ROWS, c_void_p, c_int, c_int64,
                                               c_int64, c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "i8f_linear_lora_requests_workspace_bytes": (c_size_t, [_ROWS, c_int64, c_int64, c_int64, c_int, c_int]),
+    "i8f_linear_lora_requests": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int,
+                                         c_void_p, c_void_p, c_int64, c_int64, _ROWS, c_void_p, c_int64, c_int64, c_int64,
+                                         c_int64, c_int, c_void_p, c_size_t, c_void_p]),
     "i8f_linear_w8a16_small_lora_requests_workspace_bytes": (c_size_t, [_ROWS, c_int64, c_int64]),
     "i8f_linear_w8a16_small_lora_requests": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int,
                                                      c_void_p, c_void_p, c_int64, c_int64, _ROWS, c_void_p, c_int64, c_int64,
@@ -108,7 +113,7 @@ _PROTOTYPES = {
 
 _lock = threading.Lock()
 _lib = None
-_device_ok: set[int] = set()
+device_ok: set[int] = set()
 
 
 def exported_symbols() -> list[str]:
@@ -155,11 +160,11 @@ def require_device(device: torch.device) -> None:
     if device.type != "cuda":
         raise NativeLibraryError(f"INT8 Fast (B200) kernels need CUDA tensors, got a tensor on {device}")
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    if idx in _device_ok:
+    if idx in device_ok:
         return
     with torch.cuda.device(idx):
         check(load().i8f_device_check(), "i8f_device_check")
-    _device_ok.add(idx)
+    device_ok.add(idx)
 
 
 def device_status(reset: bool = True) -> int:

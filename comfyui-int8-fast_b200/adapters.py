@@ -15,6 +15,9 @@ from torch import Tensor
 
 from . import _native as nat
 
+TILE_ROWS = 256     # rows of a tile of the projection
+TILE_SLOTS = 8      # adapters that a tile may have to be run on the tensor cores
+DENSE_ROWS = 256    # batches of fewer rows are chunked throughout
 CHUNK_ROWS = 4      # rows of one adapter that a small work item of the kernels takes together
 
 
@@ -45,32 +48,60 @@ class RequestRows:
         self.max_adapter = int(used.max()) if used.size else -1
         row_adapter = np.repeat(a, n)
         row_request = np.repeat(np.arange(n.size), n)
-        chunks = self._chunks(row_adapter)
-        parts = [row_adapter, row_request, chunks.reshape(-1)]
+        tiles, slots, chunks, addend_rows = self._plan(row_adapter)
+        parts = [row_adapter, row_request, tiles.reshape(-1), slots.reshape(-1), chunks.reshape(-1)]
         offsets = np.cumsum([0] + [-(-p.size // 4) * 4 for p in parts])      # 16-byte aligned tables in one buffer
         packed = np.zeros(max(int(offsets[-1]), 4), dtype=np.int32)
         for o, p in zip(offsets, parts):
             packed[o:o + p.size] = p
         self._tables = torch.from_numpy(packed).to(device)
         self.device = self._tables.device
-        base = self._tables.data_ptr()
-        self.native = nat.RequestRowsStruct(rows=self.total, row_adapter=base + 4 * int(offsets[0]),
-                                            row_request=base + 4 * int(offsets[1]), chunks=base + 4 * int(offsets[2]),
-                                            n_chunks=chunks.shape[0], max_adapter=self.max_adapter)
+        at = [self._tables.data_ptr() + 4 * int(o) for o in offsets]
+        self.native = nat.RequestRowsStruct(rows=self.total, row_adapter=at[0], row_request=at[1], tiles=at[2], slots=at[3], chunks=at[4],
+                                            n_dense=int((tiles[:, 2] < 0).sum()), n_chunks=chunks.shape[0], addend_rows=addend_rows,
+                                            max_adapter=self.max_adapter)
         self.native_ptr = ctypes.byref(self.native)
+        self.row_request_ptr = at[1]
+        self.workspace_bytes: dict = {}      # sizes the library asks for, by layer shape
 
     @staticmethod
-    def _chunks(row_adapter: np.ndarray) -> np.ndarray:
-        """[n, 4] first row, row count, adapter, 0: runs of rows with one adapter, cut into pieces of CHUNK_ROWS."""
-        if row_adapter.size == 0:
-            return np.zeros((0, 4), dtype=np.int64)
-        starts = np.concatenate([[0], np.flatnonzero(np.diff(row_adapter)) + 1])
-        ends = np.concatenate([starts[1:], [row_adapter.size]])
+    def _plan(row_adapter: np.ndarray):
+        """tiles [n, 4], slots [n, 12], chunks [n, 4] and the rows of the addend, as i8f_request_rows describes them."""
+        rows = row_adapter.size
+        n_tiles = -(-rows // TILE_ROWS)
+        tile_of = np.arange(rows) // TILE_ROWS
+        # one slot per (tile, adapter), in that order, with a bit for each of its rows
+        with_adapter = np.flatnonzero(row_adapter >= 0)
+        key = (tile_of[with_adapter] << 20) | row_adapter[with_adapter]
+        keys, slot_of = np.unique(key, return_inverse=True)
+        slot_tile, slot_adapter = keys >> 20, keys & ((1 << 20) - 1)
+        per_tile = np.bincount(slot_tile, minlength=n_tiles)
+        dense = (per_tile <= TILE_SLOTS) if rows >= DENSE_ROWS else np.zeros(n_tiles, dtype=bool)
+        keep = dense[slot_tile]
+        bits = np.zeros((keys.size, TILE_ROWS), dtype=bool)
+        bits[slot_of, with_adapter % TILE_ROWS] = True
+        slots = np.zeros((int(keep.sum()), 12), dtype=np.int32)
+        slots[:, 0] = slot_adapter[keep]
+        slots[:, 4:] = np.packbits(bits[keep], axis=1, bitorder="little").view(np.int32)
+        tiles = np.zeros((n_tiles, 4), dtype=np.int64)
+        tiles[:, 1] = np.where(dense, per_tile, 0)
+        tiles[:, 0] = np.cumsum(tiles[:, 1]) - tiles[:, 1]
+        tiles[:, 2] = np.where(dense, -1, (np.cumsum(~dense) - 1) * TILE_ROWS)
+        last = max(0, n_tiles * TILE_ROWS - rows) if n_tiles and not dense[-1] else 0
+        addend_rows = int((~dense).sum()) * TILE_ROWS - last
+        # runs of rows with one adapter in the chunked tiles, cut into pieces of CHUNK_ROWS
+        left = np.flatnonzero(~dense[tile_of]) if rows else np.zeros(0, dtype=np.int64)
+        if left.size == 0:
+            return tiles, slots, np.zeros((0, 4), dtype=np.int64), addend_rows
+        cut = (np.diff(left) != 1) | (np.diff(row_adapter[left]) != 0) | (np.diff(tile_of[left]) != 0)
+        starts = np.concatenate([[0], np.flatnonzero(cut) + 1])
+        ends = np.concatenate([starts[1:], [left.size]])
         pieces = -(-(ends - starts) // CHUNK_ROWS)
         run = np.repeat(np.arange(starts.size), pieces)
         first = starts[run] + CHUNK_ROWS * (np.arange(run.size) - np.repeat(np.cumsum(pieces) - pieces, pieces))
         count = np.minimum(CHUNK_ROWS, ends[run] - first)
-        return np.stack([first, count, row_adapter[first], np.zeros_like(first)], axis=1)
+        row = left[first]
+        return tiles, slots, np.stack([row, count, row_adapter[row], tiles[tile_of[row], 2] + row % TILE_ROWS], axis=1), addend_rows
 
 
 def stack_adapters(factors: Sequence[tuple[Tensor, Tensor] | tuple[Tensor, Tensor, float]], dtype: torch.dtype,

@@ -37,6 +37,7 @@
 
 #include "host_common.h"
 #include "ptx_sm100.cuh"
+#include "tensor_maps.h"
 
 namespace i8f {
 namespace {
@@ -44,10 +45,9 @@ namespace {
 constexpr int kBM = 128;            // rows of A per CTA == TMEM lanes
 constexpr int kStageRowBytes = 128; // one 128-byte swizzle span of K per stage
 
-enum Kind : int { kKindI8 = 0, kKindBF16 = 1, kKindF16 = 2 };
 enum EpiMode : int { kEpiI32 = 0, kEpiDequant = 1, kEpiCast = 2, kEpiAccum = 3 };
 // what joins the product in the epilogue (a template parameter, so that the plain kernels carry none of it)
-enum Extra : int { kExtraNone = 0, kExtraLora = 1, kExtraAddend = 2 };
+enum Extra : int { kExtraNone = 0, kExtraLora = 1, kExtraAddend = 2, kExtraRequests = 3 };
 
 // status codes written by bounded waits
 enum : int { kStEmptyWait = 101, kStFullWait = 102, kStAccEmptyWait = 103, kStAccFullWait = 104 };
@@ -77,10 +77,16 @@ struct GemmParams {
     int out_col0; // column of the destination matrices at which this launch's block starts
     int k_split;  // 1, or 2: the two CTAs of a cluster each take half of K for the same tile (single-CTA kernels)
     int* status;
-    // kExtraAddend: fp32 [M, ld_addend], added before the rounding to rows whose row_adapter is not negative
+    // kExtraAddend: fp32 [M, ld_addend], added before the rounding to rows whose row_adapter is not negative.
+    // kExtraRequests: each 256-row tile has either its own run of `slots` (one per adapter in the tile, with the rows that
+    // use it), whose low-rank terms are accumulated in tensor memory, or a place in the addend
     const float* addend;
     long long ld_addend;
     const int* row_adapter;
+    const RequestTile* req_tiles;
+    const RequestSlot* req_slots;
+    int lora_k16;       // 16-element steps of the rank
+    long long lora_n;   // rows of lora_b per adapter
 };
 
 constexpr int kMaxOutputs = 8;
@@ -100,7 +106,7 @@ struct alignas(64) LoraMaps {
 
 template <int BN, bool PAIR, int EXTRA = kExtraNone>
 struct Cfg {
-    static constexpr bool LORA = EXTRA == kExtraLora;
+    static constexpr bool LORA = EXTRA == kExtraLora || EXTRA == kExtraRequests;   // has the low-rank accumulator
     static constexpr int kBRows = PAIR ? BN / 2 : BN;  // rows of B this CTA stages
     static constexpr int kABytes = kBM * kStageRowBytes;
     static constexpr int kBBytes = kBRows * kStageRowBytes;
@@ -137,6 +143,12 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
     const int r = t - group * group_sz;
     m_blk = first_m + r % gm;
     n_blk = r / gm;
+}
+
+__device__ __forceinline__ int tile_m(int t, int tiles_m, int tiles_n) {
+    int m_blk, n_blk;
+    tile_coords(t, tiles_m, tiles_n, m_blk, n_blk);
+    return m_blk;
 }
 
 template <int DT>
@@ -290,7 +302,7 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, long long ro
 #pragma unroll
             for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], cb[j]);
         }
-        if constexpr (EXTRA == kExtraAddend) {
+        if constexpr (EXTRA == kExtraAddend || EXTRA == kExtraRequests) {
             if (single) {   // the low-rank term joins in fp32: one rounding in all
 #pragma unroll
                 for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], __uint_as_float(lv[j]));
@@ -483,7 +495,28 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         phase ^= 1u;
                     }
                 }
-                if constexpr (LORA) {
+                if constexpr (EXTRA == kExtraRequests) {
+                    // the same for each adapter of the tile: t again, and the adapter's slice of the bank
+                    const RequestTile rt = p.req_tiles[m_blk];
+                    for (int s = 0; ok && s < rt.n_slots; ++s) {
+                        const int row_l = static_cast<int>(p.req_slots[rt.slot_begin + s].adapter * p.lora_n) + row_b;
+                        for (int lb = 0; lb < p.lora_k_blocks; ++lb) {
+                            if (!mbar_wait_bounded(empty0 + 8 * stage, phase ^ 1u, abort_flag, p.status, kStEmptyWait)) {
+                                ok = false;
+                                break;
+                            }
+                            const uint32_t a_dst = smem_base + stage * C::kStageBytes;
+                            const uint32_t bar = mapa_cluster(full0 + 8 * stage, 0);
+                            if (leader) mbar_arrive_expect_tx(full0 + 8 * stage, 2 * C::kStageBytes);
+                            tma_load_2d_pair(a_dst, &lora.t, bar, lb * 64, row_a);
+                            tma_load_2d_pair(a_dst + C::kABytes, &lora.b, bar, lb * 64, row_l);
+                            if (++stage == C::kStages) {
+                                stage = 0;
+                                phase ^= 1u;
+                            }
+                        }
+                    }
+                } else if constexpr (LORA) {
                     // the low-rank operands ride the same ring: t rows where A rows go, lora_b rows where W rows go
                     for (int lb = 0; ok && lb < p.lora_k_blocks; ++lb) {
                         if (!mbar_wait_bounded(empty0 + 8 * stage, phase ^ 1u, abort_flag, p.status, kStEmptyWait)) {
@@ -569,6 +602,15 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         if (!mbar_wait_bounded(accempty0 + 8 * (buf ^ 1), prev_phase, abort_flag, p.status, kStAccEmptyWait)) break;
                         tc_fence_after_sync();
                     }
+                    const int n_slots = EXTRA == kExtraRequests ? p.req_tiles[tile_m(t, p.tiles_m, p.tiles_n)].n_slots : 1;
+                    for (int s = 0; ok && s < n_slots; ++s) {
+                    uint32_t off[8] = {};
+                    if constexpr (EXTRA == kExtraRequests) {
+                        // a slot's first step overwrites its rows and leaves the other slots' rows alone
+                        const RequestSlot* slot = p.req_slots + p.req_tiles[tile_m(t, p.tiles_m, p.tiles_n)].slot_begin + s;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) off[i] = ~slot->rows[i];
+                    }
                     for (int lb = 0; lb < p.lora_k_blocks; ++lb) {
                         if (!ready && !mbar_wait_bounded(full0 + 8 * stage, phase, abort_flag, p.status, kStFullWait)) {
                             ok = false;
@@ -580,13 +622,21 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         const uint64_t adesc = make_smem_desc_sw128(a_src);
                         const uint64_t bdesc = make_smem_desc_sw128(a_src + C::kABytes);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)   // 16 elements = 32 bytes of the rank per instruction
-                            mma_f16_pair(tmem_base + C::kLoraCol, adesc + 2 * k, bdesc + 2 * k, idesc_lora, (lb | k) != 0 ? 1u : 0u);
+                        for (int k = 0; k < 4; ++k) {   // 16 elements = 32 bytes of the rank per instruction
+                            if constexpr (EXTRA == kExtraRequests) {
+                                if (lb * 4 + k < p.lora_k16)
+                                    mma_f16_pair_masked(tmem_base + C::kLoraCol, adesc + 2 * k, bdesc + 2 * k, idesc_lora,
+                                                        (lb | k) != 0 ? 1u : 0u, off);
+                            } else {
+                                mma_f16_pair(tmem_base + C::kLoraCol, adesc + 2 * k, bdesc + 2 * k, idesc_lora, (lb | k) != 0 ? 1u : 0u);
+                            }
+                        }
                         mma_commit_pair(empty0 + 8 * stage);
                         if (++stage == C::kStages) {
                             stage = 0;
                             phase ^= 1u;
                         }
+                    }
                     }
                     if (!ok) break;
                 }
@@ -660,7 +710,19 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const bool row_ok = row < p.M;
             const float row_scale = (dequant && row_ok) ? __ldg(p.a_scale + row) : 0.f;
             bool has_addend = false;
-            if constexpr (EXTRA == kExtraAddend) has_addend = row_ok && __ldg(p.row_adapter + row) >= 0;
+            bool low_rank_row = false;      // the row's term is in tensor memory
+            const float* addend_row = nullptr;
+            if constexpr (EXTRA == kExtraAddend) {
+                has_addend = row_ok && __ldg(p.row_adapter + row) >= 0;
+                addend_row = p.addend + row * p.ld_addend;
+            }
+            if constexpr (EXTRA == kExtraRequests) {
+                const bool with_adapter = row_ok && __ldg(p.row_adapter + row) >= 0;
+                const int addend_row0 = p.req_tiles[m_blk].addend_row;
+                has_addend = with_adapter && addend_row0 >= 0;
+                low_rank_row = with_adapter && addend_row0 < 0;
+                addend_row = p.addend + (addend_row0 + (row - static_cast<long long>(m_blk) * C::kTileM)) * p.ld_addend;
+            }
             // this warp's share of the tile's 32-column chunks (all of them with four epilogue warps), cut at N
             constexpr int kChunksPerWarp = (BN / 32) / (C::kEpiWarps / 4);
             const int c_first = ((warp - 2) >> 2) * kChunksPerWarp;
@@ -710,7 +772,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 uint32_t lv[EXTRA != kExtraNone ? 32 : 1];
                 if constexpr (LORA) tmem_ld_32x32(t_lora + c * 32, lv);
                 if constexpr (EXTRA == kExtraAddend) {   // ld_addend is a multiple of 32: a whole chunk is always there
-                    const uint4* src = reinterpret_cast<const uint4*>(p.addend + row * p.ld_addend + col);
+                    const uint4* src = reinterpret_cast<const uint4*>(addend_row + col);
 #pragma unroll
                     for (int g = 0; g < 8; ++g) {
                         const uint4 o = has_addend ? __ldg(src + g) : make_uint4(0u, 0u, 0u, 0u);
@@ -739,6 +801,22 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     __syncwarp();
                 }
                 tmem_ld_wait();
+                if constexpr (EXTRA == kExtraRequests) {   // rows without an adapter: whatever an earlier tile left there is dropped
+                    if (has_addend) {
+                        const uint4* src = reinterpret_cast<const uint4*>(addend_row + col);
+#pragma unroll
+                        for (int g = 0; g < 8; ++g) {
+                            const uint4 o = __ldg(src + g);
+                            lv[4 * g] = o.x;
+                            lv[4 * g + 1] = o.y;
+                            lv[4 * g + 2] = o.z;
+                            lv[4 * g + 3] = o.w;
+                        }
+                    } else if (!low_rank_row) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) lv[j] = 0u;
+                    }
+                }
                 if constexpr (!PAIR) {
                     if (ksplit) {   // + the second CTA's half of K: exact for int32, one more fp32 add for the 16-bit kinds
                         const int row_in_tile = quarter * 32 + lane;
@@ -889,7 +967,7 @@ MapSlot* map_cache_slot(const MapKey& k) {
     return &slots[(h >> 20) % kMapCacheSlots];
 }
 
-int current_device();
+}  // namespace
 
 // K-major [rows, k_elems] matrix, box = one 128-byte span of K x box_rows, 128-byte swizzle.
 int make_operand_map(CUtensorMap* tm, int kind, const void* base, int64_t rows, int64_t k_elems, int64_t ld_elems,
@@ -920,6 +998,8 @@ int make_operand_map(CUtensorMap* tm, int kind, const void* base, int64_t rows, 
     return I8F_OK;
 }
 
+namespace {
+
 // Output [rows, cols] of 16-bit elements, box = 32 columns x 32 rows (one epilogue warp's chunk), 64-byte swizzle.
 int make_out_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t cols, int64_t ld_elems, bool wide = false) {
     const MapKey key{base, rows, cols, ld_elems, wide ? -2 : -1, current_device()};
@@ -945,6 +1025,8 @@ int make_out_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t cols, 
     return I8F_OK;
 }
 
+}  // namespace
+
 int current_device() {
     int dev = 0;
     cudaGetDevice(&dev);
@@ -957,6 +1039,8 @@ int sm_count() {
     if (cached[dev] == 0) cudaDeviceGetAttribute(&cached[dev], cudaDevAttrMultiProcessorCount, dev);
     return cached[dev] > 0 ? cached[dev] : 148;
 }
+
+namespace {
 
 struct Scatter {
     void* const* dests;   // base pointers of the destination matrices ([M, n_total], pitch ld elements)
@@ -973,6 +1057,7 @@ struct LoraOperands {
     int64_t ldb;
     int64_t r;
     int kind;             // kKindBF16 or kKindF16
+    int64_t adapters = 1; // b holds that many [N, r] slices one after the other
 };
 
 template <int KIND, int BN, bool PAIR, int EXTRA = kExtraNone>
@@ -984,8 +1069,10 @@ int launch_gemm(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t 
     if (C::LORA) {
         int rc_l = make_operand_map(&lmaps.t, lo->kind, lo->t, M, lo->r, lo->ldt, kBM);
         if (rc_l != I8F_OK) return rc_l;
-        rc_l = make_operand_map(&lmaps.b, lo->kind, lo->b, N, lo->r, lo->ldb, C::kBRows);
+        rc_l = make_operand_map(&lmaps.b, lo->kind, lo->b, N * lo->adapters, lo->r, lo->ldb, C::kBRows);
         if (rc_l != I8F_OK) return rc_l;
+        p.lora_k16 = static_cast<int>((lo->r + 15) / 16);
+        p.lora_n = N;
         p.lora_k_blocks = static_cast<int>((lo->r + 63) / 64);
         p.lora_bf16 = lo->kind == kKindBF16 ? 1 : 0;
     }
@@ -1268,8 +1355,7 @@ static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, 
                             const float* w_scale, int w_scale_mode, const void* bias, int bias_dtype, void* out,
                             int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int epilogue_order,
                             int add_existing, void* stream, const Scatter* scatter = nullptr, const void* gate = nullptr,
-                            const float* addend = nullptr, int64_t ld_addend = 0, const int* row_adapter = nullptr,
-                            bool check_only = false) {
+                            const RequestTerm* term = nullptr, bool check_only = false) {
     int rc = check_operands(a, lda, w, ldw, 1, M, N, K);
     if (rc != I8F_OK) return rc;
     I8F_REQUIRE(a_scale != nullptr && w_scale != nullptr, I8F_ERR_INVALID_ARG, "NULL scale pointer");
@@ -1296,11 +1382,15 @@ static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, 
     p.gate = gate;
     p.vec_ok = aligned16(out) && (ldo % 8 == 0);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (addend != nullptr) {
-        p.addend = addend;
-        p.ld_addend = ld_addend;
-        p.row_adapter = row_adapter;
-        return launch_gemm_auto<kKindI8, kExtraAddend>(a, lda, w, ldw, M, N, K, p, st);
+    if (term != nullptr) {
+        p.addend = term->addend;
+        p.ld_addend = term->ld_addend;
+        p.row_adapter = term->row_adapter;
+        if (term->tiles == nullptr) return launch_gemm_auto<kKindI8, kExtraAddend>(a, lda, w, ldw, M, N, K, p, st);
+        p.req_tiles = term->tiles;
+        p.req_slots = term->slots;
+        const LoraOperands lo{term->t, term->ldt, term->b, term->r, term->r, out_dtype == I8F_BF16 ? kKindBF16 : kKindF16, term->adapters};
+        return launch_gemm<kKindI8, 256, true, kExtraRequests>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
     }
     return launch_gemm_auto<kKindI8>(a, lda, w, ldw, M, N, K, p, st, scatter);
 }
@@ -1485,12 +1575,11 @@ int i8f_lora_up_add(const void* t, int64_t ldt, const void* lora_b, int64_t ldb,
 
 namespace i8f {
 
-int linear_w8a8_addend(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
-                       int w_scale_mode, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M,
-                       int64_t N, int64_t K, int epilogue_order, const float* addend, int64_t ld_addend, const int* row_adapter,
-                       bool check_only, cudaStream_t stream) {
+int linear_w8a8_requests(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
+                         int w_scale_mode, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M,
+                         int64_t N, int64_t K, int epilogue_order, const RequestTerm& term, bool check_only, cudaStream_t stream) {
     return linear_w8a8_impl(a, lda, a_scale, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, out_dtype, ldo, M, N, K,
-                            epilogue_order, 0, stream, nullptr, nullptr, addend, ld_addend, row_adapter, check_only);
+                            epilogue_order, 0, stream, nullptr, nullptr, &term, check_only);
 }
 
 }  // namespace i8f

@@ -42,14 +42,37 @@ inline int check_launch(const char* what) {
 
 int* device_status_word();  // device address of the status word on the current device, or nullptr
 
-// i8f_linear_w8a8 with an fp32 addend [M, ld_addend] (ld_addend a multiple of 32, 16-byte aligned) on the rows whose
-// row_adapter is not negative; in gemm_tcgen05.cu.  With `check_only` the arguments are checked and nothing is launched, so
-// that a caller can refuse a bad call before it launches what comes first.
-int linear_w8a8_addend(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
-                       int w_scale_mode, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M,
-                       int64_t N, int64_t K, int epilogue_order, const float* addend, int64_t ld_addend, const int* row_adapter,
-                       bool check_only, cudaStream_t stream);
-// The same for at most 16 rows of unquantised activations; in linear_small_m.cu.
+// One 256-row tile of a batch of requests: its run of slots, or (addend_row >= 0) its first row in the fp32 addend.
+struct RequestTile {
+    int slot_begin, n_slots, addend_row, pad;
+};
+constexpr int kMaxTileSlots = 8;      // a tile with more adapters than this is chunked
+// One adapter of a tile and the rows of the tile that use it (bit i of word j: row 32 j + i).
+struct RequestSlot {
+    int adapter, pad[3];
+    uint32_t rows[8];
+};
+
+// The low-rank term of a batch of requests beside the int8 product.  `tiles` NULL: all of it is in `addend`
+// [M, ld_addend]; else the tiles say where theirs comes from.  ld_addend is a multiple of 32, the addend 16-byte aligned.
+struct RequestTerm {
+    const int* row_adapter;
+    const float* addend;
+    int64_t ld_addend;
+    const RequestTile* tiles;
+    const RequestSlot* slots;
+    const void* t;       // [M, r], pitch ldt, in the output type
+    int64_t ldt;
+    const void* b;       // [adapters, N, r]
+    int64_t adapters, r;
+};
+
+// i8f_linear_w8a8 with such a term; in gemm_tcgen05.cu.  With `check_only` the arguments are checked and nothing is
+// launched, so that a caller can refuse a bad call before it launches what comes first.
+int linear_w8a8_requests(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
+                         int w_scale_mode, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M,
+                         int64_t N, int64_t K, int epilogue_order, const RequestTerm& term, bool check_only, cudaStream_t stream);
+// i8f_linear_w8a16_small with an fp32 addend on the rows with an adapter; in linear_small_m.cu.
 int linear_small_addend(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
                         const void* bias, int bias_dtype, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
                         const float* addend, int64_t ld_addend, const int* row_adapter, bool check_only, cudaStream_t stream);

@@ -292,8 +292,8 @@ extern "C" int i8f_gated_residual_norm(const void* x, int x_dtype, int64_t ldx, 
     I8F_REQUIRE(q == nullptr || row_scale != nullptr, I8F_ERR_INVALID_ARG, "%s: q needs row_scale", what);
     I8F_REQUIRE(ldx >= K && ldy >= K && ldxo >= K && (h == nullptr || ldh >= K) && (q == nullptr || ldq >= K), I8F_ERR_INVALID_ARG,
                 "%s: a row pitch is smaller than the row", what);
-    I8F_REQUIRE((gate == nullptr || ldg >= K) && (scale == nullptr || lds >= K) && (shift == nullptr || ldt >= K), I8F_ERR_INVALID_ARG,
-                "%s: a modulation pitch is smaller than the row", what);
+    I8F_REQUIRE((gate == nullptr || ldg == 0 || ldg >= K) && (scale == nullptr || lds == 0 || lds >= K) && (shift == nullptr || ldt == 0 || ldt >= K),
+                I8F_ERR_INVALID_ARG, "%s: a modulation pitch is smaller than the row", what);
     const int xs = dtype_size(x_dtype);
     const bool vec8 = K % 8 == 0 && vec_ok(x, ldx, xs) && vec_ok(x_out, ldxo, xs) && vec_ok(y, ldy, 2) && vec_ok(h, ldh, 2) &&
                       vec_ok(gate, ldg, 2) && vec_ok(scale, lds, 2) && vec_ok(shift, ldt, 2) && vec_ok(post_weight, 0, 2) &&

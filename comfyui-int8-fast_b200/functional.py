@@ -43,9 +43,10 @@ _SAME_DEVICE = contextlib.nullcontext()
 
 
 def _on(device: torch.device):
-    """Context in which `device` is the current one (the C ABI launches on the current device)."""
-    idx = device.index
-    return _SAME_DEVICE if idx is None or idx == torch.cuda.current_device() else torch.cuda.device(idx)
+    """Context in which `device`, a sm_100 device, is the current one (the C ABI launches on the current device)."""
+    if device.type != "cuda" or device.index not in nat.device_ok:
+        nat.require_device(device)
+    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 _WORKSPACE_BYTES: dict = {}
@@ -451,17 +452,16 @@ def _check_requests(rows: RequestRows, x: Tensor, lora_a: Tensor | None, lora_b:
 def lora_down_requests(x: Tensor, lora_a: Tensor, rows: RequestRows) -> Tensor:
     """t [M,r]: row m of x (bf16 or fp16) times the transposed lora_a [adapters, r, K] of the row's adapter, in x's dtype;
     zeros on rows without an adapter."""
-    nat.require_device(x.device)
-    x = _rows(x)
-    M, K = x.shape
-    n, r = _check_requests(rows, x, lora_a, None, x.dtype, K, 0)
-    t = torch.empty((M, r), dtype=x.dtype, device=x.device)
-    if M:
-        with _on(x.device):
+    with _on(x.device):
+        x = _rows(x)
+        M, K = x.shape
+        n, r = _check_requests(rows, x, lora_a, None, x.dtype, K, 0)
+        t = torch.empty((M, r), dtype=x.dtype, device=x.device)
+        if M:
             nat.check(nat.load().i8f_lora_down_requests(x.data_ptr(), _ld(x), lora_a.data_ptr(), n, r, rows.native_ptr, t.data_ptr(), r,
                                                         _code(x.dtype), M, K, nat.current_stream(x.device)),
                       "i8f_lora_down_requests")
-    return t
+        return t
 
 
 def linear_w8a8_lora_requests(q: Tensor, q_scale: Tensor, w: Tensor, w_scale, bias: Tensor | None, t: Tensor, lora_b: Tensor,
@@ -470,30 +470,34 @@ def linear_w8a8_lora_requests(q: Tensor, q_scale: Tensor, w: Tensor, w_scale, bi
     row's own adapter (lora_b [adapters, N, r], t from lora_down_requests; both in out_dtype).
 
     The default order keeps everything in fp32 up to one rounding; EPI_PYTORCH has the roundings of linear_w8a8_lora."""
-    nat.require_device(q.device)
-    q, w, t = _rows(q), _rows(w), _rows(t)
-    M, K = q.shape
-    N = w.shape[0]
-    _check_weight(w, K)
-    n, r = _check_requests(rows, q, None, lora_b, out_dtype, K, N)
-    if t.shape != (M, r) or t.dtype != out_dtype or t.device != q.device:
-        raise ValueError(f"t must be [{M}, {r}] in {out_dtype} on {q.device}")
-    if q_scale.numel() != M or q_scale.dtype != torch.float32:
-        raise ValueError(f"q_scale must be fp32 with one entry per row ({M})")
-    ws, mode = _wscale_arg(w_scale, q.device, N)
-    bias = _bias_arg(bias, q.device, N)
-    out = torch.empty((M, N), dtype=out_dtype, device=q.device)
-    if M and N:
-        with _on(q.device):
+    with _on(q.device):
+        q, w, t = _rows(q), _rows(w), _rows(t)
+        M, K = q.shape
+        N = w.shape[0]
+        _check_weight(w, K)
+        n, r = _check_requests(rows, q, None, lora_b, out_dtype, K, N)
+        if t.shape != (M, r) or t.dtype != out_dtype or t.device != q.device:
+            raise ValueError(f"t must be [{M}, {r}] in {out_dtype} on {q.device}")
+        if q.dtype != torch.int8 or q_scale.numel() != M or q_scale.dtype != torch.float32 or q_scale.device != q.device:
+            raise ValueError(f"q must be int8, q_scale fp32 with one entry per row ({M}) on {q.device}")
+        ws, mode = _wscale_arg(w_scale, q.device, N)
+        bias = _bias_arg(bias, q.device, N)
+        out = torch.empty((M, N), dtype=out_dtype, device=q.device)
+        if M and N:
             lib = nat.load()
-            need = lib.i8f_lora_requests_workspace_bytes(rows.native_ptr, N)
-            workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
-            nat.check(lib.i8f_linear_w8a8_lora_requests(q.data_ptr(), _ld(q), nat.ptr(q_scale.reshape(-1)), w.data_ptr(), _ld(w),
-                                                        ws.data_ptr(), mode, nat.ptr(bias), _code(bias.dtype) if bias is not None else 0,
-                                                        t.data_ptr(), _ld(t), lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(),
-                                                        _code(out_dtype), N, M, N, K, order, workspace.data_ptr(), need,
+            need = rows.workspace_bytes.get(N)
+            if need is None:
+                need = rows.workspace_bytes[N] = lib.i8f_lora_requests_workspace_bytes(rows.native_ptr, N)
+            workspace = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
+            q_scale = q_scale.reshape(-1)
+            q_scale = q_scale if q_scale.is_contiguous() else q_scale.contiguous()
+            nat.check(lib.i8f_linear_w8a8_lora_requests(q.data_ptr(), _ld(q), q_scale.data_ptr(), w.data_ptr(), _ld(w), ws.data_ptr(), mode,
+                                                        bias.data_ptr() if bias is not None else None,
+                                                        _code(bias.dtype) if bias is not None else 0, t.data_ptr(), _ld(t),
+                                                        lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(), _code(out_dtype), N, M,
+                                                        N, K, order, workspace.data_ptr() if need else None, need,
                                                         nat.current_stream(q.device)), "i8f_linear_w8a8_lora_requests")
-    return out
+        return out
 
 
 def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lora_a: Tensor, lora_b: Tensor, rows: RequestRows,
@@ -504,44 +508,61 @@ def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lor
 
     x [M,K] bf16 or fp16, out_dtype the same type.  With `hadamard` the adapters see the rotated activations unless
     `rotated_lora_input` is false, as in the single-adapter forward."""
-    if out_dtype != x.dtype:
-        raise ValueError(f"out_dtype must be the activations' type {x.dtype}, which the adapters share")
-    _check_requests(rows, x, lora_a, lora_b, out_dtype, x.shape[-1], w.shape[0])
     with _on(x.device):
-        if hadamard and rotated_lora_input:
-            q, q_scale, lora_in = quantize_rowwise(x, hadamard=True, return_rotated=True)
-        else:
-            q, q_scale = quantize_rowwise(x, hadamard=hadamard)
-            lora_in = x
-        t = lora_down_requests(lora_in, lora_a, rows)
-        return linear_w8a8_lora_requests(q, q_scale, w, w_scale, bias, t, lora_b, rows, out_dtype, order=order)
+        x, w = _rows(x), _rows(w)
+        M, K = x.shape
+        N = w.shape[0]
+        if out_dtype != x.dtype:
+            raise ValueError(f"out_dtype must be the activations' type {x.dtype}, which the adapters share")
+        _check_weight(w, K)
+        n, r = _check_requests(rows, x, lora_a, lora_b, out_dtype, K, N)
+        ws, mode = _wscale_arg(w_scale, x.device, N)
+        bias = _bias_arg(bias, x.device, N)
+        rotated = 1 if hadamard and rotated_lora_input else 0
+        if rotated and _ld(x) != K:
+            x = x.contiguous()
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        if M and N:
+            lib = nat.load()
+            size = (N, K, r, rotated)
+            need = rows.workspace_bytes.get(size)
+            if need is None:
+                need = rows.workspace_bytes[size] = lib.i8f_linear_lora_requests_workspace_bytes(rows.native_ptr, N, K, r, rotated, rotated)
+            workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
+            nat.check(lib.i8f_linear_lora_requests(x.data_ptr(), _code(x.dtype), _ld(x), 1 if hadamard else 0, rotated, w.data_ptr(),
+                                                   _ld(w), ws.data_ptr(), mode, bias.data_ptr() if bias is not None else None,
+                                                   _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(), lora_b.data_ptr(), n,
+                                                   r, rows.native_ptr, out.data_ptr(), N, M, N, K, order, workspace.data_ptr(), need,
+                                                   nat.current_stream(x.device)), "i8f_linear_lora_requests")
+        return out
 
 
 def linear_small_batch_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lora_a: Tensor, lora_b: Tensor,
                                      rows: RequestRows) -> Tensor:
     """M <= 16 rows (single tokens) of several requests: y = x @ (w * w_scale)^T + bias + (x @ lora_a[a]^T) @ lora_b[a]^T with
     the adapter a of each row, activations not quantised, one rounding to x's dtype (bf16 or fp16)."""
-    nat.require_device(x.device)
-    x, w = _rows(x), _rows(w)
-    M, K = x.shape
-    N = w.shape[0]
-    _check_weight(w, K)
-    n, r = _check_requests(rows, x, lora_a, lora_b, x.dtype, K, N)
-    ws, mode = _wscale_arg(w_scale, x.device, N)
-    bias = _bias_arg(bias, x.device, N)
-    out = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    if M and N:
-        with _on(x.device):
+    with _on(x.device):
+        x, w = _rows(x), _rows(w)
+        M, K = x.shape
+        N = w.shape[0]
+        _check_weight(w, K)
+        n, r = _check_requests(rows, x, lora_a, lora_b, x.dtype, K, N)
+        ws, mode = _wscale_arg(w_scale, x.device, N)
+        bias = _bias_arg(bias, x.device, N)
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        if M and N:
             lib = nat.load()
-            need = lib.i8f_linear_w8a16_small_lora_requests_workspace_bytes(rows.native_ptr, N, r)
+            need = rows.workspace_bytes.get((N, r))
+            if need is None:
+                need = rows.workspace_bytes[(N, r)] = lib.i8f_linear_w8a16_small_lora_requests_workspace_bytes(rows.native_ptr, N, r)
             workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
-            nat.check(lib.i8f_linear_w8a16_small_lora_requests(x.data_ptr(), _code(x.dtype), _ld(x), w.data_ptr(), _ld(w), ws.data_ptr(), mode,
-                                                               nat.ptr(bias), _code(bias.dtype) if bias is not None else 0,
-                                                               lora_a.data_ptr(), lora_b.data_ptr(), n, r, rows.native_ptr,
-                                                               out.data_ptr(), N, M, N, K, workspace.data_ptr(), need,
-                                                               nat.current_stream(x.device)),
+            nat.check(lib.i8f_linear_w8a16_small_lora_requests(x.data_ptr(), _code(x.dtype), _ld(x), w.data_ptr(), _ld(w), ws.data_ptr(),
+                                                               mode, bias.data_ptr() if bias is not None else None,
+                                                               _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(),
+                                                               lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(), N, M, N, K,
+                                                               workspace.data_ptr(), need, nat.current_stream(x.device)),
                       "i8f_linear_w8a16_small_lora_requests")
-    return out
+        return out
 
 
 def _bias_arg(bias: Tensor | None, device: torch.device, n: int) -> Tensor | None:
@@ -549,73 +570,83 @@ def _bias_arg(bias: Tensor | None, device: torch.device, n: int) -> Tensor | Non
         return None
     if bias.numel() != n:
         raise ValueError(f"bias must have {n} elements, got {bias.numel()}")
-    return bias.to(device).contiguous()
+    return bias if bias.device == device and bias.is_contiguous() else bias.to(device).contiguous()
 
 
-def _modulation(v: Tensor | None, name: str, y: Tensor, requests: int) -> Tensor | None:
-    """One row of K values per request ([requests, K]) or one for all ([K])."""
+def _modulation(v: Tensor | None, name: str, y: Tensor, requests: int):
+    """One row of K values per request ([requests, K]) or one for all ([K]): the tensor, its pointer, its pitch and whether
+    it has a row per request."""
     if v is None:
-        return None
+        return None, None, 0, False
+    K = y.shape[1]
     if v.dim() == 1:
         v = v[None]
-    if v.dim() != 2 or v.shape[1] != y.shape[1] or v.shape[0] not in (1, requests):
-        raise ValueError(f"{name} must be [{y.shape[1]}] or [{requests}, {y.shape[1]}], got {tuple(v.shape)}")
-    v = v.to(device=y.device, dtype=y.dtype)
-    if v.stride(1) != 1 and v.shape[1] > 1:
+    if v.dim() != 2 or v.shape[1] != K or v.shape[0] not in (1, requests):
+        raise ValueError(f"{name} must be [{K}] or [{requests}, {K}], got {tuple(v.shape)}")
+    if v.dtype != y.dtype or v.device != y.device:
+        v = v.to(device=y.device, dtype=y.dtype)
+    per_request = v.shape[0] > 1
+    if (v.stride(1) != 1 and K > 1) or (per_request and v.stride(0) < K):
         v = v.contiguous()
-    if v.shape[0] > 1 and v.stride(0) < v.shape[1]:
+    return v, v.data_ptr(), v.stride(0) if per_request else K, per_request
+
+
+def _weight_vector(v: Tensor | None, name: str, y: Tensor):
+    if v is None:
+        return None, None
+    if v.numel() != y.shape[1]:
+        raise ValueError(f"{name} must have {y.shape[1]} elements")
+    if v.dtype != y.dtype or v.device != y.device:
+        v = v.to(device=y.device, dtype=y.dtype)
+    if not v.is_contiguous():
         v = v.contiguous()
-    return v
+    return v, v.data_ptr()
 
 
 def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm, post_weight, norm, weight, scale, shift, eps,
                          x_out, want_h, want_q):
-    nat.require_device(y.device)
-    if x.dim() != 2 or y.dim() != 2 or x.shape != y.shape or x.device != y.device:
-        raise ValueError(f"x and y must be 2-D tensors of one shape on one device, got {tuple(x.shape)} and {tuple(y.shape)}")
-    if y.dtype not in (torch.bfloat16, torch.float16) or x.dtype not in (y.dtype, torch.float32):
-        raise ValueError(f"y must be bf16 or fp16 and x of the same type or fp32, got {y.dtype} and {x.dtype}")
-    if post_norm not in nat.NORM_CODE or norm not in ("rms", "layer"):
-        raise ValueError("post_norm is None, 'rms' or 'layer'; norm is 'rms' or 'layer'")
-    M, K = y.shape
-    requests = 1
-    if rows is not None:
-        if rows.device != y.device or rows.total != M:
-            raise ValueError(f"the row plan is for {rows.total} rows on {rows.device}, the call has {M} on {y.device}")
-        requests = rows.requests
-    given = x
-    x, y = _rows(x), _rows(y)
-    vectors = [_modulation(v, name, y, requests) for v, name in ((gate, "gate"), (scale, "scale"), (shift, "shift"))]
-    weights = []
-    for v, name in ((post_weight, "post_weight"), (weight, "weight")):
-        if v is not None and v.numel() != K:
-            raise ValueError(f"{name} must have {K} elements")
-        weights.append(None if v is None else v.reshape(-1).to(device=y.device, dtype=y.dtype).contiguous())
-    if x_out is None:
-        x_out = torch.empty((M, K), dtype=x.dtype, device=x.device)
-    elif x_out.shape != (M, K) or x_out.dtype != x.dtype or x_out.device != x.device or (K > 1 and x_out.stride(1) != 1) or (
-            M > 1 and x_out.stride(0) < K):
-        raise ValueError("x_out must have x's shape, type and device, rows of unit inner stride that do not overlap")
-    elif x_out is given:
-        x = x_out
-    h = torch.empty((M, K), dtype=y.dtype, device=y.device) if want_h else None
-    q = torch.empty((M, K), dtype=torch.int8, device=y.device) if want_q else None
-    q_scale = torch.empty((M, 1), dtype=torch.float32, device=y.device) if want_q else None
-    if M and K:
-        # one vector for all rows: a pitch that the row plan's request index multiplies is not used with row_request NULL
-        shared = all(v is None or v.shape[0] == 1 for v in vectors)
-        if not shared:
-            vectors = [v if v is None or v.shape[0] == requests else v.expand(requests, K).contiguous() for v in vectors]
-        g, s, t = vectors
-        with _on(y.device):
+    device = y.device
+    with _on(device):
+        if x.dim() != 2 or y.dim() != 2 or x.shape != y.shape or x.device != device:
+            raise ValueError(f"x and y must be 2-D tensors of one shape on one device, got {tuple(x.shape)} and {tuple(y.shape)}")
+        if y.dtype not in (torch.bfloat16, torch.float16) or x.dtype not in (y.dtype, torch.float32):
+            raise ValueError(f"y must be bf16 or fp16 and x of the same type or fp32, got {y.dtype} and {x.dtype}")
+        if post_norm not in nat.NORM_CODE or norm not in ("rms", "layer"):
+            raise ValueError("post_norm is None, 'rms' or 'layer'; norm is 'rms' or 'layer'")
+        M, K = y.shape
+        requests = 1
+        if rows is not None:
+            if rows.device != device or rows.total != M:
+                raise ValueError(f"the row plan is for {rows.total} rows on {rows.device}, the call has {M} on {device}")
+            requests = rows.requests
+        given = x
+        x, y = _rows(x), _rows(y)
+        gate, g, ldg, many_g = _modulation(gate, "gate", y, requests)
+        scale, s, lds, many_s = _modulation(scale, "scale", y, requests)
+        shift, t, ldt, many_t = _modulation(shift, "shift", y, requests)
+        post_weight, pw = _weight_vector(post_weight, "post_weight", y)
+        weight, nw = _weight_vector(weight, "weight", y)
+        if x_out is None:
+            x_out = torch.empty((M, K), dtype=x.dtype, device=device)
+        elif x_out.shape != (M, K) or x_out.dtype != x.dtype or x_out.device != device or (K > 1 and x_out.stride(1) != 1) or (
+                M > 1 and x_out.stride(0) < K):
+            raise ValueError("x_out must have x's shape, type and device, rows of unit inner stride that do not overlap")
+        elif x_out is given:
+            x = x_out
+        h = torch.empty((M, K), dtype=y.dtype, device=device) if want_h else None
+        q = torch.empty((M, K), dtype=torch.int8, device=device) if want_q else None
+        q_scale = torch.empty((M, 1), dtype=torch.float32, device=device) if want_q else None
+        if M and K:
+            row_request = rows.row_request_ptr if many_g or many_s or many_t else None
+            # a vector for all rows beside others per request: a pitch of 0 gives every request the same row
+            if row_request is not None:
+                ldg, lds, ldt = ldg if many_g else 0, lds if many_s else 0, ldt if many_t else 0
             nat.check(nat.load().i8f_gated_residual_norm(
-                x.data_ptr(), _code(x.dtype), _ld(x), y.data_ptr(), _code(y.dtype), _ld(y), M, K,
-                None if shared else rows.native.row_request, nat.ptr(g), _ld(g) if g is not None else 0, 1 if gate_tanh else 0,
-                float(residual_scale), nat.NORM_CODE[post_norm], nat.ptr(weights[0]), nat.NORM_CODE[norm], nat.ptr(weights[1]),
-                nat.ptr(s), _ld(s) if s is not None else 0, nat.ptr(t), _ld(t) if t is not None else 0, float(eps),
-                x_out.data_ptr(), _ld(x_out), nat.ptr(h), K, nat.ptr(q), K, nat.ptr(q_scale), nat.current_stream(y.device)),
-                "i8f_gated_residual_norm")
-    return x_out, h, q, q_scale
+                x.data_ptr(), _code(x.dtype), _ld(x), y.data_ptr(), _code(y.dtype), _ld(y), M, K, row_request, g, ldg, 1 if gate_tanh else 0,
+                residual_scale, nat.NORM_CODE[post_norm], pw, nat.NORM_CODE[norm], nw, s, lds, t, ldt, eps, x_out.data_ptr(), _ld(x_out),
+                h.data_ptr() if want_h else None, K, q.data_ptr() if want_q else None, K, q_scale.data_ptr() if want_q else None,
+                nat.current_stream(device)), "i8f_gated_residual_norm")
+        return x_out, h, q, q_scale
 
 
 def gated_residual_norm(x: Tensor, y: Tensor, gate: Tensor | None = None, *, rows: RequestRows | None = None, gate_tanh: bool = False,

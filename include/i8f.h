@@ -306,8 +306,16 @@ typedef struct i8f_request_rows {
     int64_t rows;               /* rows of the batch, M */
     const int32_t* row_adapter; /* [rows]: index into the bank of adapters, -1: none */
     const int32_t* row_request; /* [rows]: request of the row (gated_residual_norm) */
-    const int32_t* chunks;      /* [n_chunks][4]: first row, row count (1..4), adapter or -1, 0; the chunks cover every row once */
+    /* The batch in tiles of 256 rows: [ceil(rows / 256)][4] = first slot, slots, addend row, 0.  A dense tile (addend row
+     * -1) has one slot for each adapter in it, at most 8; a chunked one none, its rows start at `addend row` of the fp32
+     * addend and are covered by chunks. */
+    const int32_t* tiles;
+    const int32_t* slots;       /* [][12]: adapter, 0, 0, 0, then 256 bits: the rows of the tile that use it */
+    const int32_t* chunks;      /* [n_chunks][4]: first row, row count (1..4), adapter or -1, addend row; every row of a chunked
+                                   tile is in one chunk */
+    int64_t n_dense;            /* dense tiles; 0 for a batch of at most 16 rows */
     int64_t n_chunks;
+    int64_t addend_rows;        /* rows of the addend: 256 per chunked tile, the last one may be cut at the end of the batch */
     int32_t max_adapter;        /* largest adapter index in use, -1 if none */
 } i8f_request_rows;
 
@@ -322,7 +330,8 @@ int i8f_lora_down_requests(const void* x, int64_t ldx, const void* bank_a, int64
  *   I8F_EPI_PYTORCH: out = round(round(dequant (+bias)) + round(t[m] @ bank_b[adapter(m)]^T)), the roundings of
  *                    i8f_linear_w8a8_lora
  * bank_b [adapters, N, r] contiguous in out_dtype, t from i8f_lora_down_requests; the other arguments as in
- * i8f_linear_w8a8.  `workspace`: i8f_lora_requests_workspace_bytes of device memory, 16-byte aligned. */
+ * i8f_linear_w8a8.  `workspace`: i8f_lora_requests_workspace_bytes of device memory (0 where no tile is
+ * chunked), 16-byte aligned. */
 size_t i8f_lora_requests_workspace_bytes(const i8f_request_rows* rows, int64_t N);
 int i8f_linear_w8a8_lora_requests(const int8_t* a, int64_t lda, const float* a_scale,
                                   const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
@@ -330,6 +339,17 @@ int i8f_linear_w8a8_lora_requests(const int8_t* a, int64_t lda, const float* a_s
                                   int64_t adapters, int64_t r, const i8f_request_rows* rows,
                                   void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int epilogue_order,
                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* The whole forward of such a layer: (rotate) -> per-token quantise -> int8 GEMM, with the adapters beside it.  x, the
+ * banks and out share x_dtype.  With hadamard128 the adapters see the rotated activations if rotated_lora_input is set
+ * (ldx == K then).  `workspace`: 256-byte aligned device memory. */
+size_t i8f_linear_lora_requests_workspace_bytes(const i8f_request_rows* rows, int64_t N, int64_t K, int64_t r, int hadamard128,
+                                                int rotated_lora_input);
+int i8f_linear_lora_requests(const void* x, int x_dtype, int64_t ldx, int hadamard128, int rotated_lora_input,
+                             const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
+                             const void* bias, int bias_dtype, const void* bank_a, const void* bank_b, int64_t adapters, int64_t r,
+                             const i8f_request_rows* rows, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                             int epilogue_order, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The form for at most 16 rows (single tokens), activations not quantised:
  *   out = round(w_scale * (x @ w^T) + bias + round(x[m] @ bank_a[a]^T) @ bank_b[a]^T), a = adapter(m)
@@ -352,7 +372,7 @@ int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx
  *   h     = norm(x_out) * weight * (1 + scale[q]) + shift[q]
  * fp32 throughout; h comes from the unrounded x_out, so each output is rounded once.  x, x_out [M,K] in x_dtype
  * (y_dtype or I8F_F32); y, h and all vectors in y_dtype (I8F_BF16 or I8F_F16).  gate, scale, shift: [requests, K] with
- * pitches ldg, lds, ldt, each may be NULL (1, 0, 0), as may the weights [K].  h [M,K] and the per-token int8 form of h
+ * pitches ldg, lds, ldt (0: one row for every request), each may be NULL (1, 0, 0), as may the weights [K].  h [M,K] and the per-token int8 form of h
  * (q [M,K], row_scale [M] as in i8f_quant_rowwise) may be asked for separately or both; NULL: not wanted.  x_out may be x.
  * K at most 16384; rows of any length, pitch and alignment (16-byte aligned rows of a multiple of 8 elements are read
  * and written in 16-byte pieces). */

@@ -7,34 +7,60 @@ import torch
 
 
 def tables(rows):
-    """row_adapter, row_request and chunks of a plan made on the CPU, read back through the struct the library gets."""
+    """The tables of a plan made on the CPU, read back through the struct that the library gets."""
     n = rows.native
 
-    def at(ptr, count):
-        return np.ctypeslib.as_array(ctypes.cast(ptr, ctypes.POINTER(ctypes.c_int32)), (count,)).copy() if count else np.zeros(0, np.int32)
+    def at(ptr, *shape):
+        count = int(np.prod(shape))
+        if not count:
+            return np.zeros(shape, np.int32)
+        assert ptr % 16 == 0
+        return np.ctypeslib.as_array(ctypes.cast(ptr, ctypes.POINTER(ctypes.c_int32)), (count,)).copy().reshape(shape)
 
-    return at(n.row_adapter, n.rows), at(n.row_request, n.rows), at(n.chunks, 4 * n.n_chunks).reshape(-1, 4)
+    tiles = at(n.tiles, -(-n.rows // 256), 4)
+    return (at(n.row_adapter, n.rows), at(n.row_request, n.rows), tiles, at(n.slots, int(tiles[:, 1].sum()), 12), at(n.chunks, n.n_chunks, 4))
 
 
 @pytest.mark.parametrize("lengths,adapters", [
     ([1], None), ([1], [3]), ([0, 5, 0], [0, 1, 2]), ([1] * 9, [0, 0, 0, 0, 0, 1, -1, -1, 1]), ([257, 3, 0, 255], [2, -1, 5, 2]),
-    ([4, 4, 1, 300], [1, 1, 1, 0]), ([0, 0], [0, 0]), ([1000], [-1]),
+    ([4, 4, 1, 300], [1, 1, 1, 0]), ([0, 0], [0, 0]), ([1000], [-1]), ([1] * 400, [i % 9 for i in range(400)]), ([255], [0]), ([256], [0]),
+    ([1] * 300 + [500] + [1] * 100, [i % 20 for i in range(401)]), ([600] + [1] * 50, [0] * 51), ([130, 2, 700], [1048575, -1, 7]),
 ])
 def test_row_plan_describes_every_row_once(pkg, lengths, adapters):
     rows = pkg.adapters.RequestRows(lengths, adapters, device="cpu")
+    M = sum(lengths)
     want_adapter = [a for n, a in zip(lengths, adapters or [-1] * len(lengths)) for _ in range(n)]
     want_request = [i for i, n in enumerate(lengths) for _ in range(n)]
-    row_adapter, row_request, chunks = tables(rows)
-    assert rows.total == rows.native.rows == sum(lengths) and rows.requests == len(lengths)
+    row_adapter, row_request, tiles, slots, chunks = tables(rows)
+    assert rows.total == rows.native.rows == M and rows.requests == len(lengths)
     assert row_adapter.tolist() == want_adapter and row_request.tolist() == want_request
     assert rows.native.max_adapter == max(want_adapter, default=-1)
-    covered = []
-    for first, count, adapter, _ in chunks.tolist():
-        assert 1 <= count <= 4 and all(want_adapter[first + i] == adapter for i in range(count))
-        covered += range(first, first + count)
-    assert covered == list(range(sum(lengths)))
-    for ptr in (rows.native.row_adapter, rows.native.row_request, rows.native.chunks):
-        assert ptr % 16 == 0
+    assert rows.native.n_dense == (tiles[:, 2] < 0).sum() and (M > 16 or rows.native.n_dense == 0)
+    # dense tiles: one slot for each adapter, its rows and no others
+    next_slot = 0
+    addend_at = {}
+    for i, (begin, count, addend, _) in enumerate(tiles.tolist()):
+        tile_rows = range(256 * i, min(M, 256 * i + 256))
+        if addend >= 0:
+            assert count == 0
+            addend_at.update({m: addend + m - 256 * i for m in tile_rows})
+            continue
+        assert addend == -1 and 0 <= count <= 8 and begin == next_slot
+        next_slot += count
+        mine = slots[begin:begin + count]
+        assert sorted(mine[:, 0].tolist()) == sorted({want_adapter[m] for m in tile_rows} - {-1})
+        for slot in mine:
+            bits = np.unpackbits(slot[4:].view(np.uint8), bitorder="little")
+            assert (256 * i + np.flatnonzero(bits)).tolist() == [m for m in tile_rows if want_adapter[m] == slot[0]]
+    # chunked tiles: every row in one chunk, with a place of its own in the addend
+    covered = {}
+    for first, count, adapter, addend in chunks.tolist():
+        assert 1 <= count <= 4
+        for j in range(count):
+            assert first + j not in covered and want_adapter[first + j] == adapter
+            covered[first + j] = addend + j
+    assert covered == addend_at
+    assert rows.native.addend_rows == len(addend_at) and sorted(addend_at.values()) == list(range(len(addend_at)))
 
 
 @pytest.mark.parametrize("lengths,adapters", [([], None), ([-1], None), ([2, 3], [0]), ([2], [-2]), ([2], [1 << 20]), ([1 << 30, 1 << 30], None)])
@@ -78,7 +104,8 @@ ODD = ctypes.c_void_p(4098)
 
 
 def native_rows(pkg, rows=8, max_adapter=1, **kw):
-    s = pkg._native.RequestRowsStruct(rows=rows, row_adapter=4096, row_request=4096, chunks=4096, n_chunks=2, max_adapter=max_adapter)
+    s = pkg._native.RequestRowsStruct(rows=rows, row_adapter=4096, row_request=4096, tiles=4096, slots=4096, chunks=4096, n_dense=0, n_chunks=2,
+                                      addend_rows=rows, max_adapter=max_adapter)
     for k, v in kw.items():
         setattr(s, k, v)
     return ctypes.byref(s)
@@ -107,8 +134,23 @@ def test_abi_refuses_bad_adapter_calls(pkg):
                      (-2, dict(t=ODD)), (-2, dict(bank=ODD)), (-6, dict(ws=None)), (-6, dict(ws_bytes=64)), (-2, dict(ws=ODD))):
         assert gemm(**kw) == want, kw
         assert nat.last_error()
+    for rows in (dict(n_chunks=0), dict(n_chunks=-1, n_dense=2), dict(n_dense=1, slots=None), dict(addend_rows=0), dict(row_adapter=None)):
+        assert gemm(rows=native_rows(pkg, **rows)) == -1, rows
     assert gemm(M=0, rows=native_rows(pkg, rows=0)) == 0
     assert gemm(N=0) == 0
+
+    def whole(x=P, dt=nat.I8F_BF16, ldx=64, had=0, rot=0, w=P, ws=P, wsb=1 << 20, bank_a=P, bank_b=P, adapters=2, r=16, rows=None, M=8, N=64,
+              K=64, order=1, ldo=64):
+        return lib.i8f_linear_lora_requests(x, dt, ldx, had, rot, w, K, P, 0, None, 0, bank_a, bank_b, adapters, r,
+                                            rows or native_rows(pkg, rows=M), P, ldo, M, N, K, order, ws, wsb, None)
+
+    for want, kw in ((-1, dict(rows=native_rows(pkg, rows=7))), (-3, dict(dt=nat.I8F_F32)), (-2, dict(K=72, ldx=72)), (-1, dict(adapters=1)),
+                     (-1, dict(bank_a=None)), (-1, dict(bank_b=None)), (-3, dict(r=12)), (-1, dict(x=None)), (-1, dict(w=None)),
+                     (-1, dict(ldx=56)), (-2, dict(x=ODD)), (-2, dict(w=ODD)), (-1, dict(ldo=63)), (-1, dict(order=2)),
+                     (-6, dict(ws=None)), (-6, dict(wsb=64)), (-2, dict(ws=ODD)), (-3, dict(had=1, rot=1, K=128, ldx=136))):
+        assert whole(**kw) == want, kw
+        assert nat.last_error()
+    assert whole(M=0, rows=native_rows(pkg, rows=0)) == 0 and whole(N=0) == 0
 
     def small(x=P, dt=nat.I8F_BF16, ldx=64, bank_a=P, bank_b=P, adapters=2, r=16, rows=None, M=8, N=64, K=64, ws=P, ws_bytes=1 << 20):
         return lib.i8f_linear_w8a16_small_lora_requests(x, dt, ldx, P, K, P, 0, None, 0, bank_a, bank_b, adapters, r,
@@ -116,7 +158,7 @@ def test_abi_refuses_bad_adapter_calls(pkg):
 
     for want, kw in ((-1, dict(rows=native_rows(pkg, rows=7))), (-3, dict(M=17)), (-3, dict(dt=nat.I8F_F32)), (-1, dict(adapters=1)), (-3, dict(r=4)),
                      (-1, dict(bank_a=None)), (-2, dict(bank_b=ODD)), (-2, dict(K=72, ldx=72)), (-6, dict(ws=None)), (-6, dict(ws_bytes=64)),
-                     (-1, dict(x=None))):
+                     (-1, dict(x=None)), (-1, dict(rows=native_rows(pkg, n_dense=1)))):
         assert small(**kw) == want, kw
         assert nat.last_error()
 
