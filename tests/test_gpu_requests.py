@@ -282,6 +282,21 @@ NORM = [
     ([257, 1024], 6144, torch.bfloat16, torch.bfloat16, "rms", "rms", True, False, True, True, True, 1.0),
     ([33], 8200, torch.bfloat16, torch.bfloat16, None, "rms", False, True, True, False, True, 1.0),
     ([2000, 1, 999, 1700], 4096, torch.bfloat16, torch.bfloat16, "rms", "rms", True, True, True, False, True, 1.0),
+    # many rows whose length eight does not divide: they start anywhere between two 16-byte boundaries
+    ([300, 0, 477], 2305, torch.float16, torch.float16, "layer", "layer", False, True, True, True, True, 0.5),
+    ([1000, 3], 1027, torch.bfloat16, torch.float32, "rms", "layer", True, True, True, True, True, 1.0),
+    ([1, 400], 4094, torch.bfloat16, torch.bfloat16, None, "rms", False, False, True, False, True, 1.0),
+    ([700], 4101, torch.float16, torch.float32, "layer", "rms", True, True, False, True, False, 1.0),
+    ([300], 9001, torch.bfloat16, torch.bfloat16, "rms", "rms", True, True, True, True, True, 1.0),
+    ([260], 12287, torch.float16, torch.float16, "rms", "layer", False, True, True, True, True, 1.0),
+    # many rows of other lengths: a warp each, a group each, one row of the ring at a time
+    ([500, 800], 64, torch.bfloat16, torch.float32, "rms", "layer", True, True, True, True, True, 1.0),
+    ([999], 1016, torch.float16, torch.float16, "layer", "rms", False, True, True, True, True, 1.0),
+    ([400, 111], 251, torch.bfloat16, torch.bfloat16, "layer", "layer", False, True, True, True, True, 1.0),
+    ([256], 8192, torch.bfloat16, torch.float32, "layer", "layer", False, True, True, True, True, 1.0),
+    ([310], 12288, torch.bfloat16, torch.bfloat16, "rms", "rms", True, True, True, True, True, 1.0),
+    ([280], 16384, torch.float16, torch.float16, "rms", "layer", False, True, True, True, True, 1.0),
+    ([1] * 600, 2048, torch.bfloat16, torch.bfloat16, "rms", "rms", True, True, True, False, True, 1.0),
 ]
 
 
