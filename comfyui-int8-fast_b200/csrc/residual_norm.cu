@@ -443,7 +443,12 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
     constexpr int kGroups = kWorkers / GT;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) float s_part[2 * kWorkers / 32];
-    __shared__ __align__(8) unsigned long long s_full[kMaxSlots], s_empty[kMaxSlots];
+    // Two barriers for the arrival of a slot's rows, used in turn.  A slot passes from group to group and copies land in any
+    // order, so a group may come for its row while the row before it in the slot, another group's, is still on its way: on
+    // one barrier that group would take the phase before for its own (they have the same parity).  The barrier's previous
+    // row is then two rounds back, and that one has been consumed: the row in between could not have been issued otherwise,
+    // and it was issued before the group's own previous row (there are more slots than groups).
+    __shared__ __align__(8) unsigned long long s_full[2 * kMaxSlots], s_empty[kMaxSlots];
     __shared__ int s_abort;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     float* const s_gate = reinterpret_cast<float*>(smem);
@@ -455,6 +460,7 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
     if (threadIdx.x == 0) {
         for (int i = 0; i < n_slots; ++i) {
             mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_full[n_slots + i]), 1);
             mbar_init(smem_u32(&s_empty[i]), 1);
         }
         s_abort = 0;
@@ -465,25 +471,22 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
 
     if (threadIdx.x >= kWorkers) {
         if (threadIdx.x == kWorkers) {
-            int slot = 0;
-            uint32_t phase = 0;
+            int turn = 0;       // row number modulo 2 * n_slots
             for (int64_t row = row0; row < row1; ++row) {
-                if (!mbar_wait_bounded(smem_u32(&s_empty[slot]), phase ^ 1u, &s_abort, status, kStNormEmpty)) break;
+                const int slot = turn < n_slots ? turn : turn - n_slots;
+                if (!mbar_wait_bounded(smem_u32(&s_empty[slot]), turn < n_slots ? 1u : 0u, &s_abort, status, kStNormEmpty)) break;
                 const uintptr_t px = reinterpret_cast<uintptr_t>(static_cast<const TX*>(a.x) + row * a.ldx);
                 const uintptr_t py = reinterpret_cast<uintptr_t>(static_cast<const TY*>(a.y) + row * a.ldy);
                 const uint32_t nx = static_cast<uint32_t>(((px & 15) + a.K * sizeof(TX) + 15) & ~uintptr_t(15));
                 const uint32_t ny = static_cast<uint32_t>(((py & 15) + a.K * sizeof(TY) + 15) & ~uintptr_t(15));
                 uint32_t dst = smem_u32(ring) + static_cast<uint32_t>(slot * (x_slot + y_slot));
-                const uint32_t bar = smem_u32(&s_full[slot]);
+                const uint32_t bar = smem_u32(&s_full[turn]);
                 mbar_arrive_expect_tx(bar, nx + ny);
                 // an fp32 row starts in the 16-byte half of its 8-element vector that its place in memory says
                 const uint32_t half = XDT == I8F_F32 && SHIFT ? static_cast<uint32_t>((py & 15) / 2 - (px & 15) / 4) * 4u : 0u;
                 bulk_load(dst + half, reinterpret_cast<const void*>(px & ~uintptr_t(15)), nx, bar);
                 bulk_load(dst + x_slot, reinterpret_cast<const void*>(py & ~uintptr_t(15)), ny, bar);
-                if (++slot == n_slots) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
+                if (++turn == 2 * n_slots) turn = 0;
             }
         }
     } else {
@@ -492,8 +495,8 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
         const float inv_k = 1.0f / static_cast<float>(K);
         const bool quant = a.q != nullptr;
         GroupReduce<GT> red{s_part + group * 2 * (GT / 32), 1 + group, 0};
-        int slot = group % n_slots, have = -1;
-        uint32_t phase = static_cast<uint32_t>(group / n_slots) & 1u;
+        int turn = group, have = -1;      // row number modulo 2 * n_slots; fewer groups than slots
+        uint32_t phase = 0;
         int64_t row = row0 + group;
         for (int64_t seg0 = row0; seg0 < row1;) {
             // the rows [seg0, seg1) of the share belong to one request
@@ -540,9 +543,11 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
                 asm volatile("bar.sync 15, 512;" ::: "memory");
             }
             for (; row < seg1; row += kGroups) {
-                // after a wait that ran out the rows are walked to the end all the same (every later wait gives up at once):
-                // the groups meet at barriers and may not leave one another there
-                mbar_wait_bounded(smem_u32(&s_full[slot]), phase, &s_abort, status, kStNormFull);
+                // After a wait that ran out the rows are walked to the end all the same (every later wait gives up at once):
+                // the groups meet at barriers and may not leave one another there.
+                mbar_wait_bounded(smem_u32(&s_full[turn]), phase, &s_abort, status, kStNormFull);
+                __syncwarp();
+                const int slot = turn < n_slots ? turn : turn - n_slots;
                 const uintptr_t py = reinterpret_cast<uintptr_t>(static_cast<const TY*>(a.y) + row * a.ldy);
                 const int o = SHIFT ? static_cast<int>((py >> 1) & 7) : 0;      // elements between the boundary and the row
                 const TX* const sx = reinterpret_cast<const TX*>(ring + slot * (x_slot + y_slot)) + o;
@@ -693,9 +698,9 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
                         }
                     }
                 }
-                slot += kGroups;
-                while (slot >= n_slots) {
-                    slot -= n_slots;
+                turn += kGroups;
+                if (turn >= 2 * n_slots) {
+                    turn -= 2 * n_slots;
                     phase ^= 1u;
                 }
             }
@@ -707,7 +712,8 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
 }
 
-// Launches the ring kernel if its columns and at least `min_slots` rows fit an SM; *done says whether they did.
+// Launches the ring kernel if its columns and at least `min_slots` rows (more than there are groups, or two for a single one)
+// fit an SM; *done says whether they did.
 template <int XDT, int YDT, int GT, int VPT, bool SHIFT>
 int launch_ring(const NormArgs& a, int min_slots, int sms, cudaStream_t st, bool* done) {
     const int slot = slot_bytes(a.K * dtype_size(XDT)) + slot_bytes(a.K * dtype_size(YDT));

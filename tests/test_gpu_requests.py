@@ -380,6 +380,22 @@ def test_gated_residual_norm_special_rows(cuda_pkg):
         assert h[4:].isfinite().all() and qs[4:].isfinite().all() and not h[5].any()
 
 
+@pytest.mark.parametrize("K,xdt", [(4096, torch.float32), (4096, torch.bfloat16), (2305, torch.bfloat16), (8192, torch.bfloat16)])
+def test_gated_residual_norm_many_launches(cuda_pkg, K, xdt):
+    """Rows arrive in any order and every launch gives the same bits (the fixture checks that no wait ran out)."""
+    F = cuda_pkg.functional
+    g = gen(13)
+    x, y = torch.randn(9000, K, generator=g, device=DEV).to(xdt), torch.randn(9000, K, generator=g, device=DEV).bfloat16()
+    mod = torch.randn(3, K, generator=g, device=DEV).bfloat16()
+    rows = cuda_pkg.adapters.RequestRows([4000, 1, 4999], None, DEV)
+    want = F.gated_residual_norm(x, y, mod, rows=rows, post_norm="rms", norm="layer")
+    wrong = torch.zeros((), dtype=torch.int64, device=DEV)
+    for _ in range(400):
+        got = F.gated_residual_norm(x, y, mod, rows=rows, post_norm="rms", norm="layer")
+        wrong += (got[0] != want[0]).any() | (got[1] != want[1]).any()
+    assert int(wrong) == 0
+
+
 def test_gated_residual_norm_refuses(cuda_pkg):
     F, E = cuda_pkg.functional, cuda_pkg._native.NativeLibraryError
     Rows = cuda_pkg.adapters.RequestRows
