@@ -36,6 +36,7 @@
 #include <cuda_fp16.h>
 
 #include "host_common.h"
+#include "low_rank.cuh"
 #include "ptx_sm100.cuh"
 #include "tensor_maps.h"
 
@@ -47,10 +48,10 @@ constexpr int kStageRowBytes = 128; // one 128-byte swizzle span of K per stage
 
 enum EpiMode : int { kEpiI32 = 0, kEpiDequant = 1, kEpiCast = 2, kEpiAccum = 3 };
 // what joins the product in the epilogue (a template parameter, so that the plain kernels carry none of it)
-enum Extra : int { kExtraNone = 0, kExtraLora = 1, kExtraAddend = 2, kExtraRequests = 3 };
+enum Extra : int { kExtraNone = 0, kExtraLora = 1, kExtraAddend = 2, kExtraRequests = 3, kExtraRows = 4 };
 
 // status codes written by bounded waits
-enum : int { kStEmptyWait = 101, kStFullWait = 102, kStAccEmptyWait = 103, kStAccFullWait = 104 };
+enum : int { kStEmptyWait = 101, kStFullWait = 102, kStAccEmptyWait = 103, kStAccFullWait = 104, kStLowEmptyWait = 106, kStLowFullWait = 107 };
 
 struct GemmParams {
     int M, N;
@@ -87,6 +88,12 @@ struct GemmParams {
     const RequestSlot* req_slots;
     int lora_k16;       // 16-element steps of the rank
     long long lora_n;   // rows of lora_b per adapter
+    // kExtraRows: eight more warps work the low-rank term of the tile's rows out (low_rank.cuh) while the MMAs run
+    const uint16_t* row_t;
+    long long ld_row_t;
+    const uint16_t* row_b;
+    int row_r;
+    int early_b;        // the weights are older than the kernel before this one: the first slabs are fetched beside its tail
 };
 
 constexpr int kMaxOutputs = 8;
@@ -114,8 +121,11 @@ struct Cfg {
     // Epilogue warps: four (one per 32-lane quarter of tensor memory) or, where the epilogue cannot hide under the
     // next tile's MMAs (single accumulator buffer, below), eight: two per quarter, each taking half of the columns.
     static constexpr int kEpiWarps = (LORA && 3 * BN > 512) ? 8 : 4;
-    static constexpr int kThreads = 64 + 32 * kEpiWarps;
-    static constexpr int kRingBudget = (kEpiWarps == 8 ? 160 : 192) * 1024;   // eight warps need more staging space
+    static constexpr int kLowWarps = EXTRA == kExtraRows ? 8 : 0;
+    static constexpr int kThreads = 64 + 32 * (kEpiWarps + kLowWarps);
+    static constexpr int kLowPitch = BN + 4;   // floats; rows four banks apart: the epilogue's row-per-thread reads do not collide
+    static constexpr int kLowBytes = EXTRA == kExtraRows ? kBM * kLowPitch * 4 : 0;
+    static constexpr int kRingBudget = (kEpiWarps == 8 ? 160 : EXTRA == kExtraRows ? 128 : 192) * 1024;   // eight warps need more staging space
     static constexpr int kStages = kRingBudget / kStageBytes > 8 ? 8 : kRingBudget / kStageBytes;
     // TMEM: two int32/fp32 accumulator buffers at columns 0 and BN, so the epilogue of a tile overlaps the MMAs of the
     // next; with LORA one more fp32 accumulator behind them.  The LoRA accumulator needs no double buffering: it is
@@ -130,7 +140,8 @@ struct Cfg {
     static constexpr int kBarrierBytes = 1024;
     static constexpr int kEpiBytes = kEpiWarps * 2 * BN * 4;  // per epilogue warp: BN column scales + BN biases (fp32)
     static constexpr int kOutStageBytes = kEpiWarps * 2 * 2048;  // per epilogue warp: two 32-row x 64-byte output chunks
-    static constexpr int kSmemBytes = kStages * kStageBytes + kBarrierBytes + kEpiBytes + kOutStageBytes + 1024;  // + slack
+    static constexpr int kSmemBytes = kStages * kStageBytes + kBarrierBytes + kEpiBytes + kOutStageBytes + kLowBytes + 1024;  // + slack
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory of an SM");
     static constexpr int kTileM = PAIR ? 2 * kBM : kBM;
 };
 
@@ -302,7 +313,7 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, long long ro
 #pragma unroll
             for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], cb[j]);
         }
-        if constexpr (EXTRA == kExtraAddend || EXTRA == kExtraRequests) {
+        if constexpr (EXTRA != kExtraNone && EXTRA != kExtraLora) {
             if (single) {   // the low-rank term joins in fp32: one rounding in all
 #pragma unroll
                 for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], __uint_as_float(lv[j]));
@@ -411,6 +422,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + kBarOff + 16 * C::kStages + 36);
     float* epi_smem = reinterpret_cast<float*>(gen_base + kBarOff + C::kBarrierBytes);
     const uint32_t out_stage0 = smem_base + kBarOff + C::kBarrierBytes + C::kEpiBytes;  // 1024-byte aligned
+    float* const low_smem = reinterpret_cast<float*>(gen_base + kBarOff + C::kBarrierBytes + C::kEpiBytes + C::kOutStageBytes);
+    const uint32_t low_full = tmem_slot + 8, low_empty = tmem_slot + 16;      // kExtraRows: the tile's low-rank rows are there / read
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -425,6 +438,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         for (int b = 0; b < 2; ++b) {
             mbar_init(accfull0 + 8 * b, 1);
             mbar_init(accempty0 + 8 * b, (PAIR ? 2 : 1) * C::kEpiWarps);  // one arrival per epilogue warp (of both CTAs)
+        }
+        if constexpr (EXTRA == kExtraRows) {
+            mbar_init(low_full, C::kLowWarps);
+            mbar_init(low_empty, C::kEpiWarps);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -446,10 +463,6 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot_ptr;
-    // Programmatic dependent launch: everything above (barriers, tensor memory, descriptor prefetch) may run while the
-    // kernel before this one in the stream is still finishing; nothing below may start before its results are visible.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-
     const int num_tiles = p.tiles_m * p.tiles_n;
     // K split (single-CTA kernels, sub-wave problems): a cluster of two CTAs owns ONE tile, each CTA runs half of the K
     // slabs into its own tensor memory, the second CTA hands its partial tile to the first through distributed shared
@@ -461,6 +474,36 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int tile_first = (PAIR || ksplit) ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
     const int kb_begin = ksplit ? static_cast<int>(krank) * (p.num_k_blocks >> 1) : 0;
     const int kb_end = (ksplit && krank == 0) ? (p.num_k_blocks >> 1) : p.num_k_blocks;
+
+    // Programmatic dependent launch: everything above (barriers, tensor memory, descriptor prefetch) may run while the
+    // kernel before this one in the stream is still finishing; nothing below may start before its results are visible.
+    int early = 0;      // slabs of the weights that are on their way already (their bytes are announced with the slab's)
+    if constexpr (EXTRA == kExtraRows) {
+        if (p.early_b && tile_first < num_tiles) {
+            // the weights and the adapters do not come from that kernel: the ring's first slabs and the bank's rows of the
+            // first tile (into L2) travel while it finishes
+            int m_blk, n_blk;
+            tile_coords(tile_first, p.tiles_m, p.tiles_n, m_blk, n_blk);
+            if (warp == 0 && lane == 0) {
+                early = min(C::kStages, kb_end - kb_begin);
+                for (int i = 0; i < early; ++i) {
+                    mbar_arrive_expect_tx(full0 + 8 * i, C::kStageBytes);
+                    tma_load_2d(smem_base + i * C::kStageBytes + C::kABytes, &tmB, full0 + 8 * i, (kb_begin + i) * kElemsPerStage, n_blk * BN);
+                }
+            }
+            if (krank == 0 && warp >= 2 + C::kEpiWarps) {
+                const int bytes = min(BN, p.N - n_blk * BN) * p.row_r * 2;
+                for (int i = warp - 2 - C::kEpiWarps; i < kBM; i += C::kLowWarps) {
+                    const int m = m_blk * kBM + i;
+                    const int a = m < p.M ? __ldg(p.row_adapter + m) : -1;
+                    if (a < 0 || (i >= C::kLowWarps && __ldg(p.row_adapter + m - 1) == a)) continue;      // the row above has asked
+                    const uint8_t* at = reinterpret_cast<const uint8_t*>(p.row_b + (a * p.lora_n + n_blk * BN) * p.row_r);
+                    for (int o = lane * 128; o < bytes; o += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + o));
+                }
+            }
+        }
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp == 0) {
         if (lane == 0) {
@@ -485,6 +528,9 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         if (leader) mbar_arrive_expect_tx(full0 + 8 * stage, 2 * C::kStageBytes);
                         tma_load_2d_pair(a_dst, &tmA, bar, kb * kElemsPerStage, row_a);
                         tma_load_2d_pair(b_dst, &tmB, bar, kb * kElemsPerStage, row_b);
+                    } else if (EXTRA == kExtraRows && early > 0) {
+                        --early;
+                        tma_load_2d(a_dst, &tmA, full0 + 8 * stage, kb * kElemsPerStage, row_a);
                     } else {
                         mbar_arrive_expect_tx(full0 + 8 * stage, C::kStageBytes);
                         tma_load_2d(a_dst, &tmA, full0 + 8 * stage, kb * kElemsPerStage, row_a);
@@ -652,12 +698,63 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             cluster_arrive();
             cluster_wait();
         }
+    } else if (EXTRA == kExtraRows && warp >= 2 + C::kEpiWarps) {
+        if constexpr (EXTRA == kExtraRows) {
+            uint32_t low_phase = 0;
+            for (int t = tile_first; krank == 0 && t < num_tiles; t += tile_step) {
+                int m_blk, n_blk;
+                tile_coords(t, p.tiles_m, p.tiles_n, m_blk, n_blk);
+                if (!mbar_wait_bounded(low_empty, low_phase ^ 1u, abort_flag, p.status, kStLowEmptyWait)) break;
+                low_phase ^= 1u;
+                const int cols = min(BN, p.N - n_blk * BN);
+                // four rows at a time, with their adapters' rows of lora_b: read once where the four share an adapter
+                const int first = warp - 2 - C::kEpiWarps;
+                constexpr int kQuads = kBM / 4 / C::kLowWarps;      // of this warp
+                int ids = -1;
+                {
+                    const int m = m_blk * kBM + (first + (lane >> 2) * C::kLowWarps) * 4 + (lane & 3);
+                    if (lane < 4 * kQuads && m < p.M) ids = __ldg(p.row_adapter + m);
+                }
+#pragma unroll 1
+                for (int i = 0; i < kQuads; ++i) {
+                    const int quad = first + i * C::kLowWarps;
+                    const int m0 = m_blk * kBM + quad * 4;
+                    if (m0 >= p.M) break;
+                    const uint16_t* b[4];      // by row
+                    int a[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        a[j] = __shfl_sync(0xFFFFFFFFu, ids, 4 * i + j);
+                        b[j] = a[j] >= 0 ? p.row_b + (a[j] * p.lora_n + n_blk * BN) * p.row_r : nullptr;
+                    }
+                    const uint16_t* rows_t = p.row_t + m0 * p.ld_row_t;
+                    float* dst = low_smem + quad * 4 * C::kLowPitch;
+                    if (a[0] >= 0 && a[0] == a[1] && a[0] == a[2] && a[0] == a[3]) {      // rows past the end have no adapter
+                        const uint16_t* const one[1] = {b[0]};
+                        if (p.lora_bf16) low_rank_rows<true, 1, 4>(rows_t, p.ld_row_t, {0}, {4}, one, cols, p.row_r, dst, C::kLowPitch, lane);
+                        else low_rank_rows<false, 1, 4>(rows_t, p.ld_row_t, {0}, {4}, one, cols, p.row_r, dst, C::kLowPitch, lane);
+                    } else {
+                        if (p.lora_bf16) low_rank_rows<true, 4, 2>(rows_t, p.ld_row_t, {0, 1, 2, 3}, {1, 1, 1, 1}, b, cols, p.row_r, dst, C::kLowPitch, lane);
+                        else low_rank_rows<false, 4, 2>(rows_t, p.ld_row_t, {0, 1, 2, 3}, {1, 1, 1, 1}, b, cols, p.row_r, dst, C::kLowPitch, lane);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(low_full);
+            }
+            if (ksplit) {
+                cluster_arrive();
+                cluster_wait();
+                cluster_arrive();
+                cluster_wait();
+            }
+        }
     } else {
         const int quarter = warp & 3;  // TMEM lanes [32*quarter, 32*quarter+32) belong to this warp
         float* col_scale = epi_smem + (warp - 2) * 2 * BN;
         float* col_bias = col_scale + BN;
         int buf = 0;
         uint32_t acc_phase = 0;
+        uint32_t low_phase = 0;
         const bool dequant = p.epi_mode == kEpiDequant;
         const bool per_ch = dequant && p.w_scale_mode == I8F_WSCALE_CHANNEL;
         const bool has_bias = dequant && p.bias != nullptr;
@@ -716,6 +813,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 has_addend = row_ok && __ldg(p.row_adapter + row) >= 0;
                 addend_row = p.addend + row * p.ld_addend;
             }
+            if constexpr (EXTRA == kExtraRows) {
+                has_addend = row_ok && __ldg(p.row_adapter + row) >= 0;
+                addend_row = low_smem + (quarter * 32 + lane) * C::kLowPitch;
+            }
             if constexpr (EXTRA == kExtraRequests) {
                 const bool with_adapter = row_ok && __ldg(p.row_adapter + row) >= 0;
                 const int addend_row0 = p.req_tiles[m_blk].addend_row;
@@ -762,6 +863,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     if (krank == 1 || !acc_ok) break;
                 }
             }
+            if constexpr (EXTRA == kExtraRows) {
+                if (!mbar_wait_bounded(low_full, low_phase, abort_flag, p.status, kStLowFullWait)) break;
+                low_phase ^= 1u;
+            }
             const uint32_t t_lora = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(C::kLoraCol);
             bool released = false;
 #pragma unroll 1
@@ -771,6 +876,17 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 tmem_ld_32x32(t_addr + c * 32, v);
                 uint32_t lv[EXTRA != kExtraNone ? 32 : 1];
                 if constexpr (LORA) tmem_ld_32x32(t_lora + c * 32, lv);
+                if constexpr (EXTRA == kExtraRows) {
+                    const uint4* src = reinterpret_cast<const uint4*>(addend_row + c * 32);
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        const uint4 o = has_addend ? src[g] : make_uint4(0u, 0u, 0u, 0u);
+                        lv[4 * g] = o.x;
+                        lv[4 * g + 1] = o.y;
+                        lv[4 * g + 2] = o.z;
+                        lv[4 * g + 3] = o.w;
+                    }
+                }
                 if constexpr (EXTRA == kExtraAddend) {   // ld_addend is a multiple of 32: a whole chunk is always there
                     const uint4* src = reinterpret_cast<const uint4*>(addend_row + col);
 #pragma unroll
@@ -873,6 +989,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     }
                     ++out_chunk;
                 }
+            }
+            if constexpr (EXTRA == kExtraRows) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(low_empty);
             }
             if (!released) {   // a warp whose share lies past N read nothing
                 tc_fence_before_sync();
@@ -1289,6 +1409,10 @@ int launch_gemm_auto(const void* a, int64_t lda, const void* b, int64_t ldb, int
     switch (plan.choice) {
         case 1: return launch_gemm<KIND, 256, true, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter);
         case 2: return launch_gemm<KIND, 256, false, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
+        default: break;
+    }
+    if constexpr (EXTRA != kExtraNone) return fail(I8F_ERR_INVALID_ARG, "no such tile");
+    else switch (plan.choice) {
         case 3: return launch_gemm<KIND, 128, false, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
         case 5: return launch_gemm<KIND, 32, false, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
         default: return launch_gemm<KIND, 64, false, EXTRA>(a, lda, b, ldb, M, N, K, p, st, scatter, nullptr, k_split);
@@ -1386,7 +1510,20 @@ static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, 
         p.addend = term->addend;
         p.ld_addend = term->ld_addend;
         p.row_adapter = term->row_adapter;
-        if (term->tiles == nullptr) return launch_gemm_auto<kKindI8, kExtraAddend>(a, lda, w, ldw, M, N, K, p, st);
+        if (term->tiles == nullptr) {
+            const GemmPlan plan = plan_gemm(M, N, K, 1, sm_count(), false, forced_tile(), ksplit_enabled());
+            if (plan.choice < 3) return launch_gemm_auto<kKindI8, kExtraAddend>(a, lda, w, ldw, M, N, K, p, st);
+            p.row_t = static_cast<const uint16_t*>(term->t);
+            p.ld_row_t = term->ldt;
+            p.row_b = static_cast<const uint16_t*>(term->b);
+            p.row_r = static_cast<int>(term->r);
+            p.early_b = term->after_own ? 1 : 0;
+            p.lora_n = N;
+            p.lora_bf16 = out_dtype == I8F_BF16 ? 1 : 0;
+            if (plan.choice == 3) return launch_gemm<kKindI8, 128, false, kExtraRows>(a, lda, w, ldw, M, N, K, p, st, nullptr, nullptr, plan.k_split);
+            if (plan.choice == 5) return launch_gemm<kKindI8, 32, false, kExtraRows>(a, lda, w, ldw, M, N, K, p, st, nullptr, nullptr, plan.k_split);
+            return launch_gemm<kKindI8, 64, false, kExtraRows>(a, lda, w, ldw, M, N, K, p, st, nullptr, nullptr, plan.k_split);
+        }
         p.req_tiles = term->tiles;
         p.req_slots = term->slots;
         const LoraOperands lo{term->t, term->ldt, term->b, term->r, term->r, out_dtype == I8F_BF16 ? kKindBF16 : kKindF16, term->adapters};
@@ -1574,6 +1711,10 @@ int i8f_lora_up_add(const void* t, int64_t ldt, const void* lora_b, int64_t ldb,
 }  // extern "C"
 
 namespace i8f {
+
+bool requests_need_addend(int64_t M, int64_t N, int64_t K) {
+    return plan_gemm(M, N, K, 1, sm_count(), false, forced_tile(), ksplit_enabled()).choice < 3;
+}
 
 int linear_w8a8_requests(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
                          int w_scale_mode, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M,

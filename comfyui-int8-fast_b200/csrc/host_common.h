@@ -53,8 +53,9 @@ struct RequestSlot {
     uint32_t rows[8];
 };
 
-// The low-rank term of a batch of requests beside the int8 product.  `tiles` NULL: all of it is in `addend`
-// [M, ld_addend]; else the tiles say where theirs comes from.  ld_addend is a multiple of 32, the addend 16-byte aligned.
+// The low-rank term of a batch of requests beside the int8 product.  `tiles` NULL: a small batch, whose rows' terms the kernel
+// works out itself beside the MMAs, or, where requests_need_addend() says so, finds in `addend` [M, ld_addend]; else the
+// tiles say where theirs comes from.  ld_addend is a multiple of 32, the addend 16-byte aligned.
 struct RequestTerm {
     const int* row_adapter;
     const float* addend;
@@ -65,17 +66,24 @@ struct RequestTerm {
     int64_t ldt;
     const void* b;       // [adapters, N, r]
     int64_t adapters, r;
+    // the kernel before this one in the stream is the library's own and started when everything before it was complete, so
+    // the weights and banks may be read beside its tail
+    bool after_own;
 };
+
+// Whether the product of these sizes runs on 256-wide tiles, whose epilogue has no room for rows worked out beside it.
+bool requests_need_addend(int64_t M, int64_t N, int64_t K);
 
 // i8f_linear_w8a8 with such a term; in gemm_tcgen05.cu.  With `check_only` the arguments are checked and nothing is
 // launched, so that a caller can refuse a bad call before it launches what comes first.
 int linear_w8a8_requests(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
                          int w_scale_mode, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M,
                          int64_t N, int64_t K, int epilogue_order, const RequestTerm& term, bool check_only, cudaStream_t stream);
-// i8f_linear_w8a16_small with an fp32 addend on the rows with an adapter; in linear_small_m.cu.
-int linear_small_addend(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
-                        const void* bias, int bias_dtype, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
-                        const float* addend, int64_t ld_addend, const int* row_adapter, bool check_only, cudaStream_t stream);
+// i8f_linear_w8a16_small with the low-rank term of each row's adapter (row_adapter, t, b, r of `term`); in linear_small_m.cu.
+// The kernel before it in the stream may only be the one that writes t.
+int linear_small_requests(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
+                          const void* bias, int bias_dtype, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                          const RequestTerm& term, bool check_only, cudaStream_t stream);
 
 }  // namespace i8f
 

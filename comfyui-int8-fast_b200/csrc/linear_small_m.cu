@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 
 #include "host_common.h"
+#include "low_rank.cuh"
 
 namespace i8f {
 namespace {
@@ -136,22 +137,26 @@ __device__ __forceinline__ void consume_chunk(const uint4& wlo, const uint4& whi
 // stand-in (the last feature / token 0) instead of carrying predicates; those results are never stored.
 // kDepth: weight chunks in flight per lane (a register ring); the activations (L1/L2 hits) are fetched per chunk.
 //
-// REQ: the form beside per-request adapters, y = dt(scale * (x . w^T) + bias + addend) with an fp32 addend [M, ld_addend] on
-// the rows whose row_adapter is not negative.  The weights enter the product as the integers they are (exact in bf16 and
+// REQ: the form beside per-request adapters, y = dt(scale * (x . w^T) + bias + t[m] . B_a(m)^T) for the rows whose adapter
+// a(m) is not negative; each warp works the low-rank term of its rows out for the block's features (low_rank.cuh) before the
+// partial sums meet.  t comes from the kernel before this one, whose tail the products overlap.  The weights enter the product as the integers they are (exact in bf16 and
 // fp16, and one multiply per weight less) and everything is rounded once, at the end; the plain form keeps the
 // reference's roundings of the scaled weight and of the bias.
-struct SmallAddend {
-    const float* addend;
-    int64_t ld;
+struct SmallTerm {
     const int* row_adapter;
+    const uint16_t* t;
+    int64_t ldt;
+    const uint16_t* b;
+    int r;
 };
 template <int DT, bool HI_ROWS, int kDepth, bool REQ>
 __global__ void __launch_bounds__(kThreads, HI_ROWS ? 3 : 4)
 small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict__ w, int64_t ldw,
                const float* __restrict__ w_scale, int per_row, const void* __restrict__ bias, int bias_dt,
-               void* __restrict__ out, int64_t ldo, int M, int64_t N, int64_t K, const SmallAddend req) {
+               void* __restrict__ out, int64_t ldo, int M, int64_t N, int64_t K, const SmallTerm req) {
     constexpr int kHalves = HI_ROWS ? 2 : 1;
     __shared__ float4 s_part[2][kWarps][kHalves][32];
+    __shared__ float s_low[REQ ? 2 : 1][REQ ? kMaxSmallM : 1][17];      // the block's low-rank rows, buffered as s_part is
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int64_t n_blocks = (N + 15) / 16;
@@ -186,7 +191,22 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
 
     int64_t nb = blockIdx.x;          // the grid never exceeds the number of blocks
     open_block(nb, sc_lo, sc_hi);
+    int64_t my_adapter[kHalves];      // of the rows whose low-rank term this warp works out
+    if constexpr (REQ) {
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) my_adapter[h] = warp + h * kWarps < M ? __ldg(req.row_adapter + warp + h * kWarps) : -1;
+    }
     for (int iter = 0;; ++iter) {
+        if constexpr (REQ) {
+            // the block's rows of B are on their way to L2 while its weights stream
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                const int64_t n = nb * 16 + (lane >> 1);
+                if (my_adapter[h] >= 0 && n < N)
+                    for (int e = (lane & 1) * 64; e < req.r; e += 128)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(req.b + (my_adapter[h] * N + n) * req.r + e));
+            }
+        }
         float acc[kHalves][4];
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) acc[h][0] = acc[h][1] = acc[h][2] = acc[h][3] = 0.0f;
@@ -240,6 +260,20 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
             s_part[buf][warp][h][lane] = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
+        if constexpr (REQ) {
+            if (iter == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+            const int cols = static_cast<int>(N - nb * 16 < 16 ? N - nb * 16 : 16);
+            // rows warp and warp + 8 together
+            const uint16_t* b[kHalves];
+            int at[kHalves], one[kHalves];
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                b[h] = my_adapter[h] >= 0 ? req.b + (my_adapter[h] * N + nb * 16) * req.r : nullptr;      // rows past M have none
+                at[h] = warp + h * kWarps;
+                one[h] = 1;
+            }
+            low_rank_rows<DT == I8F_BF16, kHalves, 1>(req.t, req.ldt, at, one, b, cols, req.r, s_low[buf][0], 17, lane);
+        }
         __syncthreads();
         const int first = (iter * kHalves) % kWarps;     // the summing duty rotates over the warps
         if (warp >= first && warp < first + kHalves) {
@@ -259,7 +293,7 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
                 if (REQ && m < M && n < N) {
                     float r = v[e] * (per_row ? __ldg(w_scale + n) : __ldg(w_scale));
                     if (bias != nullptr) r += load_bias(bias, bias_dt, n);
-                    if (__ldg(req.row_adapter + m) >= 0) r += __ldg(req.addend + m * req.ld + n);
+                    if (__ldg(req.row_adapter + m) >= 0) r += s_low[buf][m][g + (e >> 1) * 8];
                     store_dt<DT>(out, static_cast<int64_t>(m) * ldo + n, r);
                 } else if (m < M && n < N) {
                     const float b = bias != nullptr ? round_dt<DT>(load_bias(bias, bias_dt, n)) : 0.0f;
@@ -277,7 +311,7 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
 template <int DT, bool REQ = false>
 int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int per_row,
                    const void* bias, int bias_dt, void* out, int64_t ldo, int M, int64_t N, int64_t K,
-                   cudaStream_t stream, const SmallAddend& req = SmallAddend{}) {
+                   cudaStream_t stream, const SmallTerm& req = SmallTerm{}) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -295,7 +329,21 @@ int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, con
     }
     const int64_t resident = static_cast<int64_t>(per_sm) * sms;
     const int grid = static_cast<int>(blocks < resident ? blocks : resident);
-    kernel<<<grid, kThreads, 0, stream>>>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, req);
+    if constexpr (REQ) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+        cfg.blockDim = dim3(kThreads, 1, 1);
+        cfg.stream = stream;
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, req);
+        if (e != cudaSuccess) return fail(I8F_ERR_CUDA, "small_m_kernel launch: %s", cudaGetErrorString(e));
+    } else {
+        kernel<<<grid, kThreads, 0, stream>>>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, req);
+    }
     return check_launch("small_m_kernel");
 }
 
@@ -341,14 +389,15 @@ extern "C" int i8f_linear_w8a16_small(const void* x, int x_dtype, int64_t ldx, c
 
 namespace i8f {
 
-int linear_small_addend(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
-                        const void* bias, int bias_dtype, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
-                        const float* addend, int64_t ld_addend, const int* row_adapter, bool check_only, cudaStream_t stream) {
+int linear_small_requests(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int w_scale_mode,
+                          const void* bias, int bias_dtype, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                          const RequestTerm& term, bool check_only, cudaStream_t stream) {
     bool empty;
     const int rc = check_small(x, x_dtype, ldx, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, ldo, M, N, K, &empty);
     if (rc != I8F_OK || empty || check_only) return rc;
     const int per_row = w_scale_mode == I8F_WSCALE_CHANNEL;
-    const SmallAddend req{addend, ld_addend, row_adapter};
+    const SmallTerm req{term.row_adapter, static_cast<const uint16_t*>(term.t), term.ldt, static_cast<const uint16_t*>(term.b),
+                        static_cast<int>(term.r)};
     if (x_dtype == I8F_BF16)
         return dispatch_small<I8F_BF16, true>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dtype, out, ldo, static_cast<int>(M), N,
                                               K, stream, req);

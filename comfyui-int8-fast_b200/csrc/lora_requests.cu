@@ -15,104 +15,156 @@
 #include <cuda_fp16.h>
 
 #include "host_common.h"
+#include "low_rank.cuh"
 #include "ptx_sm100.cuh"
 #include "tensor_maps.h"
 
 namespace i8f {
 namespace {
 
-constexpr int kChunkRows = 4;
+constexpr int kChunkRows = kLowRankRows;
 
 static_assert(sizeof(RequestTile) == 16 && sizeof(RequestSlot) == 48, "layout of the plan's tables");
 
-template <int DT>
-__device__ __forceinline__ void unpack8(const uint4& r, float (&v)[8]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (DT == I8F_BF16) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
-    }
-}
 template <int DT>
 __device__ __forceinline__ void store_dt(void* out, int64_t idx, float v) {
     if constexpr (DT == I8F_BF16) static_cast<__nv_bfloat16*>(out)[idx] = __float2bfloat16_rn(v);
     else static_cast<__half*>(out)[idx] = __float2half_rn(v);
 }
 
-// One warp per (chunk, rank row): the dot products of the chunk's rows with one row of its adapter's A.  Bound by the
-// bytes of A; x comes from L2.  A chunk without an adapter gets zeros.
-template <int DT>
-__global__ void __launch_bounds__(128)
-down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ bank_a, int64_t K, int64_t r,
-                   const int4* __restrict__ chunks, void* __restrict__ t, int64_t ldt) {
-    const int lane = threadIdx.x & 31;
+// ------------------------------------------------------------------ chunks: ordinary warps
+// t of one chunk for RB rank rows of its adapter, by a CTA: every thread takes the same eight columns of the chunk's rows of x
+// and of the RB rows of A, 256 threads side by side, so a CTA's share of A is in flight at once.  Bound by the bytes of A and,
+// for few chunks, by one trip to memory; x is read again by the other rank rows' CTAs from L2.  A chunk without an
+// adapter gets zeros.
+// QUANT: the CTAs of the first rank rows also turn the chunk's rows into int8 (the arithmetic of i8f_quant_rowwise: step =
+// max(absmax / 127, 1e-30), rint(x * (1 / step))), which saves a small batch a launch of its own for that.
+constexpr int kChunkThreads = 256;
+constexpr int kChunkWarps = kChunkThreads / 32;
+
+struct QuantOut {
+    int8_t* q;
+    int64_t ldq;
+    float* scale;
+};
+
+template <int DT, int RB, bool QUANT>
+__global__ void __launch_bounds__(kChunkThreads)
+down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ bank_a, int K, int r,
+                   const int4* __restrict__ chunks, void* __restrict__ t, int64_t ldt, const QuantOut out) {
+    constexpr int kValues = RB * kChunkRows;
+    __shared__ float s_part[kChunkWarps][kValues];
+    __shared__ uint32_t s_max[kChunkWarps][kChunkRows];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 c = chunks[blockIdx.x];      // first row, rows, adapter
-    const int64_t j = static_cast<int64_t>(blockIdx.y) * 4 + (threadIdx.x >> 5);
-    if (j >= r) return;
-    float acc[kChunkRows] = {0.f, 0.f, 0.f, 0.f};
+    const int j0 = blockIdx.y * RB;
+    const int nvec = K >> 3;
+    const uint16_t* const x0 = static_cast<const uint16_t*>(x) + c.x * ldx;
     if (c.z >= 0) {
-        const uint4* a = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(bank_a) + (c.z * r + j) * K);
-        const uint16_t* x0 = static_cast<const uint16_t*>(x) + c.x * ldx;
-        const int64_t nvec = K >> 3;
-#pragma unroll 4
-        for (int64_t v = lane; v < nvec; v += 32) {
-            float fa[8];
-            unpack8<DT>(__ldg(a + v), fa);
+        float acc[RB][kChunkRows];
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+#pragma unroll
+            for (int m = 0; m < kChunkRows; ++m) acc[j][m] = 0.f;
+        const uint4* const a = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(bank_a) + (static_cast<int64_t>(c.z) * r + j0) * K);
+#pragma unroll 2
+        for (int v = threadIdx.x; v < nvec; v += kChunkThreads) {
+            uint4 ra[RB], rx[kChunkRows];
+#pragma unroll
+            for (int j = 0; j < RB; ++j) ra[j] = __ldg(a + static_cast<int64_t>(j) * nvec + v);
+#pragma unroll
+            for (int m = 0; m < kChunkRows; ++m)
+                rx[m] = m < c.y ? __ldg(reinterpret_cast<const uint4*>(x0 + m * ldx) + v) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
             for (int m = 0; m < kChunkRows; ++m) {
                 if (m < c.y) {
                     float fx[8];
-                    unpack8<DT>(__ldg(reinterpret_cast<const uint4*>(x0 + m * ldx) + v), fx);
+                    widen8<DT == I8F_BF16>(rx[m], fx);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) acc[m] = fmaf(fx[e], fa[e], acc[m]);
+                    for (int j = 0; j < RB; ++j) {
+                        float fa[8];
+                        widen8<DT == I8F_BF16>(ra[j], fa);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) acc[j][m] = fmaf(fx[e], fa[e], acc[j][m]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+#pragma unroll
+            for (int m = 0; m < kChunkRows; ++m) {
+                if (m < c.y) {
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) acc[j][m] += __shfl_xor_sync(0xFFFFFFFFu, acc[j][m], d);
+                    if (lane == 0) s_part[warp][j * kChunkRows + m] = acc[j][m];
                 }
             }
         }
     }
-#pragma unroll
-    for (int m = 0; m < kChunkRows; ++m) {
-#pragma unroll
-        for (int d = 16; d; d >>= 1) acc[m] += __shfl_xor_sync(0xFFFFFFFFu, acc[m], d);
-        if (lane == 0 && m < c.y) store_dt<DT>(t, (static_cast<int64_t>(c.x) + m) * ldt + j, acc[m]);
+    const bool quant = QUANT && blockIdx.y == 0;
+    if (quant) {
+        // 16-bit patterns without their sign order like the values
+        for (int m = 0; m < c.y; ++m) {
+            uint32_t m2 = 0u;
+            for (int v = threadIdx.x; v < nvec; v += kChunkThreads) {
+                const uint4 w = __ldg(reinterpret_cast<const uint4*>(x0 + m * ldx) + v);
+                m2 = __vmaxu2(__vmaxu2(__vmaxu2(m2, w.x & 0x7FFF7FFFu), __vmaxu2(w.y & 0x7FFF7FFFu, w.z & 0x7FFF7FFFu)), w.w & 0x7FFF7FFFu);
+            }
+            const uint32_t big = __reduce_max_sync(0xFFFFFFFFu, max(m2 & 0xFFFFu, m2 >> 16));
+            if (lane == 0) s_max[warp][m] = big;
+        }
     }
-}
-
-// One thread per (chunk, output column): the chunk's rows of t against one row of its adapter's B, into the fp32 addend of
-// the int8 product's epilogue.  Bound by the bytes of B.  Rows without an adapter are not written.
-template <int DT>
-__global__ void __launch_bounds__(128)
-up_chunks_kernel(const void* __restrict__ t, int64_t ldt, const void* __restrict__ bank_b, int64_t N, int64_t r,
-                 const int4* __restrict__ chunks, float* __restrict__ addend, int64_t ld_addend) {
-    const int4 c = chunks[blockIdx.x];      // first row, rows, adapter, first row in the addend
-    const int64_t n = static_cast<int64_t>(blockIdx.y) * 128 + threadIdx.x;
-    if (c.z < 0 || n >= N) return;
-    const uint4* b = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(bank_b) + (c.z * N + n) * r);
-    const uint16_t* t0 = static_cast<const uint16_t*>(t) + c.x * ldt;
-    float acc[kChunkRows] = {0.f, 0.f, 0.f, 0.f};
-    const int nvec = static_cast<int>(r >> 3);
-    for (int v = 0; v < nvec; ++v) {
-        float fb[8];
-        unpack8<DT>(__ldg(b + v), fb);
+    __syncthreads();
+    if (threadIdx.x < kValues) {
+        const int j = threadIdx.x / kChunkRows, m = threadIdx.x % kChunkRows;
+        if (m < c.y) {
+            float v = 0.f;
+            if (c.z >= 0)
+                for (int w = 0; w < kChunkWarps; ++w) v += s_part[w][threadIdx.x];
+            store_dt<DT>(t, (static_cast<int64_t>(c.x) + m) * ldt + j0 + j, v);
+        }
+    }
+    if (quant) {
+        constexpr float kMagic = 12582912.0f;      // 1.5 * 2^23
+        for (int m = 0; m < c.y; ++m) {
+            uint32_t big = s_max[0][m];
 #pragma unroll
-        for (int m = 0; m < kChunkRows; ++m) {
-            if (m < c.y) {
-                float ft[8];
-                unpack8<DT>(__ldg(reinterpret_cast<const uint4*>(t0 + m * ldt) + v), ft);
+            for (int w = 1; w < kChunkWarps; ++w) big = max(big, s_max[w][m]);
+            const float amax = DT == I8F_BF16 ? __uint_as_float(big << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(big)));
+            const float step = fmaxf(__fdiv_rn(amax, 127.0f), 1e-30f);
+            const float inv = __fdiv_rn(1.0f, step);
+            const int64_t row = static_cast<int64_t>(c.x) + m;
+            if (threadIdx.x == 0) out.scale[row] = step;
+            for (int v = threadIdx.x; v < nvec; v += kChunkThreads) {
+                float f[8];
+                uint32_t u[8];
+                widen8<DT == I8F_BF16>(__ldg(reinterpret_cast<const uint4*>(x0 + m * ldx) + v), f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc[m] = fmaf(ft[e], fb[e], acc[m]);
+                for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__fadd_rn(__fmul_rn(f[e], inv), kMagic)) & 0xFFu;
+                *reinterpret_cast<uint2*>(out.q + row * out.ldq + v * 8) =
+                    make_uint2(u[0] | (u[1] << 8) | (u[2] << 16) | (u[3] << 24), u[4] | (u[5] << 8) | (u[6] << 16) | (u[7] << 24));
             }
         }
     }
-#pragma unroll
-    for (int m = 0; m < kChunkRows; ++m)
-        if (m < c.y) addend[(static_cast<int64_t>(c.w) + m) * ld_addend + n] = acc[m];
+}
+
+// The up projection of the chunks into the fp32 addend of the int8 product's epilogue: one warp per (chunk, 64 columns).
+// Bound by the bytes of B.  Rows without an adapter are not written.
+constexpr int kUpCols = 64;
+template <int DT>
+__global__ void __launch_bounds__(128)
+up_chunks_kernel(const void* __restrict__ t, int64_t ldt, const void* __restrict__ bank_b, int N, int r,
+                 const int4* __restrict__ chunks, float* __restrict__ addend, int64_t ld_addend) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 c = chunks[blockIdx.x];      // first row, rows, adapter, first row in the addend
+    const int n0 = (blockIdx.y * 4 + (threadIdx.x >> 5)) * kUpCols;
+    if (c.z < 0 || n0 >= N) return;
+    const uint16_t* const b[1] = {static_cast<const uint16_t*>(bank_b) + (static_cast<int64_t>(c.z) * N + n0) * r};
+    low_rank_rows<DT == I8F_BF16, 1, 4>(static_cast<const uint16_t*>(t) + c.x * ldt, ldt, {0}, {c.y}, b, min(kUpCols, N - n0), r,
+                                        addend + static_cast<int64_t>(c.w) * ld_addend + n0, ld_addend, threadIdx.x & 31);
 }
 
 // ------------------------------------------------------------------ down projection on the tensor cores
@@ -460,21 +512,45 @@ int launch_down_tiles(const void* x, int64_t ldx, const void* bank_a, int64_t ad
     return check_launch("down_tiles_kernel");
 }
 
+// `out`: also quantise the rows (only where the chunks cover the whole batch).
 int launch_down_chunks(const void* x, int64_t ldx, const void* bank_a, int64_t r, const i8f_request_rows* rows, void* t, int64_t ldt,
-                       int dtype, int64_t K, cudaStream_t st) {
-    const dim3 grid(static_cast<unsigned>(rows->n_chunks), static_cast<unsigned>((r + 3) / 4));
+                       int dtype, int64_t K, const QuantOut* out, cudaStream_t st) {
     const int4* chunks = reinterpret_cast<const int4*>(rows->chunks);
-    if (dtype == I8F_BF16) down_chunks_kernel<I8F_BF16><<<grid, 128, 0, st>>>(x, ldx, bank_a, K, r, chunks, t, ldt);
-    else down_chunks_kernel<I8F_F16><<<grid, 128, 0, st>>>(x, ldx, bank_a, K, r, chunks, t, ldt);
+    // two rank rows per CTA where the chunks alone would leave SMs idle, else eight (x is then read a quarter as often)
+    const bool few = rows->n_chunks * (r / 8) < 2 * sm_count();
+    const dim3 grid(static_cast<unsigned>(rows->n_chunks), static_cast<unsigned>(r / (few ? 2 : 8)));
+    const QuantOut q = out != nullptr ? *out : QuantOut{};
+    const int k = static_cast<int>(K), rank = static_cast<int>(r);
+#define I8F_DOWN(DT, RB, Q) down_chunks_kernel<DT, RB, Q><<<grid, kChunkThreads, 0, st>>>(x, ldx, bank_a, k, rank, chunks, t, ldt, q)
+#define I8F_DOWN_RB(DT)                                     \
+    do {                                                    \
+        if (few && out != nullptr) I8F_DOWN(DT, 2, true);   \
+        else if (few) I8F_DOWN(DT, 2, false);               \
+        else if (out != nullptr) I8F_DOWN(DT, 8, true);     \
+        else I8F_DOWN(DT, 8, false);                        \
+    } while (0)
+    if (dtype == I8F_BF16) I8F_DOWN_RB(I8F_BF16);
+    else I8F_DOWN_RB(I8F_F16);
+#undef I8F_DOWN_RB
+#undef I8F_DOWN
     return check_launch("down_chunks_kernel");
 }
 
 int launch_up_chunks(const void* t, int64_t ldt, const void* bank_b, int64_t r, const i8f_request_rows* rows, int dtype, int64_t N,
                      float* addend, cudaStream_t st) {
-    const dim3 grid(static_cast<unsigned>(rows->n_chunks), static_cast<unsigned>((N + 127) / 128));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows->n_chunks), static_cast<unsigned>((N + 4 * kUpCols - 1) / (4 * kUpCols)));
+    cfg.blockDim = dim3(128, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
     const int4* chunks = reinterpret_cast<const int4*>(rows->chunks);
-    if (dtype == I8F_BF16) up_chunks_kernel<I8F_BF16><<<grid, 128, 0, st>>>(t, ldt, bank_b, N, r, chunks, addend, addend_pitch(N));
-    else up_chunks_kernel<I8F_F16><<<grid, 128, 0, st>>>(t, ldt, bank_b, N, r, chunks, addend, addend_pitch(N));
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, dtype == I8F_BF16 ? up_chunks_kernel<I8F_BF16> : up_chunks_kernel<I8F_F16>, t, ldt, bank_b,
+                                             static_cast<int>(N), static_cast<int>(r), chunks, addend, addend_pitch(N));
+    if (e != cudaSuccess) return fail(I8F_ERR_CUDA, "up_chunks_kernel launch: %s", cudaGetErrorString(e));
     return check_launch("up_chunks_kernel");
 }
 
@@ -484,7 +560,7 @@ int launch_down(const void* x, int64_t ldx, const void* bank_a, int64_t adapters
         const int rc = launch_down_tiles(x, ldx, bank_a, adapters, r, rows, t, ldt, dtype, M, K, after_reader, st);
         if (rc != I8F_OK) return rc;
     }
-    return has_chunks(rows) ? launch_down_chunks(x, ldx, bank_a, r, rows, t, ldt, dtype, K, st) : I8F_OK;
+    return has_chunks(rows) ? launch_down_chunks(x, ldx, bank_a, r, rows, t, ldt, dtype, K, nullptr, st) : I8F_OK;
 }
 
 RequestTerm request_term(const void* t, int64_t ldt, const void* bank_b, int64_t adapters, int64_t r, const i8f_request_rows* rows,
@@ -543,7 +619,7 @@ int i8f_linear_w8a8_lora_requests(const int8_t* a, int64_t lda, const float* a_s
     float* addend = static_cast<float*>(workspace);
     const RequestTerm term = request_term(t, ldt, bank_b, adapters, r, rows, N, addend);
     for (const bool check_only : {true, false}) {     // everything is checked before anything is launched
-        if (!check_only && has_chunks(rows)) {
+        if (!check_only && has_chunks(rows) && (has_dense(rows) || requests_need_addend(M, N, K))) {
             rc = launch_up_chunks(t, ldt, bank_b, r, rows, out_dtype, N, addend, st);
             if (rc != I8F_OK) return rc;
         }
@@ -600,15 +676,21 @@ int i8f_linear_lora_requests(const void* x, int x_dtype, int64_t ldx, int hadama
     if (rc != I8F_OK) return rc;
     rc = check_up(t, r, bank_b, adapters, r, rows, x_dtype, N);
     if (rc != I8F_OK) return rc;
-    const RequestTerm term = request_term(t, r, bank_b, adapters, r, rows, N, addend);
+    RequestTerm term = request_term(t, r, bank_b, adapters, r, rows, N, addend);
+    term.after_own = true;
     rc = linear_w8a8_requests(q, K, q_scale, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, x_dtype, ldo, M, N, K, epilogue_order,
                               term, true, st);
     if (rc != I8F_OK) return rc;
-    rc = i8f_quant_rowwise(x, x_dtype, M, K, ldx, q, K, q_scale, hadamard128, rotated, stream);
+    if (!has_dense(rows) && !hadamard128) {
+        const QuantOut out_q{q, K, q_scale};
+        rc = launch_down_chunks(x, ldx, bank_a, r, rows, t, r, x_dtype, K, &out_q, st);
+    } else {
+        rc = i8f_quant_rowwise(x, x_dtype, M, K, ldx, q, K, q_scale, hadamard128, rotated, stream);
+        if (rc != I8F_OK) return rc;
+        rc = launch_down(lora_in, ldx, bank_a, adapters, r, rows, t, r, x_dtype, M, K, !keep_rotated, st);
+    }
     if (rc != I8F_OK) return rc;
-    rc = launch_down(lora_in, ldx, bank_a, adapters, r, rows, t, r, x_dtype, M, K, !keep_rotated, st);
-    if (rc != I8F_OK) return rc;
-    if (has_chunks(rows)) {
+    if (has_chunks(rows) && (has_dense(rows) || requests_need_addend(M, N, K))) {
         rc = launch_up_chunks(t, r, bank_b, r, rows, x_dtype, N, addend, st);
         if (rc != I8F_OK) return rc;
     }
@@ -618,7 +700,7 @@ int i8f_linear_lora_requests(const void* x, int x_dtype, int64_t ldx, int hadama
 
 size_t i8f_linear_w8a16_small_lora_requests_workspace_bytes(const i8f_request_rows* rows, int64_t N, int64_t r) {
     if (rows == nullptr || rows->rows <= 0 || N <= 0 || r <= 0) return 0;
-    return padded(static_cast<size_t>(rows->rows) * static_cast<size_t>(r) * 2) + addend_bytes(rows, N);
+    return static_cast<size_t>(rows->rows) * static_cast<size_t>(r) * 2;
 }
 
 int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale,
@@ -628,8 +710,8 @@ int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx
     int rc = check_rows(rows, M);
     if (rc != I8F_OK || M == 0 || N == 0) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = linear_small_addend(x, x_dtype, ldx, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, ldo, M, N, K, nullptr, 0, nullptr, true,
-                             st);
+    const RequestTerm term = request_term(workspace, r, bank_b, adapters, r, rows, N, nullptr);
+    rc = linear_small_requests(x, x_dtype, ldx, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, ldo, M, N, K, term, true, st);
     if (rc != I8F_OK) return rc;
     I8F_REQUIRE(!has_dense(rows), I8F_ERR_INVALID_ARG, "a row plan of at most 16 rows has chunks only");
     rc = check_bank(bank_a, adapters, r, rows, x_dtype, "bank_a");
@@ -638,17 +720,13 @@ int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx
     I8F_REQUIRE(workspace != nullptr && workspace_bytes >= need, I8F_ERR_WORKSPACE, "workspace too small: have %zu bytes, need %zu",
                 workspace_bytes, need);
     I8F_REQUIRE(aligned16(workspace), I8F_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-    float* addend = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + need - addend_bytes(rows, N));
     rc = check_down(x, ldx, bank_a, adapters, r, rows, workspace, r, x_dtype, K);
     if (rc != I8F_OK) return rc;
     rc = check_up(workspace, r, bank_b, adapters, r, rows, x_dtype, N);
     if (rc != I8F_OK) return rc;
-    rc = launch_down_chunks(x, ldx, bank_a, r, rows, workspace, r, x_dtype, K, st);
+    rc = launch_down_chunks(x, ldx, bank_a, r, rows, workspace, r, x_dtype, K, nullptr, st);
     if (rc != I8F_OK) return rc;
-    rc = launch_up_chunks(workspace, r, bank_b, r, rows, x_dtype, N, addend, st);
-    if (rc != I8F_OK) return rc;
-    return linear_small_addend(x, x_dtype, ldx, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, ldo, M, N, K, addend,
-                               addend_pitch(N), rows->row_adapter, false, st);
+    return linear_small_requests(x, x_dtype, ldx, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, ldo, M, N, K, term, false, st);
 }
 
 }  // extern "C"

@@ -44,9 +44,18 @@ _SAME_DEVICE = contextlib.nullcontext()
 
 def _on(device: torch.device):
     """Context in which `device`, a sm_100 device, is the current one (the C ABI launches on the current device)."""
-    if device.type != "cuda" or device.index not in nat.device_ok:
+    idx = device.index
+    if idx not in nat.device_ok or device.type != "cuda":
         nat.require_device(device)
-    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _SAME_DEVICE if idx == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _pitched(t: Tensor) -> tuple[Tensor, int]:
+    """2-D view with unit inner stride and its row pitch in elements."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t, t.shape[1] or 1
+    t = _rows(t)
+    return t, _ld(t)
 
 
 _WORKSPACE_BYTES: dict = {}
@@ -428,22 +437,23 @@ def lora_up_add_(y: Tensor, t: Tensor, lora_b: Tensor) -> Tensor:
 
 def _check_requests(rows: RequestRows, x: Tensor, lora_a: Tensor | None, lora_b: Tensor | None, dtype: torch.dtype, K: int, N: int):
     """The row plan and the bank of adapters against the call; returns (adapters, rank)."""
-    if rows.device != x.device:
-        raise ValueError(f"the row plan is on {rows.device}, the activations on {x.device}")
+    device = x.device
+    if rows.device != device:
+        raise ValueError(f"the row plan is on {rows.device}, the activations on {device}")
     if rows.total != x.shape[0]:
         raise ValueError(f"the row plan is for {rows.total} rows, the call has {x.shape[0]}")
-    n = r = None
-    for name, bank, inner in (("lora_a", lora_a, (1, K)), ("lora_b", lora_b, (2, N))):
-        if bank is None:
-            continue
-        if bank.dim() != 3 or bank.dtype != dtype or bank.device != x.device or not bank.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous [adapters, ...] bank of {dtype} on {x.device}, got {bank.dtype} "
+    for name, bank in (("lora_a", lora_a), ("lora_b", lora_b)):
+        if bank is not None and (bank.dim() != 3 or bank.dtype is not dtype or bank.device != device or not bank.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous [adapters, ...] bank of {dtype} on {device}, got {bank.dtype} "
                              f"{tuple(bank.shape)} on {bank.device}")
-        rank = bank.shape[1] if inner[0] == 1 else bank.shape[2]
-        other = bank.shape[2] if inner[0] == 1 else bank.shape[1]
-        if other != inner[1] or (n is not None and (bank.shape[0], rank) != (n, r)):
-            raise ValueError(f"{name} {tuple(bank.shape)} does not fit the layer [{N}, {K}] or the other factor")
-        n, r = bank.shape[0], rank
+    if lora_a is not None:
+        n, r, k = lora_a.shape
+        if k != K or (lora_b is not None and lora_b.shape != (n, N, r)):
+            raise ValueError(f"the bank {tuple(lora_a.shape)}, {None if lora_b is None else tuple(lora_b.shape)} does not fit a layer [{N}, {K}]")
+    else:
+        n, k, r = lora_b.shape
+        if k != N:
+            raise ValueError(f"lora_b {tuple(lora_b.shape)} does not fit a layer [{N}, {K}]")
     if rows.max_adapter >= n:
         raise ValueError(f"the rows name adapter {rows.max_adapter}, the bank has {n}")
     return n, r
@@ -508,32 +518,36 @@ def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lor
 
     x [M,K] bf16 or fp16, out_dtype the same type.  With `hadamard` the adapters see the rotated activations unless
     `rotated_lora_input` is false, as in the single-adapter forward."""
-    with _on(x.device):
-        x, w = _rows(x), _rows(w)
+    device = x.device
+    with _on(device):
+        x, ldx = _pitched(x)
+        w, ldw = _pitched(w)
         M, K = x.shape
         N = w.shape[0]
         if out_dtype != x.dtype:
             raise ValueError(f"out_dtype must be the activations' type {x.dtype}, which the adapters share")
         _check_weight(w, K)
         n, r = _check_requests(rows, x, lora_a, lora_b, out_dtype, K, N)
-        ws, mode = _wscale_arg(w_scale, x.device, N)
-        bias = _bias_arg(bias, x.device, N)
+        ws, mode = _wscale_arg(w_scale, device, N)
+        bias = _bias_arg(bias, device, N)
         rotated = 1 if hadamard and rotated_lora_input else 0
-        if rotated and _ld(x) != K:
-            x = x.contiguous()
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        if rotated and ldx != K:
+            x, ldx = x.contiguous(), K
+        out = x.new_empty((M, N))
         if M and N:
             lib = nat.load()
             size = (N, K, r, rotated)
             need = rows.workspace_bytes.get(size)
             if need is None:
                 need = rows.workspace_bytes[size] = lib.i8f_linear_lora_requests_workspace_bytes(rows.native_ptr, N, K, r, rotated, rotated)
-            workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
-            nat.check(lib.i8f_linear_lora_requests(x.data_ptr(), _code(x.dtype), _ld(x), 1 if hadamard else 0, rotated, w.data_ptr(),
-                                                   _ld(w), ws.data_ptr(), mode, bias.data_ptr() if bias is not None else None,
-                                                   _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(), lora_b.data_ptr(), n,
-                                                   r, rows.native_ptr, out.data_ptr(), N, M, N, K, order, workspace.data_ptr(), need,
-                                                   nat.current_stream(x.device)), "i8f_linear_lora_requests")
+            workspace = x.new_empty((need,), dtype=torch.uint8)
+            rc = lib.i8f_linear_lora_requests(x.data_ptr(), _code(x.dtype), ldx, 1 if hadamard else 0, rotated, w.data_ptr(), ldw,
+                                              ws.data_ptr(), mode, bias.data_ptr() if bias is not None else None,
+                                              _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(), lora_b.data_ptr(), n, r,
+                                              rows.native_ptr, out.data_ptr(), N, M, N, K, order, workspace.data_ptr(), need,
+                                              nat.current_stream(device))
+            if rc:
+                nat.check(rc, "i8f_linear_lora_requests")
         return out
 
 
@@ -541,27 +555,30 @@ def linear_small_batch_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor
                                      rows: RequestRows) -> Tensor:
     """M <= 16 rows (single tokens) of several requests: y = x @ (w * w_scale)^T + bias + (x @ lora_a[a]^T) @ lora_b[a]^T with
     the adapter a of each row, activations not quantised, one rounding to x's dtype (bf16 or fp16)."""
-    with _on(x.device):
-        x, w = _rows(x), _rows(w)
+    device = x.device
+    with _on(device):
+        x, ldx = _pitched(x)
+        w, ldw = _pitched(w)
         M, K = x.shape
         N = w.shape[0]
         _check_weight(w, K)
         n, r = _check_requests(rows, x, lora_a, lora_b, x.dtype, K, N)
-        ws, mode = _wscale_arg(w_scale, x.device, N)
-        bias = _bias_arg(bias, x.device, N)
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        ws, mode = _wscale_arg(w_scale, device, N)
+        bias = _bias_arg(bias, device, N)
+        out = x.new_empty((M, N))
         if M and N:
             lib = nat.load()
             need = rows.workspace_bytes.get((N, r))
             if need is None:
                 need = rows.workspace_bytes[(N, r)] = lib.i8f_linear_w8a16_small_lora_requests_workspace_bytes(rows.native_ptr, N, r)
-            workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
-            nat.check(lib.i8f_linear_w8a16_small_lora_requests(x.data_ptr(), _code(x.dtype), _ld(x), w.data_ptr(), _ld(w), ws.data_ptr(),
-                                                               mode, bias.data_ptr() if bias is not None else None,
-                                                               _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(),
-                                                               lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(), N, M, N, K,
-                                                               workspace.data_ptr(), need, nat.current_stream(x.device)),
-                      "i8f_linear_w8a16_small_lora_requests")
+            workspace = x.new_empty((need,), dtype=torch.uint8)
+            rc = lib.i8f_linear_w8a16_small_lora_requests(x.data_ptr(), _code(x.dtype), ldx, w.data_ptr(), ldw, ws.data_ptr(), mode,
+                                                          bias.data_ptr() if bias is not None else None,
+                                                          _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(),
+                                                          lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(), N, M, N, K,
+                                                          workspace.data_ptr(), need, nat.current_stream(device))
+            if rc:
+                nat.check(rc, "i8f_linear_w8a16_small_lora_requests")
         return out
 
 
@@ -579,16 +596,19 @@ def _modulation(v: Tensor | None, name: str, y: Tensor, requests: int):
     if v is None:
         return None, None, 0, False
     K = y.shape[1]
-    if v.dim() == 1:
+    shape = v.shape
+    if len(shape) == 1:
         v = v[None]
-    if v.dim() != 2 or v.shape[1] != K or v.shape[0] not in (1, requests):
-        raise ValueError(f"{name} must be [{K}] or [{requests}, {K}], got {tuple(v.shape)}")
-    if v.dtype != y.dtype or v.device != y.device:
+        shape = v.shape
+    if len(shape) != 2 or shape[1] != K or shape[0] not in (1, requests):
+        raise ValueError(f"{name} must be [{K}] or [{requests}, {K}], got {tuple(shape)}")
+    if v.dtype is not y.dtype or v.device != y.device:
         v = v.to(device=y.device, dtype=y.dtype)
-    per_request = v.shape[0] > 1
-    if (v.stride(1) != 1 and K > 1) or (per_request and v.stride(0) < K):
-        v = v.contiguous()
-    return v, v.data_ptr(), v.stride(0) if per_request else K, per_request
+    per_request = shape[0] > 1
+    pitch, inner = v.stride()
+    if (inner != 1 and K > 1) or (per_request and pitch < K):
+        v, pitch = v.contiguous(), K
+    return v, v.data_ptr(), pitch if per_request else K, per_request
 
 
 def _weight_vector(v: Tensor | None, name: str, y: Tensor):
@@ -607,45 +627,53 @@ def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm,
                          x_out, want_h, want_q):
     device = y.device
     with _on(device):
-        if x.dim() != 2 or y.dim() != 2 or x.shape != y.shape or x.device != device:
-            raise ValueError(f"x and y must be 2-D tensors of one shape on one device, got {tuple(x.shape)} and {tuple(y.shape)}")
-        if y.dtype not in (torch.bfloat16, torch.float16) or x.dtype not in (y.dtype, torch.float32):
-            raise ValueError(f"y must be bf16 or fp16 and x of the same type or fp32, got {y.dtype} and {x.dtype}")
+        shape, dtype = y.shape, y.dtype
+        if len(shape) != 2 or x.shape != shape or x.device != device:
+            raise ValueError(f"x and y must be 2-D tensors of one shape on one device, got {tuple(x.shape)} and {tuple(shape)}")
+        if (dtype is not torch.bfloat16 and dtype is not torch.float16) or (x.dtype is not dtype and x.dtype is not torch.float32):
+            raise ValueError(f"y must be bf16 or fp16 and x of the same type or fp32, got {dtype} and {x.dtype}")
         if post_norm not in nat.NORM_CODE or norm not in ("rms", "layer"):
             raise ValueError("post_norm is None, 'rms' or 'layer'; norm is 'rms' or 'layer'")
-        M, K = y.shape
+        M, K = shape
         requests = 1
         if rows is not None:
             if rows.device != device or rows.total != M:
                 raise ValueError(f"the row plan is for {rows.total} rows on {rows.device}, the call has {M} on {device}")
             requests = rows.requests
         given = x
-        x, y = _rows(x), _rows(y)
+        x, ldx = _pitched(x)
+        y, ldy = _pitched(y)
         gate, g, ldg, many_g = _modulation(gate, "gate", y, requests)
         scale, s, lds, many_s = _modulation(scale, "scale", y, requests)
         shift, t, ldt, many_t = _modulation(shift, "shift", y, requests)
         post_weight, pw = _weight_vector(post_weight, "post_weight", y)
         weight, nw = _weight_vector(weight, "weight", y)
+        ldo = K
         if x_out is None:
-            x_out = torch.empty((M, K), dtype=x.dtype, device=device)
-        elif x_out.shape != (M, K) or x_out.dtype != x.dtype or x_out.device != device or (K > 1 and x_out.stride(1) != 1) or (
-                M > 1 and x_out.stride(0) < K):
-            raise ValueError("x_out must have x's shape, type and device, rows of unit inner stride that do not overlap")
-        elif x_out is given:
-            x = x_out
-        h = torch.empty((M, K), dtype=y.dtype, device=device) if want_h else None
-        q = torch.empty((M, K), dtype=torch.int8, device=device) if want_q else None
-        q_scale = torch.empty((M, 1), dtype=torch.float32, device=device) if want_q else None
+            x_out = x.new_empty(shape)
+        else:
+            if x_out.shape != shape or x_out.dtype is not x.dtype or x_out.device != device or (K > 1 and x_out.stride(1) != 1) or (
+                    M > 1 and x_out.stride(0) < K):
+                raise ValueError("x_out must have x's shape, type and device, rows of unit inner stride that do not overlap")
+            if x_out is given:
+                x = x_out
+            ldo = _ld(x_out)
+        h = y.new_empty(shape) if want_h else None
+        q = y.new_empty(shape, dtype=torch.int8) if want_q else None
+        q_scale = y.new_empty((M, 1), dtype=torch.float32) if want_q else None
         if M and K:
-            row_request = rows.row_request_ptr if many_g or many_s or many_t else None
-            # a vector for all rows beside others per request: a pitch of 0 gives every request the same row
-            if row_request is not None:
+            row_request = None
+            if many_g or many_s or many_t:
+                # a vector for all rows beside others per request: a pitch of 0 gives every request the same row
+                row_request = rows.row_request_ptr
                 ldg, lds, ldt = ldg if many_g else 0, lds if many_s else 0, ldt if many_t else 0
-            nat.check(nat.load().i8f_gated_residual_norm(
-                x.data_ptr(), _code(x.dtype), _ld(x), y.data_ptr(), _code(y.dtype), _ld(y), M, K, row_request, g, ldg, 1 if gate_tanh else 0,
-                residual_scale, nat.NORM_CODE[post_norm], pw, nat.NORM_CODE[norm], nw, s, lds, t, ldt, eps, x_out.data_ptr(), _ld(x_out),
+            rc = nat.load().i8f_gated_residual_norm(
+                x.data_ptr(), _code(x.dtype), ldx, y.data_ptr(), _code(dtype), ldy, M, K, row_request, g, ldg, 1 if gate_tanh else 0,
+                residual_scale, nat.NORM_CODE[post_norm], pw, nat.NORM_CODE[norm], nw, s, lds, t, ldt, eps, x_out.data_ptr(), ldo,
                 h.data_ptr() if want_h else None, K, q.data_ptr() if want_q else None, K, q_scale.data_ptr() if want_q else None,
-                nat.current_stream(device)), "i8f_gated_residual_norm")
+                nat.current_stream(device))
+            if rc:
+                nat.check(rc, "i8f_gated_residual_norm")
         return x_out, h, q, q_scale
 
 
