@@ -48,10 +48,11 @@ constexpr int kStageRowBytes = 128; // one 128-byte swizzle span of K per stage
 
 enum EpiMode : int { kEpiI32 = 0, kEpiDequant = 1, kEpiCast = 2, kEpiAccum = 3 };
 // what joins the product in the epilogue (a template parameter, so that the plain kernels carry none of it)
-enum Extra : int { kExtraNone = 0, kExtraLora = 1, kExtraAddend = 2, kExtraRequests = 3, kExtraRows = 4 };
+enum Extra : int { kExtraNone = 0, kExtraLora = 1, kExtraAddend = 2, kExtraRequests = 3, kExtraRows = 4, kExtraFold = 5 };
 
 // status codes written by bounded waits
-enum : int { kStEmptyWait = 101, kStFullWait = 102, kStAccEmptyWait = 103, kStAccFullWait = 104, kStLowEmptyWait = 106, kStLowFullWait = 107 };
+enum : int { kStEmptyWait = 101, kStFullWait = 102, kStAccEmptyWait = 103, kStAccFullWait = 104, kStLowEmptyWait = 106, kStLowFullWait = 107,
+               kStScaledWait = 108, kStFoldedWait = 109 };
 
 struct GemmParams {
     int M, N;
@@ -79,7 +80,7 @@ struct GemmParams {
     int k_split;  // 1, or 2: the two CTAs of a cluster each take half of K for the same tile (single-CTA kernels)
     int* status;
     // kExtraAddend: fp32 [M, ld_addend], added before the rounding to rows whose row_adapter is not negative.
-    // kExtraRequests: each 256-row tile has either its own run of `slots` (one per adapter in the tile, with the rows that
+    // kExtraRequests, kExtraFold: each 256-row tile has either its own run of `slots` (one per adapter in the tile, with the rows that
     // use it), whose low-rank terms are accumulated in tensor memory, or a place in the addend
     const float* addend;
     long long ld_addend;
@@ -120,7 +121,7 @@ struct Cfg {
     static constexpr int kStageBytes = kABytes + kBBytes;
     // Epilogue warps: four (one per 32-lane quarter of tensor memory) or, where the epilogue cannot hide under the
     // next tile's MMAs (single accumulator buffer, below), eight: two per quarter, each taking half of the columns.
-    static constexpr int kEpiWarps = (LORA && 3 * BN > 512) ? 8 : 4;
+    static constexpr int kEpiWarps = ((LORA && 3 * BN > 512) || EXTRA == kExtraFold) ? 8 : 4;
     static constexpr int kLowWarps = EXTRA == kExtraRows ? 8 : 0;
     static constexpr int kThreads = 64 + 32 * (kEpiWarps + kLowWarps);
     static constexpr int kLowPitch = BN + 4;   // floats; rows four banks apart: the epilogue's row-per-thread reads do not collide
@@ -289,9 +290,13 @@ template <int OUT, int EXTRA>
 __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, long long row, bool row_ok, int col,
                                                const uint32_t (&v)[32], const uint32_t (&lv)[EXTRA != kExtraNone ? 32 : 1], float row_scale,
                                                float ws_scalar, const float* cs, const float* cb, const OldChunk& old,
-                                               uint32_t stage, int lane, int wide_half = -1, const uint32_t* cg = nullptr) {
+                                               uint32_t stage, int lane, int wide_half = -1, const uint32_t* cg = nullptr,
+                                               bool folded = false) {
     uint32_t yp[16];
-    if (p.epi_mode == kEpiDequant) {
+    if (EXTRA == kExtraFold && folded) {      // everything is in the accumulator already
+#pragma unroll
+        for (int i = 0; i < 16; ++i) yp[i] = pack2<OUT>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+    } else if (p.epi_mode == kEpiDequant) {
         const bool per_ch = p.w_scale_mode == I8F_WSCALE_CHANNEL;
         const bool single = p.epi_order == I8F_EPI_SINGLE;
         float y[32];
@@ -423,6 +428,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     float* epi_smem = reinterpret_cast<float*>(gen_base + kBarOff + C::kBarrierBytes);
     const uint32_t out_stage0 = smem_base + kBarOff + C::kBarrierBytes + C::kEpiBytes;  // 1024-byte aligned
     float* const low_smem = reinterpret_cast<float*>(gen_base + kBarOff + C::kBarrierBytes + C::kEpiBytes + C::kOutStageBytes);
+    const uint32_t scaled0 = tmem_slot + 8, folded0 = tmem_slot + 24;        // kExtraFold, one per accumulator buffer
     const uint32_t low_full = tmem_slot + 8, low_empty = tmem_slot + 16;      // kExtraRows: the tile's low-rank rows are there / read
 
     const int warp = threadIdx.x >> 5;
@@ -442,6 +448,12 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if constexpr (EXTRA == kExtraRows) {
             mbar_init(low_full, C::kLowWarps);
             mbar_init(low_empty, C::kEpiWarps);
+        }
+        if constexpr (EXTRA == kExtraFold) {
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(scaled0 + 8 * b, 2 * C::kEpiWarps);
+                mbar_init(folded0 + 8 * b, 1);
+            }
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -474,6 +486,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int tile_first = (PAIR || ksplit) ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
     const int kb_begin = ksplit ? static_cast<int>(krank) * (p.num_k_blocks >> 1) : 0;
     const int kb_end = (ksplit && krank == 0) ? (p.num_k_blocks >> 1) : p.num_k_blocks;
+
+    // kExtraFold: before which slab of the next tile's K loop a tile's low-rank term is added (late enough for the epilogue warps
+    // to have scaled the accumulator, early enough for them to store it before the buffer's next turn)
+    const int fold_at = min(p.num_k_blocks / 2, 12);
 
     // Programmatic dependent launch: everything above (barriers, tensor memory, descriptor prefetch) may run while the
     // kernel before this one in the stream is still finishing; nothing below may start before its results are visible.
@@ -510,12 +526,44 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
+            // the low-rank operands of one tile, for each of its adapters: t rows where A rows go, the adapter's rows of the
+            // bank where W rows go
+            auto load_low_rank = [&](int tile) -> bool {
+                int m_blk, n_blk;
+                tile_coords(tile, p.tiles_m, p.tiles_n, m_blk, n_blk);
+                const int row_a = m_blk * C::kTileM + static_cast<int>(rank) * kBM;
+                const int row_b = n_blk * BN + static_cast<int>(rank) * C::kBRows;
+                const RequestTile rt = p.req_tiles[m_blk];
+                for (int s = 0; s < rt.n_slots; ++s) {
+                    const int row_l = static_cast<int>(p.req_slots[rt.slot_begin + s].adapter * p.lora_n) + row_b;
+                    for (int lb = 0; lb < p.lora_k_blocks; ++lb) {
+                        if (!mbar_wait_bounded(empty0 + 8 * stage, phase ^ 1u, abort_flag, p.status, kStEmptyWait)) return false;
+                        const uint32_t a_dst = smem_base + stage * C::kStageBytes;
+                        const uint32_t bar = mapa_cluster(full0 + 8 * stage, 0);
+                        if (leader) mbar_arrive_expect_tx(full0 + 8 * stage, 2 * C::kStageBytes);
+                        tma_load_2d_pair(a_dst, &lora.t, bar, lb * 64, row_a);
+                        tma_load_2d_pair(a_dst + C::kABytes, &lora.b, bar, lb * 64, row_l);
+                        if (++stage == C::kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+                return true;
+            };
+            int unfolded = -1;      // kExtraFold: the tile whose low-rank operands are still to be loaded
             for (int t = tile_first; ok && t < num_tiles; t += tile_step) {
                 int m_blk, n_blk;
                 tile_coords(t, p.tiles_m, p.tiles_n, m_blk, n_blk);
                 const int row_a = m_blk * C::kTileM + static_cast<int>(rank) * kBM;
                 const int row_b = n_blk * BN + static_cast<int>(rank) * C::kBRows;
                 for (int kb = kb_begin; kb < kb_end; ++kb) {
+                    if constexpr (EXTRA == kExtraFold) {
+                        if (kb == fold_at && unfolded >= 0 && !load_low_rank(unfolded)) {
+                            ok = false;
+                            break;
+                        }
+                    }
                     if (!mbar_wait_bounded(empty0 + 8 * stage, phase ^ 1u, abort_flag, p.status, kStEmptyWait)) {
                         ok = false;
                         break;
@@ -541,27 +589,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         phase ^= 1u;
                     }
                 }
-                if constexpr (EXTRA == kExtraRequests) {
-                    // the same for each adapter of the tile: t again, and the adapter's slice of the bank
-                    const RequestTile rt = p.req_tiles[m_blk];
-                    for (int s = 0; ok && s < rt.n_slots; ++s) {
-                        const int row_l = static_cast<int>(p.req_slots[rt.slot_begin + s].adapter * p.lora_n) + row_b;
-                        for (int lb = 0; lb < p.lora_k_blocks; ++lb) {
-                            if (!mbar_wait_bounded(empty0 + 8 * stage, phase ^ 1u, abort_flag, p.status, kStEmptyWait)) {
-                                ok = false;
-                                break;
-                            }
-                            const uint32_t a_dst = smem_base + stage * C::kStageBytes;
-                            const uint32_t bar = mapa_cluster(full0 + 8 * stage, 0);
-                            if (leader) mbar_arrive_expect_tx(full0 + 8 * stage, 2 * C::kStageBytes);
-                            tma_load_2d_pair(a_dst, &lora.t, bar, lb * 64, row_a);
-                            tma_load_2d_pair(a_dst + C::kABytes, &lora.b, bar, lb * 64, row_l);
-                            if (++stage == C::kStages) {
-                                stage = 0;
-                                phase ^= 1u;
-                            }
-                        }
-                    }
+                if constexpr (EXTRA == kExtraFold) {
+                    unfolded = t;
+                } else if constexpr (EXTRA == kExtraRequests) {
+                    if (ok) ok = load_low_rank(t);
                 } else if constexpr (LORA) {
                     // the low-rank operands ride the same ring: t rows where A rows go, lora_b rows where W rows go
                     for (int lb = 0; ok && lb < p.lora_k_blocks; ++lb) {
@@ -581,6 +612,9 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     }
                 }
             }
+            if constexpr (EXTRA == kExtraFold) {
+                if (ok && unfolded >= 0) load_low_rank(unfolded);
+            }
         }
         if (ksplit) {   // every thread of both CTAs takes part in the two barriers of the hand-over (see the epilogue)
             cluster_arrive();
@@ -599,11 +633,53 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             // asks for the NEXT slab's barrier before it issues its own MMAs, so the round trip of that query passes
             // under the MMA issue instead of in front of it (the issue loop, not the tensor core, bounds narrow tiles).
             bool ready = false;
+            // kExtraFold: the MMAs of a tile's adapters on top of its scaled accumulator, each under its row mask
+            uint32_t scaled_phase = 0;      // bit b: buffer b
+            int unfolded = -1;
+            auto fold = [&](int tile, int b) -> bool {
+                const RequestTile rt = p.req_tiles[tile_m(tile, p.tiles_m, p.tiles_n)];
+                if (rt.n_slots == 0) return true;
+                const uint32_t idesc = p.lora_bf16 ? make_idesc(kDFmtF32, kFmtBF16, C::kTileM, BN) : make_idesc(kDFmtF32, kFmtF16, C::kTileM, BN);
+                if (!mbar_wait_bounded(scaled0 + 8 * b, (scaled_phase >> b) & 1u, abort_flag, p.status, kStScaledWait)) return false;
+                scaled_phase ^= 1u << b;
+                tc_fence_after_sync();
+                for (int s = 0; s < rt.n_slots; ++s) {
+                    const RequestSlot* slot = p.req_slots + rt.slot_begin + s;
+                    uint32_t off[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) off[i] = ~slot->rows[i];
+                    for (int lb = 0; lb < p.lora_k_blocks; ++lb) {
+                        if (!ready && !mbar_wait_bounded(full0 + 8 * stage, phase, abort_flag, p.status, kStFullWait)) return false;
+                        ready = false;
+                        tc_fence_after_sync();
+                        const uint32_t a_src = smem_base + stage * C::kStageBytes;
+                        const uint64_t adesc = make_smem_desc_sw128(a_src);
+                        const uint64_t bdesc = make_smem_desc_sw128(a_src + C::kABytes);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (lb * 4 + k < p.lora_k16)
+                                mma_f16_pair_masked(tmem_base + static_cast<uint32_t>(b * BN), adesc + 2 * k, bdesc + 2 * k, idesc, 1u, off);
+                        mma_commit_pair(empty0 + 8 * stage);
+                        if (++stage == C::kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+                mma_commit_pair(folded0 + 8 * b);
+                return true;
+            };
             for (int t = tile_first; ok && t < num_tiles; t += tile_step) {
                 if (!mbar_wait_bounded(accempty0 + 8 * buf, acc_phase ^ 1u, abort_flag, p.status, kStAccEmptyWait)) break;
                 tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * BN);
                 for (int kb = 0; kb < kb_end - kb_begin; ++kb) {
+                    if constexpr (EXTRA == kExtraFold) {
+                        if (kb == fold_at && unfolded >= 0 && !fold(unfolded, buf ^ 1)) {
+                            ok = false;
+                            break;
+                        }
+                    }
                     if (!ready && !mbar_wait_bounded(full0 + 8 * stage, phase, abort_flag, p.status, kStFullWait)) {
                         ok = false;
                         break;
@@ -686,10 +762,14 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     }
                     if (!ok) break;
                 }
+                if constexpr (EXTRA == kExtraFold) unfolded = t;
                 if constexpr (PAIR) mma_commit_pair(accfull0 + 8 * buf);  // accumulator complete
                 else mma_commit(accfull0 + 8 * buf);
                 if constexpr (C::kAccBufs == 2) buf ^= 1;
                 if (buf == 0) acc_phase ^= 1u;
+            }
+            if constexpr (EXTRA == kExtraFold) {
+                if (ok && unfolded >= 0) fold(unfolded, buf ^ 1);
             }
         }
         if (ksplit) {
@@ -754,7 +834,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         float* col_bias = col_scale + BN;
         int buf = 0;
         uint32_t acc_phase = 0;
-        uint32_t low_phase = 0;
+        uint32_t low_phase = 0, folded_phase = 0;
         const bool dequant = p.epi_mode == kEpiDequant;
         const bool per_ch = dequant && p.w_scale_mode == I8F_WSCALE_CHANNEL;
         const bool has_bias = dequant && p.bias != nullptr;
@@ -817,6 +897,13 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 has_addend = row_ok && __ldg(p.row_adapter + row) >= 0;
                 addend_row = low_smem + (quarter * 32 + lane) * C::kLowPitch;
             }
+            bool folded = false;
+            if constexpr (EXTRA == kExtraFold) {
+                const int addend_row0 = p.req_tiles[m_blk].addend_row;
+                folded = p.req_tiles[m_blk].n_slots > 0;
+                has_addend = addend_row0 >= 0 && row_ok && __ldg(p.row_adapter + row) >= 0;
+                addend_row = p.addend + (addend_row0 + (row - static_cast<long long>(m_blk) * C::kTileM)) * p.ld_addend;
+            }
             if constexpr (EXTRA == kExtraRequests) {
                 const bool with_adapter = row_ok && __ldg(p.row_adapter + row) >= 0;
                 const int addend_row0 = p.req_tiles[m_blk].addend_row;
@@ -866,6 +953,34 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             if constexpr (EXTRA == kExtraRows) {
                 if (!mbar_wait_bounded(low_full, low_phase, abort_flag, p.status, kStLowFullWait)) break;
                 low_phase ^= 1u;
+            }
+            if constexpr (EXTRA == kExtraFold) {
+                if (folded) {
+                    // scale in place: int32 sums -> fp32 values (and the bias), on which the low-rank MMAs accumulate.  The next
+                    // tile's MMAs run meanwhile
+                    const float total = __fmul_rn(ws_scalar, row_scale);
+#pragma unroll 1
+                    for (int c = c_first; c < c_end; ++c) {
+                        uint32_t v[32];
+                        tmem_ld_32x32(t_addr + c * 32, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            float y = __int2float_rn(static_cast<int>(v[j]));
+                            y = __fmul_rn(y, per_ch ? __fmul_rn(row_scale, col_scale[c * 32 + j]) : total);
+                            if (has_bias) y = __fadd_rn(y, col_bias[c * 32 + j]);
+                            v[j] = __float_as_uint(y);
+                        }
+                        tmem_st_32x32(t_addr + c * 32, v);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(mapa_cluster(scaled0 + 8 * buf, 0));
+                    if (!mbar_wait_bounded(folded0 + 8 * buf, (folded_phase >> buf) & 1u, abort_flag, p.status, kStFoldedWait)) break;
+                    folded_phase ^= 1u << buf;
+                    tc_fence_after_sync();
+                }
             }
             const uint32_t t_lora = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(C::kLoraCol);
             bool released = false;
@@ -917,6 +1032,16 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     __syncwarp();
                 }
                 tmem_ld_wait();
+                if constexpr (EXTRA == kExtraFold) {
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        const uint4 o = has_addend ? __ldg(reinterpret_cast<const uint4*>(addend_row + col) + g) : make_uint4(0u, 0u, 0u, 0u);
+                        lv[4 * g] = o.x;
+                        lv[4 * g + 1] = o.y;
+                        lv[4 * g + 2] = o.z;
+                        lv[4 * g + 3] = o.w;
+                    }
+                }
                 if constexpr (EXTRA == kExtraRequests) {   // rows without an adapter: whatever an earlier tile left there is dropped
                     if (has_addend) {
                         const uint4* src = reinterpret_cast<const uint4*>(addend_row + col);
@@ -962,11 +1087,11 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 } else if (p.out_dtype == I8F_BF16) {
                     epilogue_chunk<I8F_BF16, EXTRA>(p, row, row_ok, col, v, lv, row_scale, ws_scalar, col_scale + c * 32,
                                                    col_bias + c * bias_step, old_cur, stage, lane, wide_half,
-                                                   has_gate ? reinterpret_cast<const uint32_t*>(col_bias) + BN / 2 + c * 16 : nullptr);
+                                                   has_gate ? reinterpret_cast<const uint32_t*>(col_bias) + BN / 2 + c * 16 : nullptr, folded);
                 } else {
                     epilogue_chunk<I8F_F16, EXTRA>(p, row, row_ok, col, v, lv, row_scale, ws_scalar, col_scale + c * 32,
                                                   col_bias + c * bias_step, old_cur, stage, lane, wide_half,
-                                                  has_gate ? reinterpret_cast<const uint32_t*>(col_bias) + BN / 2 + c * 16 : nullptr);
+                                                  has_gate ? reinterpret_cast<const uint32_t*>(col_bias) + BN / 2 + c * 16 : nullptr, folded);
                 }
                 if (wide_out) {
                     if (wide_half == 1) {
@@ -1186,7 +1311,7 @@ int launch_gemm(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t 
     using C = Cfg<BN, PAIR, EXTRA>;
     CUtensorMap tmA, tmB;
     LoraMaps lmaps{};
-    if (C::LORA) {
+    if (C::LORA || EXTRA == kExtraFold) {
         int rc_l = make_operand_map(&lmaps.t, lo->kind, lo->t, M, lo->r, lo->ldt, kBM);
         if (rc_l != I8F_OK) return rc_l;
         rc_l = make_operand_map(&lmaps.b, lo->kind, lo->b, N * lo->adapters, lo->r, lo->ldb, C::kBRows);
@@ -1527,6 +1652,10 @@ static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, 
         p.req_tiles = term->tiles;
         p.req_slots = term->slots;
         const LoraOperands lo{term->t, term->ldt, term->b, term->r, term->r, out_dtype == I8F_BF16 ? kKindBF16 : kKindF16, term->adapters};
+        // one rounding: the low-rank term is accumulated onto the scaled product, both accumulator buffers stay free for the
+        // next tile (18432 x 4096 -> 12288, rank 32: FOLD_US us, with an accumulator of its own for the term 749).  The reference's
+        // roundings need the two apart
+        if (epilogue_order == I8F_EPI_SINGLE) return launch_gemm<kKindI8, 256, true, kExtraFold>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
         return launch_gemm<kKindI8, 256, true, kExtraRequests>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
     }
     return launch_gemm_auto<kKindI8>(a, lda, w, ldw, M, N, K, p, st, scatter);

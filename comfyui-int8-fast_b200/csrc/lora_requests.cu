@@ -326,9 +326,13 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     const int row_in_block = quarter * 32 + lane;
     const int64_t row = static_cast<int64_t>(block) * kDownRows + row_in_block;
     const int cols = min(p.bn, p.r - n0);
-    auto store_row = [&](int64_t m, int c, float v) {
-        if (p.bf16) store_dt<I8F_BF16>(p.t, m * p.ldt + n0 + c, v);
-        else store_dt<I8F_F16>(p.t, m * p.ldt + n0 + c, v);
+    auto pack = [&](float lo, float hi) -> uint32_t {
+        if (p.bf16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+            return *reinterpret_cast<const uint32_t*>(&h);
+        }
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
     };
     if (warp >= 2) {
         if (any) mbar_wait_bounded(done, 0, abort_flag, p.status, kStDownDone);
@@ -336,35 +340,38 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     }
     if (p.split > 1) {
         // every CTA's MMAs are done: the rings are free, and each CTA sends every other its rows of the partial sums,
-        // [source][row][column]
+        // [source][column][row]: the lanes of a remote store are neighbours
         cluster_arrive();
         cluster_wait();
         const int share = kDownRows / p.split;
         if (warp >= 2 && any) {
             const uint32_t dst = mapa_cluster(smem_base, static_cast<uint32_t>(row_in_block / share)) +
-                                 static_cast<uint32_t>((rank * share + row_in_block % share) * p.bn * 4);
+                                 static_cast<uint32_t>((rank * p.bn * share + row_in_block % share) * 4);
             for (int c = 0; c < p.bn; c += 16) {
                 uint32_t v[16];
                 tmem_ld_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, v);
                 tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; j += 4)
-                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c + j) * 4), "r"(v[j]), "r"(v[j + 1]),
-                                 "r"(v[j + 2]), "r"(v[j + 3])
-                                 : "memory");
+                for (int j = 0; j < 16; ++j)
+                    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(dst + static_cast<uint32_t>((c + j) * share * 4)), "r"(v[j]) : "memory");
             }
         }
         cluster_arrive();
         cluster_wait();
         const float* part = reinterpret_cast<const float*>(gen_base);
-        for (int i = threadIdx.x; i < share * cols; i += kDownThreads) {
-            const int rl = i / cols, c = i - rl * cols;
+        for (int i = threadIdx.x; i < share * (cols / 8); i += kDownThreads) {      // eight columns of one row; cols is a multiple of 8
+            const int rl = i & (share - 1), c = i / share * 8;
             const int64_t m = static_cast<int64_t>(block) * kDownRows + rank * share + rl;
-            if (m >= p.M) break;
-            float v = 0.f;
-            if (p.row_adapter[m] >= 0)
-                for (int src = 0; src < p.split; ++src) v += part[(src * share + rl) * p.bn + c];
-            store_row(m, c, v);
+            if (m >= p.M) continue;
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (p.row_adapter[m] >= 0) {
+                for (int src = 0; src < p.split; ++src) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += part[(src * p.bn + c + j) * share + rl];
+                }
+            }
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.t) + m * p.ldt + n0 + c) =
+                make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
         }
     } else if (warp >= 2) {
         const bool use = row < p.M && p.row_adapter[row] >= 0;
@@ -375,14 +382,7 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
             uint32_t o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float lo = use ? __uint_as_float(v[2 * j]) : 0.f, hi = use ? __uint_as_float(v[2 * j + 1]) : 0.f;
-                if (p.bf16) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-                    o[j] = *reinterpret_cast<const uint32_t*>(&h);
-                } else {
-                    const __half2 h = __floats2half2_rn(lo, hi);
-                    o[j] = *reinterpret_cast<const uint32_t*>(&h);
-                }
+                o[j] = pack(use ? __uint_as_float(v[2 * j]) : 0.f, use ? __uint_as_float(v[2 * j + 1]) : 0.f);
             }
             if (row < p.M) {      // cols is a multiple of 8
                 uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.t) + row * p.ldt + n0 + c);
