@@ -787,33 +787,41 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 if (!mbar_wait_bounded(low_empty, low_phase ^ 1u, abort_flag, p.status, kStLowEmptyWait)) break;
                 low_phase ^= 1u;
                 const int cols = min(BN, p.N - n_blk * BN);
-                // four rows at a time, with their adapters' rows of lora_b: read once where the four share an adapter
+                // eight rows of one adapter share a pass over its rows of lora_b, else four do, else they are taken four at a time
+                // with an adapter each
                 const int first = warp - 2 - C::kEpiWarps;
-                constexpr int kQuads = kBM / 4 / C::kLowWarps;      // of this warp
+                constexpr int kOctets = kBM / 8 / C::kLowWarps;      // of this warp
                 int ids = -1;
                 {
-                    const int m = m_blk * kBM + (first + (lane >> 2) * C::kLowWarps) * 4 + (lane & 3);
-                    if (lane < 4 * kQuads && m < p.M) ids = __ldg(p.row_adapter + m);
+                    const int m = m_blk * kBM + (first + (lane >> 3) * C::kLowWarps) * 8 + (lane & 7);
+                    if (lane < 8 * kOctets && m < p.M) ids = __ldg(p.row_adapter + m);
                 }
+                auto rows_of = [&](int a) { return a >= 0 ? p.row_b + (a * p.lora_n + n_blk * BN) * p.row_r : nullptr; };
 #pragma unroll 1
-                for (int i = 0; i < kQuads; ++i) {
-                    const int quad = first + i * C::kLowWarps;
-                    const int m0 = m_blk * kBM + quad * 4;
+                for (int i = 0; i < 2 * kOctets; ++i) {      // halves of octets
+                    const int octet = first + (i >> 1) * C::kLowWarps, at = 8 * (i >> 1) + 4 * (i & 1);
+                    const int row = octet * 8 + 4 * (i & 1);
+                    const int m0 = m_blk * kBM + row;
                     if (m0 >= p.M) break;
-                    const uint16_t* b[4];      // by row
                     int a[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        a[j] = __shfl_sync(0xFFFFFFFFu, ids, 4 * i + j);
-                        b[j] = a[j] >= 0 ? p.row_b + (a[j] * p.lora_n + n_blk * BN) * p.row_r : nullptr;
-                    }
+                    for (int j = 0; j < 4; ++j) a[j] = __shfl_sync(0xFFFFFFFFu, ids, at + j);
                     const uint16_t* rows_t = p.row_t + m0 * p.ld_row_t;
-                    float* dst = low_smem + quad * 4 * C::kLowPitch;
+                    float* dst = low_smem + row * C::kLowPitch;
                     if (a[0] >= 0 && a[0] == a[1] && a[0] == a[2] && a[0] == a[3]) {      // rows past the end have no adapter
-                        const uint16_t* const one[1] = {b[0]};
-                        if (p.lora_bf16) low_rank_rows<true, 1, 4>(rows_t, p.ld_row_t, {0}, {4}, one, cols, p.row_r, dst, C::kLowPitch, lane);
-                        else low_rank_rows<false, 1, 4>(rows_t, p.ld_row_t, {0}, {4}, one, cols, p.row_r, dst, C::kLowPitch, lane);
+                        int rows = 4;
+                        if ((i & 1) == 0) {
+                            const uint32_t same = __ballot_sync(0xFFFFFFFFu, ids == a[0]) >> at;
+                            if ((same & 0xFFu) == 0xFFu) {
+                                rows = 8;
+                                ++i;
+                            }
+                        }
+                        const uint16_t* const one[1] = {rows_of(a[0])};
+                        if (p.lora_bf16) low_rank_rows<true, 1, 4>(rows_t, p.ld_row_t, {0}, {rows}, one, cols, p.row_r, dst, C::kLowPitch, lane);
+                        else low_rank_rows<false, 1, 4>(rows_t, p.ld_row_t, {0}, {rows}, one, cols, p.row_r, dst, C::kLowPitch, lane);
                     } else {
+                        const uint16_t* const b[4] = {rows_of(a[0]), rows_of(a[1]), rows_of(a[2]), rows_of(a[3])};
                         if (p.lora_bf16) low_rank_rows<true, 4, 2>(rows_t, p.ld_row_t, {0, 1, 2, 3}, {1, 1, 1, 1}, b, cols, p.row_r, dst, C::kLowPitch, lane);
                         else low_rank_rows<false, 4, 2>(rows_t, p.ld_row_t, {0, 1, 2, 3}, {1, 1, 1, 1}, b, cols, p.row_r, dst, C::kLowPitch, lane);
                     }
@@ -1635,20 +1643,22 @@ static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, 
         p.addend = term->addend;
         p.ld_addend = term->ld_addend;
         p.row_adapter = term->row_adapter;
-        if (term->tiles == nullptr) {
-            const GemmPlan plan = plan_gemm(M, N, K, 1, sm_count(), false, forced_tile(), ksplit_enabled());
-            if (plan.choice < 3) return launch_gemm_auto<kKindI8, kExtraAddend>(a, lda, w, ldw, M, N, K, p, st);
+        const GemmPlan plan = plan_gemm(M, N, K, 1, sm_count(), false, forced_tile(), ksplit_enabled());
+        if (plan.choice >= 3) {
+            // narrow tiles, which plan_gemm takes for problems below a wave: the tile's rows are worked out by warps beside the MMAs,
+            // whatever the batch looks like (696 rows of 26 requests, K 1008, N 1010: 33 us per call, on 256 x 256 tiles 55)
             p.row_t = static_cast<const uint16_t*>(term->t);
             p.ld_row_t = term->ldt;
             p.row_b = static_cast<const uint16_t*>(term->b);
             p.row_r = static_cast<int>(term->r);
-            p.early_b = term->after_own ? 1 : 0;
             p.lora_n = N;
             p.lora_bf16 = out_dtype == I8F_BF16 ? 1 : 0;
+            p.early_b = term->after_own ? 1 : 0;
             if (plan.choice == 3) return launch_gemm<kKindI8, 128, false, kExtraRows>(a, lda, w, ldw, M, N, K, p, st, nullptr, nullptr, plan.k_split);
             if (plan.choice == 5) return launch_gemm<kKindI8, 32, false, kExtraRows>(a, lda, w, ldw, M, N, K, p, st, nullptr, nullptr, plan.k_split);
             return launch_gemm<kKindI8, 64, false, kExtraRows>(a, lda, w, ldw, M, N, K, p, st, nullptr, nullptr, plan.k_split);
         }
+        if (term->tiles == nullptr) return launch_gemm_auto<kKindI8, kExtraAddend>(a, lda, w, ldw, M, N, K, p, st);
         p.req_tiles = term->tiles;
         p.req_slots = term->slots;
         const LoraOperands lo{term->t, term->ldt, term->b, term->r, term->r, out_dtype == I8F_BF16 ? kKindBF16 : kKindF16, term->adapters};

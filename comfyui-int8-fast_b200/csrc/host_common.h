@@ -53,9 +53,9 @@ struct RequestSlot {
     uint32_t rows[8];
 };
 
-// The low-rank term of a batch of requests beside the int8 product.  `tiles` NULL: a small batch, whose rows' terms the kernel
-// works out itself beside the MMAs, or, where requests_need_addend() says so, finds in `addend` [M, ld_addend]; else the
-// tiles say where theirs comes from.  ld_addend is a multiple of 32, the addend 16-byte aligned.
+// The low-rank term of a batch of requests beside the int8 product.  Where requests_need_addend() says no, the kernel works
+// the rows' terms out itself beside the MMAs.  Else `tiles` say where theirs comes from (NULL: all of it is in `addend`
+// [M, ld_addend]).  ld_addend is a multiple of 32, the addend 16-byte aligned.
 struct RequestTerm {
     const int* row_adapter;
     const float* addend;
@@ -71,7 +71,8 @@ struct RequestTerm {
     bool after_own;
 };
 
-// Whether the product of these sizes runs on 256-wide tiles, whose epilogue has no room for rows worked out beside it.
+// Whether the product of these sizes runs on 256-wide tiles, which have no room for rows worked out beside it: the terms of
+// chunked rows have to be in the addend then.
 bool requests_need_addend(int64_t M, int64_t N, int64_t K);
 
 // i8f_linear_w8a8 with such a term; in gemm_tcgen05.cu.  With `check_only` the arguments are checked and nothing is

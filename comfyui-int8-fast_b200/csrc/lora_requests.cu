@@ -51,11 +51,12 @@ struct QuantOut {
 template <int DT, int RB, bool QUANT>
 __global__ void __launch_bounds__(kChunkThreads)
 down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ bank_a, int K, int r,
-                   const int4* __restrict__ chunks, void* __restrict__ t, int64_t ldt, const QuantOut out) {
+                   const int4* __restrict__ chunks, void* __restrict__ t, int64_t ldt, const QuantOut out, int wait_first) {
     constexpr int kValues = RB * kChunkRows;
     __shared__ float s_part[kChunkWarps][kValues];
     __shared__ uint32_t s_max[kChunkWarps][kChunkRows];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 c = chunks[blockIdx.x];      // first row, rows, adapter
     const int j0 = blockIdx.y * RB;
@@ -148,6 +149,8 @@ down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restri
             }
         }
     }
+    // this kernel's completion implies that of the one it may have run beside
+    if (!wait_first && threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // The up projection of the chunks into the fp32 addend of the int8 product's epilogue: one warp per (chunk, 64 columns).
@@ -175,13 +178,20 @@ up_chunks_kernel(const void* __restrict__ t, int64_t ldt, const void* __restrict
 // Two rings: x slabs (one per K step) and adapter slabs (one per K step and adapter).
 constexpr int kDownRows = 128;
 constexpr int kDownThreads = 192;
-constexpr int kAStages = 6;
+// Up to rank 128 the rings take 96 KB, so that two CTAs share an SM: clusters of four or eight whole SMs do not fill the GPU's
+// groups of SMs (4608 rows, K 4096, rank 64, clusters of four with one CTA per SM: 26.1 us in two waves).
+constexpr int kAStages = 4;
 constexpr int kASlab = kDownRows * 128;
-constexpr int kBRingBytes = 96 * 1024;
-constexpr int kMaxBStages = 12;
-constexpr int kDownSmem = kAStages * kASlab + kBRingBytes + 1024 /* barriers */ + 1024 /* alignment */;
+constexpr int kMaxBStages = 8;
 constexpr int kMaxBN = 256;
-static_assert(kDownRows * kMaxBN * 4 <= kAStages * kASlab + kBRingBytes, "the partial sums land where the rings were");
+__host__ __device__ constexpr int b_ring_bytes(int bn) { return bn <= 128 ? 32 * 1024 : 64 * 1024; }
+__host__ __device__ constexpr int b_ring_stages(int bn) {
+    return b_ring_bytes(bn) / (bn * 128) < kMaxBStages ? b_ring_bytes(bn) / (bn * 128) : kMaxBStages;
+}
+constexpr int down_smem(int bn) { return kAStages * kASlab + b_ring_bytes(bn) + 1024 /* barriers */ + 1024 /* alignment */; }
+static_assert(b_ring_stages(kMaxBN) >= 2 && b_ring_stages(128) >= 2, "a slab in use and one on its way");
+static_assert(kDownRows * kMaxBN * 4 <= kAStages * kASlab + b_ring_bytes(kMaxBN) && kDownRows * 128 * 4 <= kAStages * kASlab + b_ring_bytes(128),
+              "the partial sums land where the rings were");
 
 enum : int { kStDownEmptyA = 121, kStDownEmptyB = 122, kStDownFullA = 123, kStDownFullB = 124, kStDownDone = 125 };
 
@@ -195,7 +205,7 @@ struct DownParams {
     int* status;
 };
 
-__global__ void __launch_bounds__(kDownThreads, 1)
+__global__ void __launch_bounds__(kDownThreads, 2)
 down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a, const DownParams p) {
     const int block = blockIdx.y;
     const int half = block & 1;
@@ -207,8 +217,7 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     uint8_t* gen_base = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t a_ring = smem_base, b_ring = smem_base + kAStages * kASlab;
     const uint32_t b_slab = static_cast<uint32_t>(p.bn) * 128u;
-    constexpr int kBarOff = kAStages * kASlab + kBRingBytes;
-    const uint32_t full_a = smem_base + kBarOff, empty_a = full_a + 8 * kAStages, full_b = empty_a + 8 * kAStages,
+    const uint32_t full_a = smem_base + kAStages * kASlab + b_ring_bytes(p.bn), empty_a = full_a + 8 * kAStages, full_b = empty_a + 8 * kAStages,
                    empty_b = full_b + 8 * kMaxBStages, done = empty_b + 8 * kMaxBStages, tmem_slot = done + 8;
     volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - smem_base));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (tmem_slot - smem_base) + 4);
@@ -462,8 +471,7 @@ int launch_down_tiles(const void* x, int64_t ldx, const void* bank_a, int64_t ad
     p.M = static_cast<int>(M);
     p.r = static_cast<int>(r);
     p.bn = r >= kMaxBN ? kMaxBN : static_cast<int>((r + 15) / 16 * 16);
-    const int fit = kBRingBytes / (p.bn * 128);
-    p.b_stages = fit < kMaxBStages ? fit : kMaxBStages;
+    p.b_stages = b_ring_stages(p.bn);
     p.num_kb = static_cast<int>((K + 63) / 64);
     p.bf16 = dtype == I8F_BF16;
     p.wait_first = after_reader ? 0 : 1;
@@ -484,19 +492,23 @@ int launch_down_tiles(const void* x, int64_t ldx, const void* bank_a, int64_t ad
     I8F_REQUIRE(blocks <= 65535, I8F_ERR_UNSUPPORTED, "M=%lld is too large", (long long)M);
     const int64_t dense = rows->n_dense * 2 < blocks ? rows->n_dense * 2 : blocks;
     p.split = 1;
-    // CTAs that share a block's K range: as many as still run at once, with at least four slabs each
+    // CTAs that share a block's K range, with at least four slabs each.  A 128-row MMA takes 128 cycles however few columns it
+    // has, so a block's K loop is bound by the tensor core of its SM (0.43 us per slab) and is spread over as many SMs as there
+    // are (us at K 4096, split 1 / 2 / 4 / 8: 9216 rows 32.8 / 21.9 / 28.2 / 28.4, 4608 rows 32.2 / 21.0 / 15.1 / 21.1,
+    // 1536 rows 31.4 / 19.9 / 12.7 / 10.2); two CTAs on every SM still gain a little (18432 rows: 34.3 / 30.3).
     while (p.split < 8 && dense * rank_tiles * p.split * 2 <= sm_count() && p.num_kb >= 8 * p.split) p.split *= 2;
+    if (p.split == 1 && p.bn <= 128 && dense * rank_tiles <= sm_count() && p.num_kb >= 8) p.split = 2;
     static bool attr_done[64] = {false};
     const int dev = current_device();
     if (!attr_done[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(down_tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDownSmem);
-        if (e != cudaSuccess) return fail(I8F_ERR_CUDA, "cudaFuncSetAttribute(smem=%d): %s", kDownSmem, cudaGetErrorString(e));
+        const cudaError_t e = cudaFuncSetAttribute(down_tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, down_smem(kMaxBN));
+        if (e != cudaSuccess) return fail(I8F_ERR_CUDA, "cudaFuncSetAttribute(smem=%d): %s", down_smem(kMaxBN), cudaGetErrorString(e));
         attr_done[dev] = true;
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.split), static_cast<unsigned>(blocks), static_cast<unsigned>(rank_tiles));
     cfg.blockDim = dim3(kDownThreads, 1, 1);
-    cfg.dynamicSmemBytes = kDownSmem;
+    cfg.dynamicSmemBytes = down_smem(p.bn);
     cfg.stream = st;
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -512,16 +524,27 @@ int launch_down_tiles(const void* x, int64_t ldx, const void* bank_a, int64_t ad
     return check_launch("down_tiles_kernel");
 }
 
-// `out`: also quantise the rows (only where the chunks cover the whole batch).
+// `out`: also quantise the rows (only where the chunks cover the whole batch).  `after_reader` as in launch_down_tiles, the kernels
+// before it being the library's own.
 int launch_down_chunks(const void* x, int64_t ldx, const void* bank_a, int64_t r, const i8f_request_rows* rows, void* t, int64_t ldt,
-                       int dtype, int64_t K, const QuantOut* out, cudaStream_t st) {
+                       int dtype, int64_t K, const QuantOut* out, bool after_reader, cudaStream_t st) {
     const int4* chunks = reinterpret_cast<const int4*>(rows->chunks);
     // two rank rows per CTA where the chunks alone would leave SMs idle, else eight (x is then read a quarter as often)
     const bool few = rows->n_chunks * (r / 8) < 2 * sm_count();
     const dim3 grid(static_cast<unsigned>(rows->n_chunks), static_cast<unsigned>(r / (few ? 2 : 8)));
     const QuantOut q = out != nullptr ? *out : QuantOut{};
     const int k = static_cast<int>(K), rank = static_cast<int>(r);
-#define I8F_DOWN(DT, RB, Q) down_chunks_kernel<DT, RB, Q><<<grid, kChunkThreads, 0, st>>>(x, ldx, bank_a, k, rank, chunks, t, ldt, q)
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kChunkThreads, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = after_reader ? 1 : 0;
+    cudaError_t e = cudaSuccess;
+#define I8F_DOWN(DT, RB, Q) e = cudaLaunchKernelEx(&cfg, down_chunks_kernel<DT, RB, Q>, x, ldx, bank_a, k, rank, chunks, t, ldt, q, after_reader ? 0 : 1)
 #define I8F_DOWN_RB(DT)                                     \
     do {                                                    \
         if (few && out != nullptr) I8F_DOWN(DT, 2, true);   \
@@ -533,6 +556,7 @@ int launch_down_chunks(const void* x, int64_t ldx, const void* bank_a, int64_t r
     else I8F_DOWN_RB(I8F_F16);
 #undef I8F_DOWN_RB
 #undef I8F_DOWN
+    if (e != cudaSuccess) return fail(I8F_ERR_CUDA, "down_chunks_kernel launch: %s", cudaGetErrorString(e));
     return check_launch("down_chunks_kernel");
 }
 
@@ -560,7 +584,7 @@ int launch_down(const void* x, int64_t ldx, const void* bank_a, int64_t adapters
         const int rc = launch_down_tiles(x, ldx, bank_a, adapters, r, rows, t, ldt, dtype, M, K, after_reader, st);
         if (rc != I8F_OK) return rc;
     }
-    return has_chunks(rows) ? launch_down_chunks(x, ldx, bank_a, r, rows, t, ldt, dtype, K, nullptr, st) : I8F_OK;
+    return has_chunks(rows) ? launch_down_chunks(x, ldx, bank_a, r, rows, t, ldt, dtype, K, nullptr, after_reader, st) : I8F_OK;
 }
 
 RequestTerm request_term(const void* t, int64_t ldt, const void* bank_b, int64_t adapters, int64_t r, const i8f_request_rows* rows,
@@ -619,7 +643,7 @@ int i8f_linear_w8a8_lora_requests(const int8_t* a, int64_t lda, const float* a_s
     float* addend = static_cast<float*>(workspace);
     const RequestTerm term = request_term(t, ldt, bank_b, adapters, r, rows, N, addend);
     for (const bool check_only : {true, false}) {     // everything is checked before anything is launched
-        if (!check_only && has_chunks(rows) && (has_dense(rows) || requests_need_addend(M, N, K))) {
+        if (!check_only && has_chunks(rows) && requests_need_addend(M, N, K)) {
             rc = launch_up_chunks(t, ldt, bank_b, r, rows, out_dtype, N, addend, st);
             if (rc != I8F_OK) return rc;
         }
@@ -683,14 +707,14 @@ int i8f_linear_lora_requests(const void* x, int x_dtype, int64_t ldx, int hadama
     if (rc != I8F_OK) return rc;
     if (!has_dense(rows) && !hadamard128) {
         const QuantOut out_q{q, K, q_scale};
-        rc = launch_down_chunks(x, ldx, bank_a, r, rows, t, r, x_dtype, K, &out_q, st);
+        rc = launch_down_chunks(x, ldx, bank_a, r, rows, t, r, x_dtype, K, &out_q, false, st);
     } else {
         rc = i8f_quant_rowwise(x, x_dtype, M, K, ldx, q, K, q_scale, hadamard128, rotated, stream);
         if (rc != I8F_OK) return rc;
         rc = launch_down(lora_in, ldx, bank_a, adapters, r, rows, t, r, x_dtype, M, K, !keep_rotated, st);
     }
     if (rc != I8F_OK) return rc;
-    if (has_chunks(rows) && (has_dense(rows) || requests_need_addend(M, N, K))) {
+    if (has_chunks(rows) && requests_need_addend(M, N, K)) {
         rc = launch_up_chunks(t, r, bank_b, r, rows, x_dtype, N, addend, st);
         if (rc != I8F_OK) return rc;
     }
@@ -724,7 +748,7 @@ int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx
     if (rc != I8F_OK) return rc;
     rc = check_up(workspace, r, bank_b, adapters, r, rows, x_dtype, N);
     if (rc != I8F_OK) return rc;
-    rc = launch_down_chunks(x, ldx, bank_a, r, rows, workspace, r, x_dtype, K, nullptr, st);
+    rc = launch_down_chunks(x, ldx, bank_a, r, rows, workspace, r, x_dtype, K, nullptr, false, st);
     if (rc != I8F_OK) return rc;
     return linear_small_requests(x, x_dtype, ldx, w, ldw, w_scale, w_scale_mode, bias, bias_dtype, out, ldo, M, N, K, term, false, st);
 }
