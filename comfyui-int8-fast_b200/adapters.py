@@ -104,6 +104,41 @@ class RequestRows:
         return tiles, slots, np.stack([row, count, row_adapter[row], tiles[tile_of[row], 2] + row % TILE_ROWS], axis=1), addend_rows
 
 
+class RequestLoras:
+    """The adapters of one quantised layer for a batch whose samples belong to several requests, as the Linear holds them.
+
+    `entries[i]` is the bank entry of request i (-1: none), `plans` a dict that the layers of a model share, so that a batch
+    shape is planned once.  Sample j of a batch belongs to request j modulo the number of requests (a batch that repeats its
+    samples, for guidance say, repeats the requests with them).
+    """
+
+    def __init__(self, lora_a: Tensor, lora_b: Tensor, entries: Sequence[int], plans: dict | None = None):
+        if lora_a.dim() != 3 or lora_b.dim() != 3 or lora_a.shape[0] != lora_b.shape[0] or lora_a.shape[1] != lora_b.shape[2]:
+            raise ValueError(f"{tuple(lora_a.shape)} and {tuple(lora_b.shape)} are no bank [n, r, K], [n, N, r]")
+        if not len(entries) or any(not -1 <= e < lora_a.shape[0] for e in entries):
+            raise ValueError(f"entries {tuple(entries)} do not index a bank of {lora_a.shape[0]}")
+        self.lora_a, self.lora_b = lora_a, lora_b
+        self.entries = tuple(int(e) for e in entries)
+        self._plans = {} if plans is None else plans
+        self._converted = None
+
+    def bank(self, device: torch.device, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+        """The bank in the compute type on the compute device, converted once."""
+        if self._converted is None or self._converted[0].device != device or self._converted[0].dtype != dtype:
+            self._converted = (self.lora_a.to(device=device, dtype=dtype).contiguous(), self.lora_b.to(device=device, dtype=dtype).contiguous())
+        return self._converted
+
+    def rows(self, samples: int, rows_per_sample: int, device: torch.device) -> RequestRows:
+        n = len(self.entries)
+        if samples % n:
+            raise ValueError(f"a batch of {samples} samples for {n} requests")
+        key = (self.entries, samples, rows_per_sample, device)
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plans[key] = RequestRows([rows_per_sample] * samples, [self.entries[j % n] for j in range(samples)], device)
+        return plan
+
+
 def stack_adapters(factors: Sequence[tuple[Tensor, Tensor] | tuple[Tensor, Tensor, float]], dtype: torch.dtype,
                    device: torch.device | str) -> tuple[Tensor, Tensor]:
     """The adapters of one layer as a bank: `factors` holds (down [r_i, K], up [N, r_i]) or (down, up, scale) of each.

@@ -18,6 +18,7 @@ import torch.nn.functional as TF
 from torch import Tensor, nn
 
 from . import functional as F
+from .adapters import RequestRows
 from .ops import StandaloneInt8Ops as Ops
 
 
@@ -98,6 +99,45 @@ def attention_prenormed(qkv: Tensor, heads: int) -> Tensor:
     return out.transpose(1, 2).reshape(t, h)
 
 
+def attention_prenormed_batch(qkv: Tensor, heads: int) -> Tensor:
+    """qkv [B, T, 3*h] (any row pitch) whose q and k are normalised already -> [B, T, h]."""
+    b, t, h3 = qkv.shape
+    h = h3 // 3
+    q, k, v = (p.unflatten(-1, (heads, h // heads)) for p in qkv.split(h, dim=-1))
+    out = TF.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
+    return out.transpose(1, 2).reshape(b, t, h)
+
+
+@dataclass(frozen=True)
+class BatchRows:
+    """Row plans of a batch of samples for the image stream, the text stream and both joined."""
+    samples: int
+    img: RequestRows
+    txt: RequestRows
+    all: RequestRows
+
+    @classmethod
+    def of(cls, samples: int, n_img: int, n_txt: int, device) -> "BatchRows":
+        return cls(samples, *(RequestRows([n] * samples, None, device) for n in (n_img, n_txt, n_img + n_txt)))
+
+
+@dataclass(frozen=True)
+class Pending:
+    """A residual stream x [rows, h] and what is still to be added to it, gate * y with one gate per sample."""
+    x: Tensor
+    y: Tensor | None = None
+    gate: Tensor | None = None
+
+    def settle(self, rows: RequestRows, shift: Tensor, scale: Tensor):
+        """The stream with that added, and its LayerNorm, modulated per sample, as per-token int8: one pass over both."""
+        y = torch.zeros_like(self.x) if self.y is None else self.y
+        return F.quantize_rowwise_gated_residual_norm(self.x, y, self.gate, rows=rows, norm="layer", scale=scale, shift=shift, eps=1e-5)
+
+    def total(self, samples: int) -> Tensor:
+        x = self.x.view(samples, -1, self.x.shape[1])
+        return x if self.y is None else gated_residual(x, self.gate, self.y.view_as(x))
+
+
 def rms_norm(x: Tensor, eps: float = 1e-6) -> Tensor:
     return TF.rms_norm(x, x.shape[-1:], eps=eps)
 
@@ -168,6 +208,29 @@ class DoubleBlock(nn.Module):
             outs.append(x)
         return outs[1], outs[0]
 
+    def forward_requests(self, img, txt, vec: Tensor, batch: "BatchRows"):
+        """The fused code for a batch of samples, each with its own modulation.  img, txt: `Pending` residual streams of
+        [B * T, h]; what a block adds last is left to the next block, whose norm and quantisation it shares a pass with."""
+        cfg = self.cfg
+        h = cfg.hidden
+        B, n_txt, n_img = batch.samples, batch.txt.total // batch.samples, batch.img.total // batch.samples
+        qkv = torch.empty((B, n_txt + n_img, 3 * h), dtype=torch.bfloat16, device=vec.device)
+        mods, xs = {}, {}
+        for name, x, blk, rows, part in (("txt", txt, self.txt, batch.txt, qkv[:, :n_txt]), ("img", img, self.img, batch.img, qkv[:, n_txt:])):
+            mods[name] = blk.mod(TF.silu(vec)).chunk(6, dim=-1)
+            xs[name], q8, scale = x.settle(rows, mods[name][0], mods[name][1])
+            part.copy_(int8_gemm(blk.qkv, q8, scale).view(B, -1, 3 * h))
+        F.rmsnorm_heads_(qkv.view(-1, 3 * h)[:, : 2 * h])
+        attn = attention_prenormed_batch(qkv, cfg.heads)
+        outs = []
+        for name, blk, rows, a in (("txt", self.txt, batch.txt, attn[:, :n_txt]), ("img", self.img, batch.img, attn[:, n_txt:])):
+            sh1, sc1, g1, sh2, sc2, g2 = mods[name]
+            y = int8_gemm(blk.proj, *F.quantize_rowwise(a.reshape(-1, h)))
+            x, q8, scale = Pending(xs[name], y, g1).settle(rows, sh2, sc2)
+            q8, scale = F.quantize_rowwise_gelu(int8_gemm(blk.mlp_up, q8, scale))
+            outs.append(Pending(x, int8_gemm(blk.mlp_down, q8, scale), g2))
+        return outs[1], outs[0]
+
     def forward(self, img: Tensor, txt: Tensor, vec: Tensor):
         cfg = self.cfg
         mods = {}
@@ -206,6 +269,17 @@ class SingleBlock(nn.Module):
         q8, xs = F.quantize_rowwise_gelu(y[:, 3 * h:], attn)
         return int8_gemm_gated_add_(self.linear2, x, gate, q8, xs)
 
+    def forward_requests(self, x: "Pending", vec: Tensor, batch: "BatchRows") -> "Pending":
+        """The fused code for a batch of samples, each with its own modulation (see DoubleBlock.forward_requests)."""
+        h = self.cfg.hidden
+        shift, scale, gate = self.mod(TF.silu(vec)).chunk(3, dim=-1)
+        x, q8, xs = x.settle(batch.all, shift, scale)
+        y = int8_gemm(self.linear1, q8, xs)
+        F.rmsnorm_heads_(y[:, : 2 * h])
+        attn = attention_prenormed_batch(y.view(batch.samples, -1, y.shape[1])[..., : 3 * h], self.cfg.heads)
+        q8, xs = F.quantize_rowwise_gelu(y[:, 3 * h:], attn.reshape(-1, h))
+        return Pending(x, int8_gemm(self.linear2, q8, xs), gate)
+
     def forward(self, x: Tensor, vec: Tensor) -> Tensor:
         h = self.cfg.hidden
         shift, scale, gate = self.mod(TF.silu(vec)).chunk(3, dim=-1)
@@ -225,13 +299,17 @@ def timestep_embedding(t: Tensor, dim: int = 256) -> Tensor:
 
 
 class SyntheticDiT(nn.Module):
-    def __init__(self, cfg: DiTConfig = DiTConfig(), seed: int = 0, device="cuda", fused: bool = True):
-        """`fused` selects the block code that uses the library's fused quantiser prologues and the per-head RMS-norm
+    def __init__(self, cfg: DiTConfig = DiTConfig(), seed: int = 0, device="cuda", fused: bool = True, fused_batch: bool = False):
+        """`fused_batch` does for batches of several samples (each with its own time step, so its own modulation) what `fused`
+        does for one: the gated residual updates, the norms around them and the quantisation run as one pass per block half.
+        Make the first call of a shape outside a graph capture (it plans the rows).  `fused` selects the block code that uses the library's fused quantiser prologues and the per-head RMS-norm
         kernel (batch 1, head size 128); otherwise every element-wise step is its own PyTorch call, which is how a
         model written against the node pack's Linear alone would run."""
         super().__init__()
         self.cfg = cfg
         self.fused = fused
+        self.fused_batch = fused_batch
+        self._batch_rows: dict = {}
         gen = torch.Generator(device=device)
         gen.manual_seed(seed)
         h = cfg.hidden
@@ -256,6 +334,18 @@ class SyntheticDiT(nn.Module):
             for blk in self.single_stream:
                 x2 = blk.forward_fused(x2, vec)
             x = x2[None]
+        elif self.fused_batch and self.cfg.head_dim == 128 and self.cfg.hidden % 8 == 0:
+            key = (img.shape[0], img.shape[1], txt.shape[1], img.device)
+            batch = self._batch_rows.get(key)
+            if batch is None:
+                batch = self._batch_rows[key] = BatchRows.of(*key)
+            img2, txt2 = Pending(img.flatten(0, 1)), Pending(txt.flatten(0, 1))
+            for blk in self.double_stream:
+                img2, txt2 = blk.forward_requests(img2, txt2, vec, batch)
+            x2 = Pending(torch.cat([txt2.total(batch.samples), img2.total(batch.samples)], dim=1).flatten(0, 1))
+            for blk in self.single_stream:
+                x2 = blk.forward_requests(x2, vec, batch)
+            x = x2.total(batch.samples)
         else:
             for blk in self.double_stream:
                 img, txt = blk(img, txt, vec)

@@ -14,6 +14,7 @@ import torch.nn.functional as TF
 from torch import Tensor, nn
 
 from . import _native as nat
+from . import adapters
 from . import custom_ops
 from . import functional as F
 from . import quarot
@@ -304,7 +305,11 @@ if _LORA_ADAPTER_AVAILABLE:
 # =============================================================================
 class DynamicLoRAHook:
     """Forward-pre-hook on the diffusion model: keeps every quantised layer's lora_A / lora_B in
-    sync with the `dynamic_loras` list carried in transformer_options."""
+    sync with the `dynamic_loras` list carried in transformer_options.
+
+    `request_loras` in transformer_options gives a batch one composition per request: a list with, for every request, a list
+    of entries like those of `dynamic_loras` (which all requests share on top).  Each quantised layer then holds a bank of the
+    distinct compositions (`request_loras`) in place of lora_A / lora_B."""
 
     def __init__(self):
         self.current_lora_id = None
@@ -314,11 +319,61 @@ class DynamicLoRAHook:
         if not opts and len(input_args) > 2 and isinstance(input_args[2], dict):
             opts = input_args[2].get("transformer_options", {})
         loras = opts.get("dynamic_loras", [])
+        requests = opts.get("request_loras", [])
         lora_id = hash(tuple((id(d["patches"]), d["strength"]) for d in loras)) if loras else None
+        if requests:
+            lora_id = (lora_id, tuple(tuple((id(d["patches"]), d["strength"]) for d in r) for r in requests))
         if lora_id != self.current_lora_id:
-            self.apply_composition(module, loras)
+            if requests:
+                self.apply_requests(module, loras, requests)
+            else:
+                self.apply_composition(module, loras)
             self.current_lora_id = lora_id
         return None
+
+    @staticmethod
+    def _factors(patches):
+        """A stack of low-rank patches as one pair: downs with their scales one below the other, ups side by side."""
+        downs, ups = [], []
+        for adapter, strength in patches:
+            up, down, alpha, mid = adapter.weights[:4]
+            rank = down.shape[0] if down.ndim >= 2 else 1
+            if mid is not None:
+                down = torch.mm(mid.flatten(1), down.flatten(1)).reshape(down.shape)
+            downs.append(down * lora_scale_of(alpha, rank, strength))
+            ups.append(up)
+        return torch.cat(downs, dim=0), torch.cat(ups, dim=1)
+
+    def apply_requests(self, diffusion_model, dynamic_loras, request_loras):
+        """One bank per layer: an entry for every distinct composition that patches it (zeros where another layer's does)."""
+        compositions: dict = {}      # key -> (entry, stack)
+        entries = []
+        for r in request_loras:
+            stack = [*(dynamic_loras or []), *r]
+            key = tuple((id(d["patches"]), d["strength"]) for d in stack)
+            entries.append(compositions.setdefault(key, (len(compositions), stack))[0] if stack else -1)
+        stacks = [stack for _, stack in compositions.values()]
+        plans: dict = {}
+        for name, module in diffusion_model.named_modules():
+            if not hasattr(module, "lora_A"):
+                continue
+            module.lora_alpha = module.lora_A = module.lora_B = None
+            module._lora_cache = None
+            module.request_loras = None
+            keys = (f"diffusion_model.{name}.weight", f"{name}.weight")
+            pairs = []
+            for stack in stacks:
+                found = [[(d["patches"][k], d["strength"]) for d in stack if k in d["patches"]] for k in keys]
+                patches = found[0] or found[1]
+                pairs.append(self._factors(patches) if patches else None)
+            if not any(p is not None for p in pairs):
+                continue
+            some = next(p for p in pairs if p is not None)
+            K, N = some[0].flatten(1).shape[1], some[1].flatten(1).shape[0]
+            empty = (some[0].new_zeros(0, K), some[1].new_zeros(N, 0))
+            device = getattr(module, "weight", torch.tensor(0)).device
+            bank = adapters.stack_adapters([p if p is not None else empty for p in pairs], some[0].dtype, device)
+            module.request_loras = adapters.RequestLoras(*bank, entries, plans)
 
     def apply_composition(self, diffusion_model, dynamic_loras):
         per_layer: dict = {}
@@ -331,20 +386,14 @@ class DynamicLoRAHook:
             patches = per_layer.get(f"diffusion_model.{name}.weight") or per_layer.get(f"{name}.weight")
             module.lora_alpha = None
             module._lora_cache = None      # converted copies of the factors belong to the tensors replaced below
+            module.request_loras = None
             if not patches:
                 module.lora_A = module.lora_B = None
                 continue
-            downs, ups = [], []
-            for adapter, strength in patches:
-                up, down, alpha, mid = adapter.weights[:4]
-                rank = down.shape[0] if down.ndim >= 2 else 1
-                if mid is not None:
-                    down = torch.mm(mid.flatten(1), down.flatten(1)).reshape(down.shape)
-                downs.append(down * lora_scale_of(alpha, rank, strength))
-                ups.append(up)
+            down, up = self._factors(patches)
             device = getattr(module, "weight", torch.tensor(0)).device
-            module.lora_A = torch.cat(downs, dim=0).to(device)   # [sum r, K]
-            module.lora_B = torch.cat(ups, dim=1).to(device)     # [N, sum r]
+            module.lora_A = down.to(device)   # [sum r, K]
+            module.lora_B = up.to(device)     # [N, sum r]
 
     @classmethod
     def register(cls, diffusion_model):
@@ -389,6 +438,22 @@ def _prepare_lora(module, device: torch.device, dtype: torch.dtype):
     return a, b
 
 
+@torch.compiler.disable
+def _request_forward(loras, x: Tensor, samples: int, weight: Tensor, w_scale, bias: Tensor | None, dtype: torch.dtype, hadamard: bool,
+                     rotated_lora_input: bool) -> Tensor:
+    """The Linear's forward for a batch with one adapter per request.  x [rows, K]: `samples` equal runs of rows."""
+    if x.shape[0] % samples:
+        raise ValueError(f"{x.shape[0]} rows are not {samples} samples of equal length")
+    plan = loras.rows(samples, x.shape[0] // samples, x.device)
+    lora_a, lora_b = loras.bank(x.device, dtype)
+    if x.shape[0] > SMALL_BATCH_ROWS:
+        return F.linear_lora_requests(x, weight, w_scale, bias, lora_a, lora_b, plan, dtype, hadamard=hadamard,
+                                      rotated_lora_input=rotated_lora_input)
+    if hadamard:
+        x = quarot.rotate_activation(x, None, quarot.GROUP_SIZE)
+    return F.linear_small_batch_lora_requests(x, weight, w_scale, bias, lora_a, lora_b, plan)
+
+
 def _define_ops(manual_cast, cast_bias_weight, uncast_bias_weight):
     class Int8TensorwiseOps(manual_cast):
         """ComfyUI custom operations: Linear layers hold int8 weights and run the sm_100a W8A8 kernels."""
@@ -411,6 +476,7 @@ def _define_ops(manual_cast, cast_bias_weight, uncast_bias_weight):
                 self.lora_A = None
                 self.lora_B = None
                 self.lora_alpha = None
+                self.request_loras = None    # adapters.RequestLoras: one adapter per request of the batch
                 self._scalar_scale_dev = None
 
             def reset_parameters(self):
@@ -552,7 +618,11 @@ def _define_ops(manual_cast, cast_bias_weight, uncast_bias_weight):
                 rows = x2.shape[0]
                 has_lora = self.lora_A is not None and self.lora_B is not None
 
-                if rows > SMALL_BATCH_ROWS and has_lora:
+                if self.request_loras is not None:
+                    samples = x.shape[0] if x.dim() > 2 else len(self.request_loras.entries)
+                    y = _request_forward(self.request_loras, x2, samples, weight, w_scale, bias, compute_dtype, self._use_quarot,
+                                         Int8TensorwiseOps.lora_uses_rotated_input)
+                elif rows > SMALL_BATCH_ROWS and has_lora:
                     # t = x @ A^T first; t @ B^T is accumulated inside the int8 GEMM kernel and added in its
                     # epilogue with the reference's roundings: y = round(round(dequant + bias) + round(lora_y))
                     lora_a, lora_b = _prepare_lora(self, x.device, compute_dtype)

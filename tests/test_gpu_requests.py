@@ -548,3 +548,66 @@ def test_draws_of_row_plans(cuda_pkg):
         term, term_tol = low_rank(x, la, lb, adapter_rows(rows), dtype)
         want, off = base + term, base_tol + term_tol + 2 * (r // 16 + 1) * E32 * (base.abs() + term.abs())
         check(y, want, off + u_of(dtype) * (want.abs() + off) + TINY[dtype])
+
+
+# ------------------------------------------------------------------ the layers and the model that use them
+@pytest.mark.parametrize("tokens", [1, 4, 5, 200])
+@pytest.mark.parametrize("quarot", [False, True])
+def test_linear_module_with_request_loras(cuda_pkg, tokens, quarot):
+    """The Linear of a batch of requests gives every sample what it gives that sample's LoRA alone."""
+    F, nat = cuda_pkg.functional, cuda_pkg._native
+    K, N, r = 256, 320, 16
+    w, ws, b, la, lb = layer(K, N, r, 3, torch.bfloat16, 41)
+    lin = cuda_pkg.ops.StandaloneInt8Ops.Linear(K, N, bias=True, device="meta")
+    lin._load_from_state_dict({"weight": w, "weight_scale": ws, "bias": b}, "", {}, True, [], [], [])
+    lin._use_quarot = quarot
+    x = torch.randn(8, tokens, K, generator=gen(42), device=DEV).bfloat16()
+    lin.request_loras = cuda_pkg.adapters.RequestLoras(la, lb, [1, -1, 2, 1])
+    y = lin(x)
+    assert y.shape == (8, tokens, N)
+    xr = cuda_pkg.quarot.rotate_activation(x.reshape(-1, K), None, 128).reshape(x.shape) if quarot else x
+    u = u_of(torch.bfloat16)
+    for j in range(8):
+        e = (1, -1, 2, 1)[j % 4]
+        at = torch.full((tokens,), e, device=DEV)
+        if 8 * tokens > 16:
+            base, off = base_quantised(*F.quantize_rowwise(x[j], hadamard=quarot), w, ws, b)
+        else:
+            base = (xr[j].to(F64) @ w.to(F64).T) * ws.to(F64).T + b.to(F64)
+            off = (2 * K + 8) * E32 * ((xr[j].to(F64).abs() @ w.to(F64).abs().T) * ws.to(F64).T + b.to(F64).abs())
+        term, term_tol = low_rank(xr[j], la, lb, at, torch.bfloat16)
+        want, off = base + term, off + term_tol + 4 * E32 * (base.abs() + term.abs())
+        check(y[j], want, off + u * (want.abs() + off))
+    with pytest.raises(ValueError):
+        lin(x[:6])
+    flat = cuda_pkg.adapters.RequestLoras(la, lb, [1, -1, 2, 1] * 2)
+    lin.request_loras = flat
+    assert torch.equal(lin(x.reshape(-1, K)).reshape(y.shape), y)      # two dimensions: as many runs of rows as requests
+
+
+def test_dit_batch_of_samples_fused(cuda_pkg):
+    """A batch of samples through the fused block code against the same model in element-wise steps: the differences are 16-bit
+    roundings that the fused pass leaves out, and the int8 steps they move."""
+    import importlib
+    dit = importlib.import_module(cuda_pkg.__name__ + ".dit")
+    cfg = dit.DiTConfig(hidden=512, heads=4, mlp_ratio=3, double_blocks=2, single_blocks=2, img_tokens=96, txt_tokens=40, txt_dim=256)
+    model = dit.SyntheticDiT(cfg, seed=3, fused_batch=True)
+    g = gen(44)
+    img = torch.randn(3, 96, cfg.in_channels, generator=g, device=DEV).bfloat16()
+    txt = torch.randn(3, 40, cfg.txt_dim, generator=g, device=DEV).bfloat16()
+    t = torch.tensor([0.9, 0.4, 0.1], device=DEV)
+    got = model(img, txt, t)
+    model.fused_batch = False
+    want = model(img, txt, t)
+    assert got.shape == want.shape
+    rel = float((got.float() - want.float()).norm() / want.float().norm())
+    assert rel < 0.05, rel
+    # every sample has its own modulation: the first sample's result does not depend on the others' time steps
+    model.fused_batch = True
+    again = model(img, txt, torch.tensor([0.9, 0.7, 0.8], device=DEV))
+    assert torch.equal(again[0], got[0]) and not torch.equal(again[1], got[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = model(img, txt, t)
+    graph.replay()
+    assert torch.equal(captured, got)

@@ -180,3 +180,78 @@ def test_abi_refuses_bad_norm_calls(pkg):
         assert call(**kw) == want, kw
         assert nat.last_error()
     assert call(M=0) == 0 and call(K=0) == 0
+
+
+class _Adapter:
+    def __init__(self, up, down, alpha=None, mid=None):
+        self.weights = (up, down, alpha, mid, None, None)
+
+
+class _Layer(torch.nn.Module):
+    def __init__(self, n, k):
+        super().__init__()
+        self.weight = torch.nn.Parameter(torch.zeros(n, k), requires_grad=False)
+        self.lora_A = self.lora_B = self.lora_alpha = self.request_loras = None
+
+
+def test_hook_gives_each_request_its_composition(pkg):
+    g = torch.Generator().manual_seed(2)
+    model = torch.nn.ModuleDict({"a": _Layer(24, 32), "b": _Layer(16, 32), "c": _Layer(8, 8)})
+
+    def entry(strength, **layers):
+        return {"patches": {f"diffusion_model.{k}.weight": _Adapter(torch.randn(n, r, generator=g), torch.randn(r, 32, generator=g), 4.0)
+                            for k, (n, r) in layers.items()}, "strength": strength}
+
+    one, two, shared = entry(0.5, a=(24, 3), b=(16, 5)), entry(1.0, a=(24, 9)), entry(2.0, b=(16, 2))
+    hook = pkg.ops.DynamicLoRAHook()
+    opts = {"request_loras": [[one], [], [one, two], [one]]}
+    hook.pre_forward(model, (), {"transformer_options": opts})
+
+    def delta(layer, i):
+        e = model[layer].request_loras.entries[i]
+        bank = model[layer].request_loras
+        return torch.zeros(bank.lora_b.shape[1], 32) if e < 0 else bank.lora_b[e] @ bank.lora_a[e]
+
+    def want(layer, *entries):
+        total = torch.zeros(model[layer].weight.shape)
+        for d in entries:
+            ad = d["patches"].get(f"diffusion_model.{layer}.weight")
+            if ad is not None:
+                up, down, alpha = ad.weights[:3]
+                total = total + (alpha / down.shape[0] * d["strength"]) * (up @ down)
+        return total
+
+    def check(per_request):
+        for layer in "ab":
+            for i, entries in enumerate(per_request):
+                # at most 14 products of magnitudes that add up to less than 200, each rounded to fp32 a few times
+                torch.testing.assert_close(delta(layer, i), want(layer, *entries), rtol=0, atol=14 * 4 * 2 ** -24 * 200)
+
+    check([[one], [], [one, two], [one]])
+    assert model["a"].request_loras.entries == (0, -1, 1, 0) and model["a"].request_loras.lora_a.shape == (2, 16, 32)
+    assert model["c"].request_loras is None and model["a"].lora_A is None
+    before = model["a"].request_loras
+    hook.pre_forward(model, (), {"transformer_options": opts})
+    assert model["a"].request_loras is before                    # the same requests: nothing is rebuilt
+    hook.pre_forward(model, (), {"transformer_options": {**opts, "dynamic_loras": [shared]}})
+    check([[shared, one], [shared], [shared, one, two], [shared, one]])
+    # plans are shared by the layers, repeated samples repeat the requests
+    plan = model["a"].request_loras.rows(8, 5, torch.device("cpu"))
+    assert plan is model["b"].request_loras.rows(8, 5, torch.device("cpu"))
+    assert plan.lengths == (5,) * 8 and plan.adapters == model["a"].request_loras.entries * 2
+    with pytest.raises(ValueError):
+        model["a"].request_loras.rows(6, 5, torch.device("cpu"))
+    # back to one composition for all, then to none
+    hook.pre_forward(model, (), {"transformer_options": {"dynamic_loras": [one]}})
+    assert model["a"].request_loras is None and model["a"].lora_A.shape == (3, 32)
+    hook.pre_forward(model, (), {"transformer_options": {}})
+    assert model["a"].request_loras is None and model["a"].lora_A is None
+
+
+def test_request_loras_refuse(pkg):
+    A = pkg.adapters.RequestLoras
+    a, b = torch.zeros(2, 8, 32), torch.zeros(2, 24, 8)
+    assert A(a, b, [0, -1, 1]).entries == (0, -1, 1)
+    for args in ((a[0], b, [0]), (a, b[:1], [0]), (a, b[:, :, :4], [0]), (a, b, []), (a, b, [2]), (a, b, [-2])):
+        with pytest.raises(ValueError):
+            A(*args)
