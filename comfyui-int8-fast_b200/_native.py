@@ -99,8 +99,8 @@ _PROTOTYPES = {
     "i8f_linear_w8a16_small_lora_requests": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int,
                                                      c_void_p, c_void_p, c_int64, c_int64, _ROWS, c_void_p, c_int64, c_int64,
                                                      c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
-    "i8f_gated_residual_norm": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p,
-                                        c_int64, c_int, c_float, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+    "i8f_gated_residual_norm": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                                        c_void_p, c_int64, c_int, c_float, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p,
                                         c_int64, c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                                         c_void_p]),
     "i8f_lora_merge_sr": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int,

@@ -23,6 +23,7 @@ namespace {
 
 constexpr float kScaleFloor = 1e-30f;
 constexpr int kMaxWarps = 16;
+constexpr int kRowsPerRequest = 6;
 constexpr int kRingRows = 256;      // batches of at least so many rows use the ring kernel
 
 struct NormArgs {
@@ -278,8 +279,11 @@ gated_residual_norm_kernel(const NormArgs a) {
 // pieces that contain the row; a row that starts `o` elements behind a boundary is handled in the vectors of its memory,
 // elements 8 v - o ... 8 v - o + 7, so that all but the first and the last are read and written in 16-byte pieces.  x, y
 // and the outputs must lie alike (o is the same for all of them), as contiguous tensors of one shape do.
-constexpr int kWorkers = 512;             // threads that take rows
-constexpr int kRingThreads = kWorkers + 32;
+// Threads that take rows.  Five groups hide a row's chain of reductions better than four (4608 x 4096 bf16: 32.3 us against 34.5,
+// with int8 rows 30.0 against 32.6); fp32 rows leave room for seven slots only, and four groups serve them better (18432 x
+// 4096: 162 us against 166).
+template <int XDT, int GT>
+constexpr int workers() { return GT == 512 ? 512 : (XDT == I8F_F32 ? 4 : 5) * GT; }
 constexpr int kMaxSlots = 16;
 constexpr int kRingSmem = 224 * 1024;
 
@@ -435,11 +439,12 @@ __device__ __forceinline__ void column8(const void* base, int64_t at, int e0, in
 }
 
 template <int XDT, int YDT, int GT, int VPT, bool SHIFT>
-__global__ void __launch_bounds__(kRingThreads, 1)
+__global__ void __launch_bounds__((workers<XDT, GT>() + 32), 1)
 gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, int* status) {
     using TX = typename Elem<XDT>::T;
     using TY = typename Elem<YDT>::T;
     using C = Columns<GT, VPT, SHIFT>;
+    constexpr int kWorkers = workers<XDT, GT>();
     constexpr int kGroups = kWorkers / GT;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) float s_part[2 * kWorkers / 32];
@@ -514,7 +519,7 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
             }
             if (req != have) {
                 have = req;
-                asm volatile("bar.sync 15, 512;" ::: "memory");      // every group is done with the request before
+                asm volatile("bar.sync 15, %0;" ::"n"(kWorkers) : "memory");      // every group is done with the request before
                 // (K + 7) / 8 vectors of the row as if it were aligned
                 for (int e0 = static_cast<int>(threadIdx.x) * 8; e0 < K; e0 += kWorkers * 8) {
                     float g[8], pw[8], sc[8], w[8], sh[8];
@@ -540,7 +545,7 @@ gated_residual_norm_ring_kernel(const NormArgs a, int n_slots, int all_columns, 
                         }
                     }
                 }
-                asm volatile("bar.sync 15, 512;" ::: "memory");
+                asm volatile("bar.sync 15, %0;" ::"n"(kWorkers) : "memory");
             }
             for (; row < seg1; row += kGroups) {
                 // After a wait that ran out the rows are walked to the end all the same (every later wait gives up at once):
@@ -732,7 +737,7 @@ int launch_ring(const NormArgs& a, int min_slots, int sms, cudaStream_t st, bool
     int* status = device_status_word();
     I8F_REQUIRE(status != nullptr, I8F_ERR_CUDA, "device status word unavailable");
     const int64_t grid = a.M < sms ? a.M : sms;
-    kern<<<static_cast<unsigned>(grid), kRingThreads, (all_columns ? 3 : 1) * kArray + n_slots * slot, st>>>(a, n_slots, all_columns, status);
+    kern<<<static_cast<unsigned>(grid), (workers<XDT, GT>() + 32), (all_columns ? 3 : 1) * kArray + n_slots * slot, st>>>(a, n_slots, all_columns, status);
     return check_launch("gated_residual_norm_ring_kernel");
 }
 
@@ -746,10 +751,11 @@ int launch_ring_for(const NormArgs& a, int sms, cudaStream_t st, bool* done) {
         const int rc = launch_ring<XDT, YDT, GT, VPT, SHIFT>(a, MIN, sms, st, done);              \
         if (rc != I8F_OK || *done) return rc;                                                     \
     }
-    // four rows at a time up to 4096 columns, longer rows one at a time; at least one row more in flight than at work
-    I8F_TRY(128, 1, 5)
-    I8F_TRY(128, 2, 5)
-    I8F_TRY(128, 4, 5)
+    // several rows at a time up to 4096 columns, longer rows one at a time; at least one row more in flight than at work
+    constexpr int kMin = workers<XDT, 128>() / 128 + 1;
+    I8F_TRY(128, 1, kMin)
+    I8F_TRY(128, 2, kMin)
+    I8F_TRY(128, 4, kMin)
     I8F_TRY(512, 2, 2)
     I8F_TRY(512, 4, 2)
 #undef I8F_TRY
@@ -757,7 +763,7 @@ int launch_ring_for(const NormArgs& a, int sms, cudaStream_t st, bool* done) {
 }
 
 template <int XDT, int YDT>
-int launch_norm(const NormArgs& a, bool vec8, bool alike, cudaStream_t st) {
+int launch_norm(const NormArgs& a, int64_t requests, bool vec8, bool alike, cudaStream_t st) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -765,8 +771,10 @@ int launch_norm(const NormArgs& a, bool vec8, bool alike, cudaStream_t st) {
     // Which kernel (us at K columns, bf16, measured): fewer than 256 rows one CTA each (64 rows of 4096: 4.2, in the ring 6.1;
     // 512 rows: 10.7 and 7.5).  Rows of up to 512 columns a warp each (4608 rows of 512: 8.4, in the ring 14.4; of 1024: 19.0
     // and 14.6), up to 256 where the rows are not aligned.
+    // Requests of a few rows each: working a request's columns out costs the ring about 4.6 us (4608 rows of 4096, one row per
+    // request: 174 us, a CTA per row 64; 18 rows per request: 40 in the ring).
     const int warp_columns = vec8 ? 512 : 256;
-    if (a.M >= kRingRows && a.K > warp_columns) {
+    if (a.M >= kRingRows && a.K > warp_columns && a.M >= kRowsPerRequest * requests) {
         bool done = false;
         const int rc = vec8 ? launch_ring_for<XDT, YDT, false>(a, sms, st, &done) : alike ? launch_ring_for<XDT, YDT, true>(a, sms, st, &done) : I8F_OK;
         if (rc != I8F_OK || done) return rc;
@@ -796,7 +804,7 @@ bool vec_ok(const void* p, int64_t ld, int elem) { return p == nullptr || (align
 using namespace i8f;
 
 extern "C" int i8f_gated_residual_norm(const void* x, int x_dtype, int64_t ldx, const void* y, int y_dtype, int64_t ldy,
-                                       int64_t M, int64_t K, const int32_t* row_request, const void* gate, int64_t ldg,
+                                       int64_t M, int64_t K, const int32_t* row_request, int64_t requests, const void* gate, int64_t ldg,
                                        int gate_tanh, float residual_scale, int post_norm, const void* post_weight, int norm,
                                        const void* weight, const void* scale, int64_t lds, const void* shift, int64_t ldt,
                                        float eps, void* x_out, int64_t ldxo, void* h, int64_t ldh, int8_t* q, int64_t ldq,
@@ -809,6 +817,7 @@ extern "C" int i8f_gated_residual_norm(const void* x, int x_dtype, int64_t ldx, 
     I8F_REQUIRE(post_norm >= I8F_NORM_NONE && post_norm <= I8F_NORM_LAYER && norm >= I8F_NORM_RMS && norm <= I8F_NORM_LAYER,
                 I8F_ERR_INVALID_ARG, "%s: unknown norm (post_norm=%d, norm=%d)", what, post_norm, norm);
     I8F_REQUIRE(eps >= 0.f, I8F_ERR_INVALID_ARG, "%s: eps must not be negative", what);
+    I8F_REQUIRE(requests >= 1, I8F_ERR_INVALID_ARG, "%s: requests must be positive", what);
     if (M == 0 || K == 0) return I8F_OK;
     I8F_REQUIRE(x != nullptr && y != nullptr && x_out != nullptr, I8F_ERR_INVALID_ARG, "%s: NULL input or output", what);
     I8F_REQUIRE(h != nullptr || q != nullptr, I8F_ERR_INVALID_ARG, "%s: h and q are both NULL", what);
@@ -858,6 +867,6 @@ extern "C" int i8f_gated_residual_norm(const void* x, int x_dtype, int64_t ldx, 
     a.eps = eps;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f32 = x_dtype == I8F_F32;
-    if (y_dtype == I8F_BF16) return f32 ? launch_norm<I8F_F32, I8F_BF16>(a, vec8, alike, st) : launch_norm<I8F_BF16, I8F_BF16>(a, vec8, alike, st);
-    return f32 ? launch_norm<I8F_F32, I8F_F16>(a, vec8, alike, st) : launch_norm<I8F_F16, I8F_F16>(a, vec8, alike, st);
+    if (y_dtype == I8F_BF16) return f32 ? launch_norm<I8F_F32, I8F_BF16>(a, requests, vec8, alike, st) : launch_norm<I8F_BF16, I8F_BF16>(a, requests, vec8, alike, st);
+    return f32 ? launch_norm<I8F_F32, I8F_F16>(a, requests, vec8, alike, st) : launch_norm<I8F_F16, I8F_F16>(a, requests, vec8, alike, st);
 }

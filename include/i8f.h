@@ -367,7 +367,8 @@ int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx
 #define I8F_NORM_RMS 1
 #define I8F_NORM_LAYER 2
 
-/* Gated residual update between two norms, per row m of request q(m) = row_request[m] (NULL: 0 for every row):
+/* Gated residual update between two norms, per row m of request q(m) = row_request[m] (NULL: 0 for every row; `requests`
+ * of them, 1 with NULL):
  *   x_out = residual_scale * x + g * post_norm(y) * post_weight       g = gate[q] or, with gate_tanh, tanh(gate[q])
  *   h     = norm(x_out) * weight * (1 + scale[q]) + shift[q]
  * fp32 throughout; h comes from the unrounded x_out, so each output is rounded once.  x, x_out [M,K] in x_dtype
@@ -377,7 +378,8 @@ int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx
  * K at most 16384; rows of any length, pitch and alignment (16-byte aligned rows of a multiple of 8 elements are read
  * and written in 16-byte pieces). */
 int i8f_gated_residual_norm(const void* x, int x_dtype, int64_t ldx, const void* y, int y_dtype, int64_t ldy,
-                            int64_t M, int64_t K, const int32_t* row_request, const void* gate, int64_t ldg, int gate_tanh,
+                            int64_t M, int64_t K, const int32_t* row_request, int64_t requests,
+                            const void* gate, int64_t ldg, int gate_tanh,
                             float residual_scale, int post_norm, const void* post_weight, int norm, const void* weight,
                             const void* scale, int64_t lds, const void* shift, int64_t ldt, float eps,
                             void* x_out, int64_t ldxo, void* h, int64_t ldh, int8_t* q, int64_t ldq, float* row_scale,

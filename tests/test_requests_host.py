@@ -168,13 +168,13 @@ def test_abi_refuses_bad_norm_calls(pkg):
     lib = nat.load()
 
     def call(x=P, xdt=nat.I8F_BF16, ldx=64, y=P, ydt=nat.I8F_BF16, ldy=64, M=8, K=64, gate=P, ldg=64, post=1, norm=1, scale=None, lds=0,
-             shift=None, ldt=0, eps=1e-6, xo=P, ldxo=64, h=P, ldh=64, q=None, ldq=0, rs=None):
-        return lib.i8f_gated_residual_norm(x, xdt, ldx, y, ydt, ldy, M, K, None, gate, ldg, 0, 1.0, post, None, norm, None, scale, lds, shift,
+             shift=None, ldt=0, eps=1e-6, xo=P, ldxo=64, h=P, ldh=64, q=None, ldq=0, rs=None, req=1):
+        return lib.i8f_gated_residual_norm(x, xdt, ldx, y, ydt, ldy, M, K, None, req, gate, ldg, 0, 1.0, post, None, norm, None, scale, lds, shift,
                                            ldt, eps, xo, ldxo, h, ldh, q, ldq, rs, None)
 
     for want, kw in ((-3, dict(ydt=nat.I8F_F32)), (-3, dict(xdt=nat.I8F_F16)), (-1, dict(M=-1)), (-1, dict(K=-8)),
                      (-3, dict(K=16392, ldx=16392, ldy=16392, ldg=16392, ldxo=16392, ldh=16392)), (-1, dict(post=3)), (-1, dict(norm=0)),
-                     (-1, dict(eps=-1.0)), (-1, dict(x=None)), (-1, dict(y=None)), (-1, dict(xo=None)), (-1, dict(h=None)),
+                     (-1, dict(eps=-1.0)), (-1, dict(req=0)), (-1, dict(x=None)), (-1, dict(y=None)), (-1, dict(xo=None)), (-1, dict(h=None)),
                      (-1, dict(h=None, q=P, ldq=64)), (-1, dict(ldx=63)), (-1, dict(ldy=63)), (-1, dict(ldxo=63)), (-1, dict(ldh=63)),
                      (-1, dict(q=P, ldq=63, rs=P)), (-1, dict(ldg=63)), (-1, dict(scale=P, lds=63)), (-1, dict(shift=P, ldt=63))):
         assert call(**kw) == want, kw
