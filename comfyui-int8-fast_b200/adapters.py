@@ -48,7 +48,7 @@ class RequestRows:
         self.max_adapter = int(used.max()) if used.size else -1
         row_adapter = np.repeat(a, n)
         row_request = np.repeat(np.arange(n.size), n)
-        tiles, slots, chunks, addend_rows = self._plan(row_adapter)
+        tiles, slots, chunks, addend_rows = self._plan(row_adapter, self.lengths, self.adapters)
         parts = [row_adapter, row_request, tiles.reshape(-1), slots.reshape(-1), chunks.reshape(-1)]
         offsets = np.cumsum([0] + [-(-p.size // 4) * 4 for p in parts])      # 16-byte aligned tables in one buffer
         packed = np.zeros(max(int(offsets[-1]), 4), dtype=np.int32)
@@ -65,34 +65,41 @@ class RequestRows:
         self.workspace_bytes: dict = {}      # sizes the library asks for, by layer shape
 
     @staticmethod
-    def _plan(row_adapter: np.ndarray):
+    def _plan(row_adapter: np.ndarray, lengths: Sequence[int], adapters: Sequence[int]):
         """tiles [n, 4], slots [n, 12], chunks [n, 4] and the rows of the addend, as i8f_request_rows describes them."""
         rows = row_adapter.size
         n_tiles = -(-rows // TILE_ROWS)
-        tile_of = np.arange(rows) // TILE_ROWS
-        # one slot per (tile, adapter), in that order, with a bit for each of its rows
-        with_adapter = np.flatnonzero(row_adapter >= 0)
-        key = (tile_of[with_adapter] << 20) | row_adapter[with_adapter]
-        keys, slot_of = np.unique(key, return_inverse=True)
-        slot_tile, slot_adapter = keys >> 20, keys & ((1 << 20) - 1)
-        per_tile = np.bincount(slot_tile, minlength=n_tiles)
-        dense = (per_tile <= TILE_SLOTS) if rows >= DENSE_ROWS else np.zeros(n_tiles, dtype=bool)
-        keep = dense[slot_tile]
-        bits = np.zeros((keys.size, TILE_ROWS), dtype=bool)
-        bits[slot_of, with_adapter % TILE_ROWS] = True
-        slots = np.zeros((int(keep.sum()), 12), dtype=np.int32)
-        slots[:, 0] = slot_adapter[keep]
-        slots[:, 4:] = np.packbits(bits[keep], axis=1, bitorder="little").view(np.int32)
+        dense = np.zeros(n_tiles, dtype=bool)
         tiles = np.zeros((n_tiles, 4), dtype=np.int64)
-        tiles[:, 1] = np.where(dense, per_tile, 0)
-        tiles[:, 0] = np.cumsum(tiles[:, 1]) - tiles[:, 1]
+        slots = np.zeros((0, 12), dtype=np.int32)
+        if rows >= DENSE_ROWS:
+            # per tile and adapter the rows that use it, as the bits of an integer
+            masks: list[dict] = [{} for _ in range(n_tiles)]
+            first = 0
+            for n, a in zip(lengths, adapters):
+                last = first + n
+                if a >= 0:
+                    for i in range(first // TILE_ROWS, -(-last // TILE_ROWS) if n else 0):
+                        lo, hi = max(first - i * TILE_ROWS, 0), min(last - i * TILE_ROWS, TILE_ROWS)
+                        masks[i][a] = masks[i].get(a, 0) | (((1 << (hi - lo)) - 1) << lo)
+                first = last
+            per_tile = np.array([len(m) for m in masks])
+            dense = per_tile <= TILE_SLOTS
+            table = [(a, mask) for m, d in zip(masks, dense) if d for a, mask in m.items()]
+            slots = np.zeros((len(table), 12), dtype=np.int32)
+            if table:
+                slots[:, 0] = [a for a, _ in table]
+                slots[:, 4:] = np.frombuffer(b"".join(mask.to_bytes(TILE_ROWS // 8, "little") for _, mask in table), dtype="<i4").reshape(-1, 8)
+            tiles[:, 1] = np.where(dense, per_tile, 0)
+            tiles[:, 0] = np.cumsum(tiles[:, 1]) - tiles[:, 1]
         tiles[:, 2] = np.where(dense, -1, (np.cumsum(~dense) - 1) * TILE_ROWS)
         last = max(0, n_tiles * TILE_ROWS - rows) if n_tiles and not dense[-1] else 0
         addend_rows = int((~dense).sum()) * TILE_ROWS - last
-        # runs of rows with one adapter in the chunked tiles, cut into pieces of CHUNK_ROWS
-        left = np.flatnonzero(~dense[tile_of]) if rows else np.zeros(0, dtype=np.int64)
-        if left.size == 0:
+        if dense.all():
             return tiles, slots, np.zeros((0, 4), dtype=np.int64), addend_rows
+        tile_of = np.arange(rows) // TILE_ROWS
+        # runs of rows with one adapter in the chunked tiles, cut into pieces of CHUNK_ROWS
+        left = np.flatnonzero(~dense[tile_of])
         cut = (np.diff(left) != 1) | (np.diff(row_adapter[left]) != 0) | (np.diff(tile_of[left]) != 0)
         starts = np.concatenate([[0], np.flatnonzero(cut) + 1])
         ends = np.concatenate([starts[1:], [left.size]])
