@@ -126,7 +126,7 @@ struct Cfg {
     static constexpr int kThreads = 64 + 32 * (kEpiWarps + kLowWarps);
     static constexpr int kLowPitch = BN + 4;   // floats; rows four banks apart: the epilogue's row-per-thread reads do not collide
     static constexpr int kLowBytes = EXTRA == kExtraRows ? kBM * kLowPitch * 4 : 0;
-    static constexpr int kRingBudget = (kEpiWarps == 8 ? 160 : EXTRA == kExtraRows ? 128 : 192) * 1024;   // eight warps need more staging space
+    static constexpr int kRingBudget = (kEpiWarps == 8 ? 160 : EXTRA == kExtraRows ? (BN > 64 ? 128 : 168) : 192) * 1024;   // eight warps need more staging space
     static constexpr int kStages = kRingBudget / kStageBytes > 8 ? 8 : kRingBudget / kStageBytes;
     // TMEM: two int32/fp32 accumulator buffers at columns 0 and BN, so the epilogue of a tile overlaps the MMAs of the
     // next; with LORA one more fp32 accumulator behind them.  The LoRA accumulator needs no double buffering: it is

@@ -37,8 +37,8 @@ __device__ __forceinline__ void store_dt(void* out, int64_t idx, float v) {
 // and of the RB rows of A, 256 threads side by side, so a CTA's share of A is in flight at once.  Bound by the bytes of A and,
 // for few chunks, by one trip to memory; x is read again by the other rank rows' CTAs from L2.  A chunk without an
 // adapter gets zeros.
-// QUANT: the CTAs of the first rank rows also turn the chunk's rows into int8 (the arithmetic of i8f_quant_rowwise: step =
-// max(absmax / 127, 1e-30), rint(x * (1 / step))), which saves a small batch a launch of its own for that.
+// QUANT: the CTAs of a chunk also turn its rows into int8, dealt out over the rank rows (the arithmetic of i8f_quant_rowwise:
+// step = max(absmax / 127, 1e-30), rint(x * (1 / step))), which saves a small batch a launch of its own for that.
 constexpr int kChunkThreads = 256;
 constexpr int kChunkWarps = kChunkThreads / 32;
 
@@ -54,7 +54,7 @@ down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restri
                    const int4* __restrict__ chunks, void* __restrict__ t, int64_t ldt, const QuantOut out, int wait_first) {
     constexpr int kValues = RB * kChunkRows;
     __shared__ float s_part[kChunkWarps][kValues];
-    __shared__ uint32_t s_max[kChunkWarps][kChunkRows];
+    __shared__ uint32_t s_max[kChunkWarps];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -62,6 +62,41 @@ down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restri
     const int j0 = blockIdx.y * RB;
     const int nvec = K >> 3;
     const uint16_t* const x0 = static_cast<const uint16_t*>(x) + c.x * ldx;
+    if constexpr (QUANT) {
+        for (int m = blockIdx.y; m < c.y; m += gridDim.y) {
+            const uint4* const xr = reinterpret_cast<const uint4*>(x0 + m * ldx);
+            // 16-bit patterns without their sign order like the values
+            uint32_t m2 = 0u;
+#pragma unroll 2
+            for (int v = threadIdx.x; v < nvec; v += kChunkThreads) {
+                const uint4 w = __ldg(xr + v);
+                m2 = __vmaxu2(__vmaxu2(__vmaxu2(m2, w.x & 0x7FFF7FFFu), __vmaxu2(w.y & 0x7FFF7FFFu, w.z & 0x7FFF7FFFu)), w.w & 0x7FFF7FFFu);
+            }
+            uint32_t big = __reduce_max_sync(0xFFFFFFFFu, max(m2 & 0xFFFFu, m2 >> 16));
+            if (lane == 0) s_max[warp] = big;
+            __syncthreads();
+            big = s_max[0];
+#pragma unroll
+            for (int w = 1; w < kChunkWarps; ++w) big = max(big, s_max[w]);
+            __syncthreads();      // before the next row's
+            const float amax = DT == I8F_BF16 ? __uint_as_float(big << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(big)));
+            const float step = fmaxf(__fdiv_rn(amax, 127.0f), 1e-30f);
+            const float inv = __fdiv_rn(1.0f, step);
+            const int64_t row = static_cast<int64_t>(c.x) + m;
+            if (threadIdx.x == 0) out.scale[row] = step;
+            constexpr float kMagic = 12582912.0f;      // 1.5 * 2^23
+#pragma unroll 2
+            for (int v = threadIdx.x; v < nvec; v += kChunkThreads) {
+                float f[8];
+                uint32_t u[8];
+                widen8<DT == I8F_BF16>(__ldg(xr + v), f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__fadd_rn(__fmul_rn(f[e], inv), kMagic)) & 0xFFu;
+                *reinterpret_cast<uint2*>(out.q + row * out.ldq + v * 8) =
+                    make_uint2(u[0] | (u[1] << 8) | (u[2] << 16) | (u[3] << 24), u[4] | (u[5] << 8) | (u[6] << 16) | (u[7] << 24));
+            }
+        }
+    }
     if (c.z >= 0) {
         float acc[RB][kChunkRows];
 #pragma unroll
@@ -104,19 +139,6 @@ down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restri
             }
         }
     }
-    const bool quant = QUANT && blockIdx.y == 0;
-    if (quant) {
-        // 16-bit patterns without their sign order like the values
-        for (int m = 0; m < c.y; ++m) {
-            uint32_t m2 = 0u;
-            for (int v = threadIdx.x; v < nvec; v += kChunkThreads) {
-                const uint4 w = __ldg(reinterpret_cast<const uint4*>(x0 + m * ldx) + v);
-                m2 = __vmaxu2(__vmaxu2(__vmaxu2(m2, w.x & 0x7FFF7FFFu), __vmaxu2(w.y & 0x7FFF7FFFu, w.z & 0x7FFF7FFFu)), w.w & 0x7FFF7FFFu);
-            }
-            const uint32_t big = __reduce_max_sync(0xFFFFFFFFu, max(m2 & 0xFFFFu, m2 >> 16));
-            if (lane == 0) s_max[warp][m] = big;
-        }
-    }
     __syncthreads();
     if (threadIdx.x < kValues) {
         const int j = threadIdx.x / kChunkRows, m = threadIdx.x % kChunkRows;
@@ -125,28 +147,6 @@ down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restri
             if (c.z >= 0)
                 for (int w = 0; w < kChunkWarps; ++w) v += s_part[w][threadIdx.x];
             store_dt<DT>(t, (static_cast<int64_t>(c.x) + m) * ldt + j0 + j, v);
-        }
-    }
-    if (quant) {
-        constexpr float kMagic = 12582912.0f;      // 1.5 * 2^23
-        for (int m = 0; m < c.y; ++m) {
-            uint32_t big = s_max[0][m];
-#pragma unroll
-            for (int w = 1; w < kChunkWarps; ++w) big = max(big, s_max[w][m]);
-            const float amax = DT == I8F_BF16 ? __uint_as_float(big << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(big)));
-            const float step = fmaxf(__fdiv_rn(amax, 127.0f), 1e-30f);
-            const float inv = __fdiv_rn(1.0f, step);
-            const int64_t row = static_cast<int64_t>(c.x) + m;
-            if (threadIdx.x == 0) out.scale[row] = step;
-            for (int v = threadIdx.x; v < nvec; v += kChunkThreads) {
-                float f[8];
-                uint32_t u[8];
-                widen8<DT == I8F_BF16>(__ldg(reinterpret_cast<const uint4*>(x0 + m * ldx) + v), f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__fadd_rn(__fmul_rn(f[e], inv), kMagic)) & 0xFFu;
-                *reinterpret_cast<uint2*>(out.q + row * out.ldq + v * 8) =
-                    make_uint2(u[0] | (u[1] << 8) | (u[2] << 16) | (u[3] << 24), u[4] | (u[5] << 8) | (u[6] << 16) | (u[7] << 24));
-            }
         }
     }
     // this kernel's completion implies that of the one it may have run beside

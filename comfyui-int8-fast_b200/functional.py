@@ -668,7 +668,7 @@ def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm,
                 row_request = rows.row_request_ptr
                 ldg, lds, ldt = ldg if many_g else 0, lds if many_s else 0, ldt if many_t else 0
             rc = nat.load().i8f_gated_residual_norm(
-                x.data_ptr(), _code(x.dtype), ldx, y.data_ptr(), _code(dtype), ldy, M, K, row_request, requests, g, ldg, 1 if gate_tanh else 0,
+                x.data_ptr(), _code(x.dtype), ldx, y.data_ptr(), _code(dtype), ldy, M, K, row_request, requests if row_request is not None else 1, g, ldg, 1 if gate_tanh else 0,
                 residual_scale, nat.NORM_CODE[post_norm], pw, nat.NORM_CODE[norm], nw, s, lds, t, ldt, eps, x_out.data_ptr(), ldo,
                 h.data_ptr() if want_h else None, K, q.data_ptr() if want_q else None, K, q_scale.data_ptr() if want_q else None,
                 nat.current_stream(device))

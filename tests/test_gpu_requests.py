@@ -95,6 +95,12 @@ LINEAR = [
     ([5, 900, 400, 1] + [1] * 30 + [1000], [0, 1, -1, 2] + [i % 3 for i in range(30)] + [1], 384, 640, 16, torch.bfloat16),
     ([2600, 0, 2008], [0, 1, 1], 256, 4104, 32, torch.float16),
     ([33, 44], [0, 0], 64, 40, 1024, torch.bfloat16),
+    # 256-wide tiles: dense and chunked ones side by side, ranks of several slabs, a batch of chunks only, the shortest rows
+    ([1] * 300 + [900], [i % 20 for i in range(300)] + [3], 256, 4096, 24, torch.bfloat16),
+    ([300, 5, 295], [1, -1, 0], 192, 4104, 264, torch.float16),
+    ([100, 60, 40], [0, -1, 1], 64, 24576, 16, torch.bfloat16),
+    ([2000, 1, 559], [0, 1, 0], 16, 2049, 8, torch.bfloat16),
+    ([256], [0], 4224, 64, 128, torch.bfloat16),
 ]
 
 
@@ -130,11 +136,12 @@ def test_linear_lora_requests(cuda_pkg, case, per_channel, bias):
     check(y2, want, off + mag + u * (want.abs() + off + mag) + 4 * TINY[dtype])
 
 
-def test_rows_without_adapter_are_the_plain_linear(cuda_pkg):
+@pytest.mark.parametrize("lengths,N", [([40, 600, 1, 7], 768), ([40, 900, 300, 7], 4096), ([3, 20, 1, 7], 520)])
+def test_rows_without_adapter_are_the_plain_linear(cuda_pkg, lengths, N):
     F, nat = cuda_pkg.functional, cuda_pkg._native
-    lengths, adapters = [40, 600, 1, 7], [-1, 0, -1, 1]
+    adapters = [-1, 0, -1, 1]
     rows = cuda_pkg.adapters.RequestRows(lengths, adapters, DEV)
-    w, ws, b, la, lb = layer(512, 768, 16, 2, torch.bfloat16, 7)
+    w, ws, b, la, lb = layer(512, N, 16, 2, torch.bfloat16, 7)
     x = torch.randn(rows.total, 512, generator=gen(8), device=DEV).bfloat16()
     none = adapter_rows(rows) < 0
     for order in (nat.EPI_SINGLE, nat.EPI_PYTORCH):
@@ -142,13 +149,14 @@ def test_rows_without_adapter_are_the_plain_linear(cuda_pkg):
         assert torch.equal(y[none], F.linear_forward(x, w, ws, b, torch.bfloat16, order=order)[none])
 
 
-@pytest.mark.parametrize("lengths", [[1, 3, 40, 300, 1, 200], [1, 3, 2, 5, 1, 4]])
-def test_nothing_leaks_between_requests(cuda_pkg, lengths):
+@pytest.mark.parametrize("lengths,N", [([1, 3, 40, 300, 1, 200], 320), ([1, 3, 2, 5, 1, 4], 320), ([1, 300, 40, 600, 1, 400], 4096),
+                                       ([1, 3, 40, 3, 1, 20], 320)])
+def test_nothing_leaks_between_requests(cuda_pkg, lengths, N):
     """An adapter of infinities and NaN, and non-finite activations, reach the rows of their own request only."""
     F = cuda_pkg.functional
     adapters = [0, 1, -1, 2, 0, 1]
     rows = cuda_pkg.adapters.RequestRows(lengths, adapters, DEV)
-    w, ws, b, la, lb = layer(256, 320, 16, 3, torch.bfloat16, 17)
+    w, ws, b, la, lb = layer(256, N, 16, 3, torch.bfloat16, 17)
     x = torch.randn(rows.total, 256, generator=gen(18), device=DEV).bfloat16()
     call = F.linear_small_batch_lora_requests if rows.total <= 16 else (lambda *a: F.linear_lora_requests(*a, torch.bfloat16))
     clean = call(x, w, ws, b, la, lb, rows)
@@ -440,7 +448,7 @@ def block_state(pkg, lengths, adapters, K, N, r, seed):
                 rows=pkg.adapters.RequestRows(lengths, adapters, DEV))
 
 
-BLOCKS = [([40, 1, 1, 1, 86], [0, 1, -1, 2, 1]), ([700, 1, 1, 1400], [1, 0, 2, 2])]
+BLOCKS = [([40, 1, 1, 1, 86], [0, 1, -1, 2, 1]), ([700, 1, 1, 1400], [1, 0, 2, 2]), ([1] * 40 + [1500], [i % 9 for i in range(40)] + [8])]
 
 
 @pytest.mark.parametrize("lengths,adapters", BLOCKS)
