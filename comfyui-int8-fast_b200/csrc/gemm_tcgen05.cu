@@ -89,7 +89,7 @@ struct GemmParams {
     const RequestSlot* req_slots;
     int lora_k16;       // 16-element steps of the rank
     long long lora_n;   // rows of lora_b per adapter
-    // kExtraRows: eight more warps work the low-rank term of the tile's rows out (low_rank.cuh) while the MMAs run
+    // kExtraRows: six more warps work the low-rank term of the tile's rows out (low_rank.cuh) while the MMAs run
     const uint16_t* row_t;
     long long ld_row_t;
     const uint16_t* row_b;
@@ -122,7 +122,7 @@ struct Cfg {
     // Epilogue warps: four (one per 32-lane quarter of tensor memory) or, where the epilogue cannot hide under the
     // next tile's MMAs (single accumulator buffer, below), eight: two per quarter, each taking half of the columns.
     static constexpr int kEpiWarps = ((LORA && 3 * BN > 512) || EXTRA == kExtraFold) ? 8 : 4;
-    static constexpr int kLowWarps = EXTRA == kExtraRows ? 8 : 0;
+    static constexpr int kLowWarps = EXTRA == kExtraRows ? 6 : 0;      // twelve warps in all: 168 registers each, no spills
     static constexpr int kThreads = 64 + 32 * (kEpiWarps + kLowWarps);
     static constexpr int kLowPitch = BN + 4;   // floats; rows four banks apart: the epilogue's row-per-thread reads do not collide
     static constexpr int kLowBytes = EXTRA == kExtraRows ? kBM * kLowPitch * 4 : 0;
@@ -790,19 +790,19 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 // eight rows of one adapter share a pass over its rows of lora_b, else four do, else they are taken four at a time
                 // with an adapter each
                 const int first = warp - 2 - C::kEpiWarps;
-                constexpr int kOctets = kBM / 8 / C::kLowWarps;      // of this warp
+                constexpr int kOctets = (kBM / 8 + C::kLowWarps - 1) / C::kLowWarps;      // of this warp
                 int ids = -1;
                 {
                     const int m = m_blk * kBM + (first + (lane >> 3) * C::kLowWarps) * 8 + (lane & 7);
-                    if (lane < 8 * kOctets && m < p.M) ids = __ldg(p.row_adapter + m);
+                    if (lane < 8 * kOctets && first + (lane >> 3) * C::kLowWarps < kBM / 8 && m < p.M) ids = __ldg(p.row_adapter + m);
                 }
                 auto rows_of = [&](int a) { return a >= 0 ? p.row_b + (a * p.lora_n + n_blk * BN) * p.row_r : nullptr; };
 #pragma unroll 1
-                for (int i = 0; i < 2 * kOctets; ++i) {      // halves of octets
+                for (int i = __any_sync(0xFFFFFFFFu, ids >= 0) ? 0 : 2 * kOctets; i < 2 * kOctets; ++i) {      // halves of octets
                     const int octet = first + (i >> 1) * C::kLowWarps, at = 8 * (i >> 1) + 4 * (i & 1);
                     const int row = octet * 8 + 4 * (i & 1);
                     const int m0 = m_blk * kBM + row;
-                    if (m0 >= p.M) break;
+                    if (row >= kBM || m0 >= p.M) break;
                     int a[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) a[j] = __shfl_sync(0xFFFFFFFFu, ids, at + j);
