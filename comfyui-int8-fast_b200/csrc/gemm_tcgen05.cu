@@ -19,6 +19,15 @@
 // epilogue short.  16-bit outputs are computed as packed pairs and leave
 // through shared memory and TMA stores.
 //
+// A batch whose rows belong to several requests, each with a low-rank adapter of
+// its own, adds t[m] @ B_a(m)^T.  On 256-wide tiles (kExtraFold) the epilogue
+// warps scale the int32 accumulator to fp32 in place and the MMAs of the tile's
+// adapters, each under a mask of the rows that use it, accumulate onto it while
+// the next tile's product runs (683 us at 18432 x 4096 -> 12288 with four
+// adapters = 2.75 POPS; with a third accumulator for the term, the form that the
+// reference's separate roundings need, kExtraRequests, 749 us).  On narrower
+// tiles (kExtraRows) six more warps work the rows' terms out beside the MMAs.
+//
 // PAIR variant (cta_group::2): two CTAs of a cluster work on one 256 x BN
 // tile.  Each loads its own 128 rows of A and its own BN/2 rows of B (half the
 // shared-memory fill bandwidth per SM for the same MMA work), the even CTA

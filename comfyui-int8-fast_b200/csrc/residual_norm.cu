@@ -11,6 +11,10 @@
 // r = 1 / sqrt(...) is the device's rsqrtf (two units in the last place).  Everything between the loads and the stores is
 // fp32: h and its int8 form come from the unrounded x', so each output is
 // rounded once.  Row sums are per-thread sums, a shuffle tree, then the warps in order: the same order every time.
+//
+// Bound by the bytes of x, y, x' and h.  Measured, inputs from HBM: 4608 x 4096 bf16 36.6 us = 4.1 TB/s (63 % of the copy rate;
+// some 8 us of it pass before the first rows leave, the rest streams at 6.7 TB/s), 18432 x 4096 with an fp32 residual
+// 157 us = 5.8 TB/s (88 %), 777 rows of 2305 in 11 requests 17.9 us, one row 4.4 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
