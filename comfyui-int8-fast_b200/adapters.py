@@ -129,6 +129,11 @@ class RequestLoras:
         self._plans = {} if plans is None else plans
         self._converted = None
 
+    @property
+    def samples(self) -> int | None:
+        """Samples of the model's current batch, where the model's hook has left word."""
+        return self._plans.get("samples")
+
     def bank(self, device: torch.device, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
         """The bank in the compute type on the compute device, converted once."""
         if self._converted is None or self._converted[0].device != device or self._converted[0].dtype != dtype:

@@ -87,9 +87,9 @@ def _wscale_arg(w_scale, device: torch.device, n_rows: int) -> tuple[Tensor, int
     return (ws if ws.is_contiguous() else ws.contiguous()), nat.WSCALE_CHANNEL   # [N] and [N,1] share their memory layout
 
 
-def _check_weight(w: Tensor, K: int) -> None:
-    if w.dtype != torch.int8 or w.shape[1] != K:
-        raise ValueError(f"weight must be int8 [N, {K}], got {w.dtype} {tuple(w.shape)}")
+def _check_weight(w: Tensor, K: int, device: torch.device | None = None) -> None:
+    if w.dtype != torch.int8 or w.shape[1] != K or (device is not None and w.device != device):
+        raise ValueError(f"weight must be int8 [N, {K}]{'' if device is None else f' on {device}'}, got {w.dtype} {tuple(w.shape)} on {w.device}")
 
 
 def quantize_rowwise(x: Tensor, hadamard: bool = False, return_rotated: bool = False):
@@ -484,7 +484,7 @@ def linear_w8a8_lora_requests(q: Tensor, q_scale: Tensor, w: Tensor, w_scale, bi
         q, w, t = _rows(q), _rows(w), _rows(t)
         M, K = q.shape
         N = w.shape[0]
-        _check_weight(w, K)
+        _check_weight(w, K, q.device)
         n, r = _check_requests(rows, q, None, lora_b, out_dtype, K, N)
         if t.shape != (M, r) or t.dtype != out_dtype or t.device != q.device:
             raise ValueError(f"t must be [{M}, {r}] in {out_dtype} on {q.device}")
@@ -526,7 +526,7 @@ def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lor
         N = w.shape[0]
         if out_dtype != x.dtype:
             raise ValueError(f"out_dtype must be the activations' type {x.dtype}, which the adapters share")
-        _check_weight(w, K)
+        _check_weight(w, K, device)
         n, r = _check_requests(rows, x, lora_a, lora_b, out_dtype, K, N)
         ws, mode = _wscale_arg(w_scale, device, N)
         bias = _bias_arg(bias, device, N)
@@ -561,7 +561,7 @@ def linear_small_batch_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor
         w, ldw = _pitched(w)
         M, K = x.shape
         N = w.shape[0]
-        _check_weight(w, K)
+        _check_weight(w, K, device)
         n, r = _check_requests(rows, x, lora_a, lora_b, x.dtype, K, N)
         ws, mode = _wscale_arg(w_scale, device, N)
         bias = _bias_arg(bias, device, N)

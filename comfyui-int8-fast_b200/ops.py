@@ -313,6 +313,8 @@ class DynamicLoRAHook:
 
     def __init__(self):
         self.current_lora_id = None
+        self._held = None       # what current_lora_id names by id(): kept alive, so that no new object can have such an id
+        self._plans: dict = {}
 
     def pre_forward(self, module, input_args, input_kwargs):
         opts = input_kwargs.get("transformer_options", {})
@@ -329,6 +331,11 @@ class DynamicLoRAHook:
             else:
                 self.apply_composition(module, loras)
             self.current_lora_id = lora_id
+            self._held = [d["patches"] for r in ([loras] + list(requests)) for d in r]
+        if requests:
+            # the samples of this call's batch: a layer that gets one row per sample, or all rows flattened, goes by it
+            x = input_args[0] if input_args else None
+            self._plans["samples"] = x.shape[0] if isinstance(x, Tensor) and x.dim() > 0 else None
         return None
 
     @staticmethod
@@ -353,7 +360,7 @@ class DynamicLoRAHook:
             key = tuple((id(d["patches"]), d["strength"]) for d in stack)
             entries.append(compositions.setdefault(key, (len(compositions), stack))[0] if stack else -1)
         stacks = [stack for _, stack in compositions.values()]
-        plans: dict = {}
+        plans = self._plans = {}
         for name, module in diffusion_model.named_modules():
             if not hasattr(module, "lora_A"):
                 continue
@@ -439,9 +446,16 @@ def _prepare_lora(module, device: torch.device, dtype: torch.dtype):
 
 
 @torch.compiler.disable
-def _request_forward(loras, x: Tensor, samples: int, weight: Tensor, w_scale, bias: Tensor | None, dtype: torch.dtype, hadamard: bool,
+def _request_forward(loras, x: Tensor, samples: int | None, weight: Tensor, w_scale, bias: Tensor | None, dtype: torch.dtype, hadamard: bool,
                      rotated_lora_input: bool) -> Tensor:
-    """The Linear's forward for a batch with one adapter per request.  x [rows, K]: `samples` equal runs of rows."""
+    """The Linear's forward for a batch with one adapter per request.  x [rows, K] holds equal runs of rows, one per sample of the
+    batch: as many as the model's batch has where the hook has said so, else `samples` (the first of three or more
+    dimensions), else one per request."""
+    known = loras.samples
+    if known and x.shape[0] % known == 0 and known % len(loras.entries) == 0:
+        samples = known
+    elif samples is None:
+        samples = len(loras.entries)
     if x.shape[0] % samples:
         raise ValueError(f"{x.shape[0]} rows are not {samples} samples of equal length")
     plan = loras.rows(samples, x.shape[0] // samples, x.device)
@@ -619,8 +633,7 @@ def _define_ops(manual_cast, cast_bias_weight, uncast_bias_weight):
                 has_lora = self.lora_A is not None and self.lora_B is not None
 
                 if self.request_loras is not None:
-                    samples = x.shape[0] if x.dim() > 2 else len(self.request_loras.entries)
-                    y = _request_forward(self.request_loras, x2, samples, weight, w_scale, bias, compute_dtype, self._use_quarot,
+                    y = _request_forward(self.request_loras, x2, x.shape[0] if x.dim() > 2 else None, weight, w_scale, bias, compute_dtype, self._use_quarot,
                                          Int8TensorwiseOps.lora_uses_rotated_input)
                 elif rows > SMALL_BATCH_ROWS and has_lora:
                     # t = x @ A^T first; t @ B^T is accumulated inside the int8 GEMM kernel and added in its

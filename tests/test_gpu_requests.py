@@ -226,7 +226,7 @@ def test_adapter_calls_refuse(cuda_pkg):
     for bad in (dict(x=x[:23]), dict(rows=Rows([20, 3], [0, 1], DEV)), dict(rows=Rows([20, 4], [0, 2], DEV)), dict(rows=Rows([24], [0], "cpu")),
                 dict(out_dtype=torch.float16), dict(x=x.half(), out_dtype=torch.float16), dict(lora_a=la[:1]), dict(lora_a=la.half()),
                 dict(lora_b=lb[:, :63]), dict(lora_b=lb.transpose(1, 2)), dict(lora_a=la[:, :, ::2]), dict(lora_a=la[0]),
-                dict(lora_b=lb.cpu()), dict(bias=b[:5]), dict(w_scale=ws[:5])):
+                dict(lora_b=lb.cpu()), dict(bias=b[:5]), dict(w_scale=ws[:5]), dict(w=w.cpu()), dict(w=w[:, :64])):
         with pytest.raises((ValueError, E)):
             F.linear_lora_requests(**{**ok, **bad})
     odd = layer(128, 64, 12, 2, torch.bfloat16, 3)
@@ -588,9 +588,11 @@ def test_linear_module_with_request_loras(cuda_pkg, tokens, quarot):
         check(y[j], want, off + u * (want.abs() + off))
     with pytest.raises(ValueError):
         lin(x[:6])
-    flat = cuda_pkg.adapters.RequestLoras(la, lb, [1, -1, 2, 1] * 2)
-    lin.request_loras = flat
+    lin.request_loras = cuda_pkg.adapters.RequestLoras(la, lb, [1, -1, 2, 1] * 2)
     assert torch.equal(lin(x.reshape(-1, K)).reshape(y.shape), y)      # two dimensions: as many runs of rows as requests
+    lin.request_loras = cuda_pkg.adapters.RequestLoras(la, lb, [1, -1, 2, 1], {"samples": 8})
+    assert torch.equal(lin(x.reshape(-1, K)).reshape(y.shape), y)      # or as the model's batch has samples
+    assert torch.equal(lin(x.reshape(1, -1, K)).reshape(y.shape), y)
 
 
 def test_dit_batch_of_samples_fused(cuda_pkg):

@@ -241,6 +241,11 @@ def test_hook_gives_each_request_its_composition(pkg):
     assert plan.lengths == (5,) * 8 and plan.adapters == model["a"].request_loras.entries * 2
     with pytest.raises(ValueError):
         model["a"].request_loras.rows(6, 5, torch.device("cpu"))
+    # the batch of the call tells the layers how many samples they see
+    hook.pre_forward(model, (torch.zeros(8, 3),), {"transformer_options": {**opts, "dynamic_loras": [shared]}})
+    assert model["a"].request_loras.samples == model["b"].request_loras.samples == 8
+    # the patches are held for as long as the hook goes by their ids
+    assert [id(p) for p in hook._held] == [id(d["patches"]) for d in (shared, one, one, two, one)]
     # back to one composition for all, then to none
     hook.pre_forward(model, (), {"transformer_options": {"dynamic_loras": [one]}})
     assert model["a"].request_loras is None and model["a"].lora_A.shape == (3, 32)
