@@ -180,6 +180,11 @@ def ptr(t: torch.Tensor | None) -> c_void_p:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def stream_handle(device: torch.device) -> int:
+    """current_stream() of a device with an index, as a plain integer."""
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def current_stream(device: torch.device) -> c_void_p:
     """The current CUDA stream of `device` as a raw handle (the library enqueues on it and nowhere else)."""
     if _raw_stream is not None:   # no Stream object is built: this call sits in front of every kernel launch

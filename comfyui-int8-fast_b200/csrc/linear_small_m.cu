@@ -19,6 +19,7 @@
 
 #include "host_common.h"
 #include "low_rank.cuh"
+#include "tensor_maps.h"
 
 namespace i8f {
 namespace {
@@ -340,9 +341,7 @@ template <int DT, bool HI, bool REQ, int FB>
 int launch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, int per_row,
                    const void* bias, int bias_dt, void* out, int64_t ldo, int M, int64_t N, int64_t K,
                    cudaStream_t stream, const SmallTerm& req) {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int sms = sm_count();
     const int64_t blocks = (N + 16 * FB - 1) / (16 * FB);
     auto kernel = small_m_kernel<DT, HI, 2, REQ, FB>;
     // persistent: as many CTAs as are resident at once, each walking feature blocks with a grid stride
@@ -382,9 +381,7 @@ int dispatch_small(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, con
     if constexpr (REQ) {
         // two groups where that saves a round of CTAs (three of one group are resident on an SM, two of two): 16 rows, K 4096,
         // rank 32, N 8192 22.7 -> 15.2 us; at N 4096 (one round either way) 13.3 against 14.3, at 12288 (two) 23.3 against 25.5
-        int dev = 0, sms = 148;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        const int sms = sm_count();
         const int64_t rounds1 = ((N + 15) / 16 + 3 * sms - 1) / (3 * sms), rounds2 = ((N + 31) / 32 + 2 * sms - 1) / (2 * sms);
         if (M > 8 && rounds2 < rounds1)
             return launch_small<DT, true, REQ, 2>(x, ldx, w, ldw, w_scale, per_row, bias, bias_dt, out, ldo, M, N, K, stream, req);

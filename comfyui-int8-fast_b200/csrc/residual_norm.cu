@@ -21,6 +21,7 @@
 #include "f32x2.cuh"
 #include "host_common.h"
 #include "ptx_sm100.cuh"
+#include "tensor_maps.h"
 
 namespace i8f {
 namespace {
@@ -736,8 +737,13 @@ int launch_ring(const NormArgs& a, int min_slots, int sms, cudaStream_t st, bool
     if (!*done) return I8F_OK;
     const int n_slots = room < kMaxSlots ? room : kMaxSlots;
     auto kern = gated_residual_norm_ring_kernel<XDT, YDT, GT, VPT, SHIFT>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
-    if (e != cudaSuccess) return fail(I8F_ERR_CUDA, "cudaFuncSetAttribute(smem=%d): %s", kRingSmem, cudaGetErrorString(e));
+    static bool attr_done[64] = {false};
+    const int dev = current_device();
+    if (!attr_done[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
+        if (e != cudaSuccess) return fail(I8F_ERR_CUDA, "cudaFuncSetAttribute(smem=%d): %s", kRingSmem, cudaGetErrorString(e));
+        attr_done[dev] = true;
+    }
     int* status = device_status_word();
     I8F_REQUIRE(status != nullptr, I8F_ERR_CUDA, "device status word unavailable");
     const int64_t grid = a.M < sms ? a.M : sms;
@@ -768,9 +774,7 @@ int launch_ring_for(const NormArgs& a, int sms, cudaStream_t st, bool* done) {
 
 template <int XDT, int YDT>
 int launch_norm(const NormArgs& a, int64_t requests, bool vec8, bool alike, cudaStream_t st) {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int sms = sm_count();
     const unsigned grid = static_cast<unsigned>(a.M), grid8 = static_cast<unsigned>((a.M + 7) / 8);
     // Which kernel (us at K columns, bf16, measured): fewer than 256 rows one CTA each (64 rows of 4096: 4.2, in the ring 6.1;
     // 512 rows: 10.7 and 7.5).  Rows of up to 512 columns a warp each (4608 rows of 512: 8.4, in the ring 14.4; of 1024: 19.0

@@ -1,5 +1,5 @@
 // Tensor maps of K-major operands, shared by the kernels that stage them by TMA (defined in gemm_tcgen05.cu, which keeps a
-// small cache of encoded maps).
+// small cache of encoded maps), and the current device with its SM count (asked for once).
 #pragma once
 #include <cstdint>
 #include <cuda.h>

@@ -545,7 +545,7 @@ def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lor
                                               ws.data_ptr(), mode, bias.data_ptr() if bias is not None else None,
                                               _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(), lora_b.data_ptr(), n, r,
                                               rows.native_ptr, out.data_ptr(), N, M, N, K, order, workspace.data_ptr(), need,
-                                              nat.current_stream(device))
+                                              nat.stream_handle(device))
             if rc:
                 nat.check(rc, "i8f_linear_lora_requests")
         return out
@@ -576,7 +576,7 @@ def linear_small_batch_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor
                                                           bias.data_ptr() if bias is not None else None,
                                                           _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(),
                                                           lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(), N, M, N, K,
-                                                          workspace.data_ptr(), need, nat.current_stream(device))
+                                                          workspace.data_ptr(), need, nat.stream_handle(device))
             if rc:
                 nat.check(rc, "i8f_linear_w8a16_small_lora_requests")
         return out
@@ -650,7 +650,7 @@ def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm,
         weight, nw = _weight_vector(weight, "weight", y)
         ldo = K
         if x_out is None:
-            x_out = x.new_empty(shape)
+            x_out = torch.empty_like(x) if x.is_contiguous() else x.new_empty(shape)
         else:
             if x_out.shape != shape or x_out.dtype is not x.dtype or x_out.device != device or (K > 1 and x_out.stride(1) != 1) or (
                     M > 1 and x_out.stride(0) < K):
@@ -658,7 +658,7 @@ def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm,
             if x_out is given:
                 x = x_out
             ldo = _ld(x_out)
-        h = y.new_empty(shape) if want_h else None
+        h = None if not want_h else torch.empty_like(y) if y.is_contiguous() else y.new_empty(shape)
         q = y.new_empty(shape, dtype=torch.int8) if want_q else None
         q_scale = y.new_empty((M, 1), dtype=torch.float32) if want_q else None
         if M and K:
@@ -671,7 +671,7 @@ def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm,
                 x.data_ptr(), _code(x.dtype), ldx, y.data_ptr(), _code(dtype), ldy, M, K, row_request, requests if row_request is not None else 1, g, ldg, 1 if gate_tanh else 0,
                 residual_scale, nat.NORM_CODE[post_norm], pw, nat.NORM_CODE[norm], nw, s, lds, t, ldt, eps, x_out.data_ptr(), ldo,
                 h.data_ptr() if want_h else None, K, q.data_ptr() if want_q else None, K, q_scale.data_ptr() if want_q else None,
-                nat.current_stream(device))
+                nat.stream_handle(device))
             if rc:
                 nat.check(rc, "i8f_gated_residual_norm")
         return x_out, h, q, q_scale
