@@ -18,6 +18,7 @@ from . import _native as nat
 TILE_ROWS = 256     # rows of a tile of the projection
 TILE_SLOTS = 8      # adapters that a tile may have to be run on the tensor cores
 DENSE_ROWS = 256    # batches of fewer rows are chunked throughout
+FEW_ROWS = 8        # rows of a tile up to which an adapter's down projection is left to chunks where the tile has others
 CHUNK_ROWS = 4      # rows of one adapter that a small work item of the kernels takes together
 
 
@@ -85,21 +86,28 @@ class RequestRows:
                 first = last
             per_tile = np.array([len(m) for m in masks])
             dense = per_tile <= TILE_SLOTS
-            table = [(a, mask) for m, d in zip(masks, dense) if d for a, mask in m.items()]
+            # an MMA costs a tile the same for one row as for all: an adapter's few rows beside others are cheaper as chunks there
+            table = [(a, int(len(m) > 1 and mask.bit_count() <= FEW_ROWS), mask) for m, d in zip(masks, dense) if d for a, mask in m.items()]
             slots = np.zeros((len(table), 12), dtype=np.int32)
             if table:
-                slots[:, 0] = [a for a, _ in table]
-                slots[:, 4:] = np.frombuffer(b"".join(mask.to_bytes(TILE_ROWS // 8, "little") for _, mask in table), dtype="<i4").reshape(-1, 8)
+                slots[:, 0] = [a for a, _, _ in table]
+                slots[:, 1] = [few for _, few, _ in table]
+                slots[:, 4:] = np.frombuffer(b"".join(mask.to_bytes(TILE_ROWS // 8, "little") for _, _, mask in table), dtype="<i4").reshape(-1, 8)
             tiles[:, 1] = np.where(dense, per_tile, 0)
             tiles[:, 0] = np.cumsum(tiles[:, 1]) - tiles[:, 1]
         tiles[:, 2] = np.where(dense, -1, (np.cumsum(~dense) - 1) * TILE_ROWS)
         last = max(0, n_tiles * TILE_ROWS - rows) if n_tiles and not dense[-1] else 0
         addend_rows = int((~dense).sum()) * TILE_ROWS - last
-        if dense.all():
+        few = np.zeros((n_tiles, TILE_ROWS), dtype=bool)      # rows of dense tiles that are chunked all the same
+        if slots[:, 1].any():
+            slot_tile = np.repeat(np.arange(n_tiles), tiles[:, 1])
+            bits = np.unpackbits(np.ascontiguousarray(slots[:, 4:]).view(np.uint8), axis=1, bitorder="little").astype(bool)
+            np.logical_or.at(few, slot_tile[slots[:, 1] > 0], bits[slots[:, 1] > 0])
+        elif dense.all():
             return tiles, slots, np.zeros((0, 4), dtype=np.int64), addend_rows
         tile_of = np.arange(rows) // TILE_ROWS
-        # runs of rows with one adapter in the chunked tiles, cut into pieces of CHUNK_ROWS
-        left = np.flatnonzero(~dense[tile_of])
+        # runs of rows with one adapter among the chunked rows, cut into pieces of CHUNK_ROWS
+        left = np.flatnonzero(~dense[tile_of] | few.reshape(-1)[:rows])
         cut = (np.diff(left) != 1) | (np.diff(row_adapter[left]) != 0) | (np.diff(tile_of[left]) != 0)
         starts = np.concatenate([[0], np.flatnonzero(cut) + 1])
         ends = np.concatenate([starts[1:], [left.size]])
@@ -108,7 +116,8 @@ class RequestRows:
         first = starts[run] + CHUNK_ROWS * (np.arange(run.size) - np.repeat(np.cumsum(pieces) - pieces, pieces))
         count = np.minimum(CHUNK_ROWS, ends[run] - first)
         row = left[first]
-        return tiles, slots, np.stack([row, count, row_adapter[row], tiles[tile_of[row], 2] + row % TILE_ROWS], axis=1), addend_rows
+        addend = np.where(dense[tile_of[row]], -1, tiles[tile_of[row], 2] + row % TILE_ROWS)
+        return tiles, slots, np.stack([row, count, row_adapter[row], addend], axis=1), addend_rows
 
 
 class RequestLoras:

@@ -47,9 +47,10 @@ struct RequestTile {
     int slot_begin, n_slots, addend_row, pad;
 };
 constexpr int kMaxTileSlots = 8;      // a tile with more adapters than this is chunked
-// One adapter of a tile and the rows of the tile that use it (bit i of word j: row 32 j + i).
+// One adapter of a tile and the rows of the tile that use it (bit i of word j: row 32 j + i).  `few`: so few rows that chunks do
+// their down projection.
 struct RequestSlot {
-    int adapter, pad[3];
+    int adapter, few, pad[2];
     uint32_t rows[8];
 };
 

@@ -164,7 +164,7 @@ up_chunks_kernel(const void* __restrict__ t, int64_t ldt, const void* __restrict
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 c = chunks[blockIdx.x];      // first row, rows, adapter, first row in the addend
     const int n0 = (blockIdx.y * 4 + (threadIdx.x >> 5)) * kUpCols;
-    if (c.z < 0 || n0 >= N) return;
+    if (c.z < 0 || c.w < 0 || n0 >= N) return;
     const uint16_t* const b[1] = {static_cast<const uint16_t*>(bank_b) + (static_cast<int64_t>(c.z) * N + n0) * r};
     low_rank_rows<DT == I8F_BF16, 1, 4>(static_cast<const uint16_t*>(t) + c.x * ldt, ldt, {0}, {c.y}, b, min(kUpCols, N - n0), r,
                                         addend + static_cast<int64_t>(c.w) * ld_addend + n0, ld_addend, threadIdx.x & 31);
@@ -228,6 +228,7 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     // the block's adapters and the complement of their rows (what their MMAs leave alone)
     __shared__ int s_adapter[kMaxTileSlots];
     __shared__ uint32_t s_off[kMaxTileSlots][4];
+    __shared__ uint32_t s_rows[4];      // the rows that the block works out; those of its other adapters are left to the chunks
     if (warp == 2) {
         bool mine = false;
         int adapter = 0;
@@ -240,6 +241,12 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                 off[i] = ~slot.rows[4 * half + i];
                 mine |= off[i] != 0xFFFFFFFFu;
             }
+            mine = mine && slot.few == 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t all = __reduce_or_sync(0xFFFFFFFFu, mine ? ~off[i] : 0u);
+            if (lane == 0) s_rows[i] = all;
         }
         const uint32_t with_rows = __ballot_sync(0xFFFFFFFFu, mine);
         if (mine) {
@@ -372,8 +379,11 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
             const int rl = i & (share - 1), c = i / share * 8;
             const int64_t m = static_cast<int64_t>(block) * kDownRows + rank * share + rl;
             if (m >= p.M) continue;
+            const int rb = rank * share + rl;      // row of the block
+            const bool here = (s_rows[rb >> 5] >> (rb & 31)) & 1u;
+            if (!here && p.row_adapter[m] >= 0) continue;      // a chunk's row
             float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (p.row_adapter[m] >= 0) {
+            if (here) {
                 for (int src = 0; src < p.split; ++src) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] += part[(src * p.bn + c + j) * share + rl];
@@ -383,7 +393,8 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                 make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
         }
     } else if (warp >= 2) {
-        const bool use = row < p.M && p.row_adapter[row] >= 0;
+        const bool use = (s_rows[quarter] >> lane) & 1u;
+        const bool write = row < p.M && (use || p.row_adapter[row] < 0);
         for (int c = 0; c < cols; c += 16) {
             uint32_t v[16];
             tmem_ld_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, v);
@@ -393,7 +404,7 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
             for (int j = 0; j < 8; ++j) {
                 o[j] = pack(use ? __uint_as_float(v[2 * j]) : 0.f, use ? __uint_as_float(v[2 * j + 1]) : 0.f);
             }
-            if (row < p.M) {      // cols is a multiple of 8
+            if (write) {      // cols is a multiple of 8
                 uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.t) + row * p.ldt + n0 + c);
                 dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
                 if (c + 8 < cols) dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
@@ -411,9 +422,10 @@ down_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     }
 }
 
-// Whether the batch has tiles for the tensor cores / chunks for the warps.
+// Whether the batch has tiles for the tensor cores / chunks for the warps / chunks whose up projection is theirs, too.
 bool has_dense(const i8f_request_rows* rows) { return rows->n_dense > 0; }
 bool has_chunks(const i8f_request_rows* rows) { return rows->n_chunks > 0; }
+bool has_addend(const i8f_request_rows* rows) { return rows->addend_rows > 0; }
 
 int check_rows(const i8f_request_rows* rows, int64_t M) {
     I8F_REQUIRE(rows != nullptr, I8F_ERR_INVALID_ARG, "rows is NULL");
@@ -422,7 +434,7 @@ int check_rows(const i8f_request_rows* rows, int64_t M) {
     I8F_REQUIRE(M == 0 || (rows->row_adapter != nullptr && rows->n_dense >= 0 && rows->n_chunks >= 0 && rows->n_dense + rows->n_chunks > 0 &&
                            (rows->n_chunks == 0 || rows->chunks != nullptr) &&
                            (rows->n_dense == 0 || (rows->tiles != nullptr && rows->slots != nullptr)) &&
-                           rows->addend_rows >= 0 && (rows->n_chunks == 0 || rows->addend_rows > 0)),
+                           rows->addend_rows >= 0 && (rows->n_dense > 0 || rows->addend_rows > 0)),
                 I8F_ERR_INVALID_ARG, "incomplete row plan");
     return I8F_OK;
 }
@@ -643,7 +655,7 @@ int i8f_linear_w8a8_lora_requests(const int8_t* a, int64_t lda, const float* a_s
     float* addend = static_cast<float*>(workspace);
     const RequestTerm term = request_term(t, ldt, bank_b, adapters, r, rows, N, addend);
     for (const bool check_only : {true, false}) {     // everything is checked before anything is launched
-        if (!check_only && has_chunks(rows) && requests_need_addend(M, N, K)) {
+        if (!check_only && has_addend(rows) && requests_need_addend(M, N, K)) {
             rc = launch_up_chunks(t, ldt, bank_b, r, rows, out_dtype, N, addend, st);
             if (rc != I8F_OK) return rc;
         }
@@ -714,7 +726,7 @@ int i8f_linear_lora_requests(const void* x, int x_dtype, int64_t ldx, int hadama
         rc = launch_down(lora_in, ldx, bank_a, adapters, r, rows, t, r, x_dtype, M, K, !keep_rotated, st);
     }
     if (rc != I8F_OK) return rc;
-    if (has_chunks(rows) && requests_need_addend(M, N, K)) {
+    if (has_addend(rows) && requests_need_addend(M, N, K)) {
         rc = launch_up_chunks(t, r, bank_b, r, rows, x_dtype, N, addend, st);
         if (rc != I8F_OK) return rc;
     }

@@ -310,9 +310,10 @@ typedef struct i8f_request_rows {
      * -1) has one slot for each adapter in it, at most 8; a chunked one none, its rows start at `addend row` of the fp32
      * addend and are covered by chunks. */
     const int32_t* tiles;
-    const int32_t* slots;       /* [][12]: adapter, 0, 0, 0, then 256 bits: the rows of the tile that use it */
+    const int32_t* slots;       /* [][12]: adapter, 1 if chunks do its down projection (else 0), 0, 0, then 256 bits: the rows of
+                                   the tile that use it */
     const int32_t* chunks;      /* [n_chunks][4]: first row, row count (1..4), adapter or -1, addend row; every row of a chunked
-                                   tile is in one chunk */
+                                   tile is in one chunk, as is every row of a dense tile's slot that says so (addend row -1) */
     int64_t n_dense;            /* dense tiles; 0 for a batch of at most 16 rows */
     int64_t n_chunks;
     int64_t addend_rows;        /* rows of the addend: 256 per chunked tile, the last one may be cut at the end of the batch */

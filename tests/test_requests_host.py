@@ -36,9 +36,9 @@ def test_row_plan_describes_every_row_once(pkg, lengths, adapters):
     assert row_adapter.tolist() == want_adapter and row_request.tolist() == want_request
     assert rows.native.max_adapter == max(want_adapter, default=-1)
     assert rows.native.n_dense == (tiles[:, 2] < 0).sum() and (M > 16 or rows.native.n_dense == 0)
-    # dense tiles: one slot for each adapter, its rows and no others
+    # dense tiles: one slot for each adapter, its rows and no others; few rows beside other adapters are chunked as well
     next_slot = 0
-    addend_at = {}
+    addend_at, few = {}, {}
     for i, (begin, count, addend, _) in enumerate(tiles.tolist()):
         tile_rows = range(256 * i, min(M, 256 * i + 256))
         if addend >= 0:
@@ -51,15 +51,18 @@ def test_row_plan_describes_every_row_once(pkg, lengths, adapters):
         assert sorted(mine[:, 0].tolist()) == sorted({want_adapter[m] for m in tile_rows} - {-1})
         for slot in mine:
             bits = np.unpackbits(slot[4:].view(np.uint8), bitorder="little")
-            assert (256 * i + np.flatnonzero(bits)).tolist() == [m for m in tile_rows if want_adapter[m] == slot[0]]
+            mine_rows = [m for m in tile_rows if want_adapter[m] == slot[0]]
+            assert (256 * i + np.flatnonzero(bits)).tolist() == mine_rows and slot[1] == (count > 1 and len(mine_rows) <= 8)
+            if slot[1]:
+                few.update(dict.fromkeys(mine_rows, -1))
     # chunked tiles: every row in one chunk, with a place of its own in the addend
     covered = {}
     for first, count, adapter, addend in chunks.tolist():
         assert 1 <= count <= 4
         for j in range(count):
             assert first + j not in covered and want_adapter[first + j] == adapter
-            covered[first + j] = addend + j
-    assert covered == addend_at
+            covered[first + j] = addend + j if addend >= 0 else -1
+    assert covered == {**addend_at, **few}
     assert rows.native.addend_rows == len(addend_at) and sorted(addend_at.values()) == list(range(len(addend_at)))
 
 
@@ -134,7 +137,8 @@ def test_abi_refuses_bad_adapter_calls(pkg):
                      (-2, dict(t=ODD)), (-2, dict(bank=ODD)), (-6, dict(ws=None)), (-6, dict(ws_bytes=64)), (-2, dict(ws=ODD))):
         assert gemm(**kw) == want, kw
         assert nat.last_error()
-    for rows in (dict(n_chunks=0), dict(n_chunks=-1, n_dense=2), dict(n_dense=1, slots=None), dict(addend_rows=0), dict(row_adapter=None)):
+    for rows in (dict(n_chunks=0), dict(n_chunks=-1, n_dense=2), dict(n_dense=1, slots=None), dict(addend_rows=0), dict(addend_rows=-1, n_dense=1),
+                 dict(row_adapter=None)):
         assert gemm(rows=native_rows(pkg, **rows)) == -1, rows
     assert gemm(M=0, rows=native_rows(pkg, rows=0)) == 0
     assert gemm(N=0) == 0
