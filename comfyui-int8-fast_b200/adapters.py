@@ -16,7 +16,8 @@ from torch import Tensor
 from . import _native as nat
 
 TILE_ROWS = 256     # rows of a tile of the projection
-TILE_SLOTS = 8      # adapters that a tile may have to be run on the tensor cores
+TILE_SLOTS = 8      # adapters with more than a few rows that a tile may have to be run on the tensor cores
+TILE_ADAPTERS = 16  # adapters in all that it may have (an up-projection MMA each; the few rows' down projection is chunked)
 DENSE_ROWS = 256    # batches of fewer rows are chunked throughout
 FEW_ROWS = 8        # rows of a tile up to which an adapter's down projection is left to chunks where the tile has others
 CHUNK_ROWS = 4      # rows of one adapter that a small work item of the kernels takes together
@@ -85,7 +86,8 @@ class RequestRows:
                         masks[i][a] = masks[i].get(a, 0) | (((1 << (hi - lo)) - 1) << lo)
                 first = last
             per_tile = np.array([len(m) for m in masks])
-            dense = per_tile <= TILE_SLOTS
+            many = np.array([sum(mask.bit_count() > FEW_ROWS for mask in m.values()) for m in masks])
+            dense = (per_tile <= TILE_ADAPTERS) & (many <= TILE_SLOTS)
             # an MMA costs a tile the same for one row as for all: an adapter's few rows beside others are cheaper as chunks there
             table = [(a, int(len(m) > 1 and mask.bit_count() <= FEW_ROWS), mask) for m, d in zip(masks, dense) if d for a, mask in m.items()]
             slots = np.zeros((len(table), 12), dtype=np.int32)

@@ -46,7 +46,7 @@ int* device_status_word();  // device address of the status word on the current 
 struct RequestTile {
     int slot_begin, n_slots, addend_row, pad;
 };
-constexpr int kMaxTileSlots = 8;      // a tile with more adapters than this is chunked
+constexpr int kMaxTileSlots = 8;      // a dense tile's adapters whose down projection is the tile's own
 // One adapter of a tile and the rows of the tile that use it (bit i of word j: row 32 j + i).  `few`: so few rows that chunks do
 // their down projection.
 struct RequestSlot {

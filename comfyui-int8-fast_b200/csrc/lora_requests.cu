@@ -11,6 +11,10 @@
 // adapters update only the rows (tensor-memory lanes) that use it, so the x tile is staged once whatever the adapters, and
 // neither an adapter nor a row can reach what belongs to another.  Tiles where single tokens of many adapters meet arrive
 // as CHUNKS instead, at most four consecutive rows with one adapter, whose factors ordinary warps read once per chunk.
+// An MMA costs a tile the same for one row as for all, so in the down projection (one per adapter and 64 columns of K) an
+// adapter's few rows beside others are chunks too; the up projection (one per adapter and 64 ranks) keeps them on the tensor
+// cores.  1531 rows, K = N = 4096, rank 64: all adapters of a tile on the tensor cores, at most 8 of them: 80 us; their few
+// rows as chunks: 72 us; then up to 16 adapters a tile, 8 of them with more rows: 60 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

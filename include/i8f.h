@@ -307,8 +307,8 @@ typedef struct i8f_request_rows {
     const int32_t* row_adapter; /* [rows]: index into the bank of adapters, -1: none */
     const int32_t* row_request; /* [rows]: request of the row (gated_residual_norm) */
     /* The batch in tiles of 256 rows: [ceil(rows / 256)][4] = first slot, slots, addend row, 0.  A dense tile (addend row
-     * -1) has one slot for each adapter in it, at most 8; a chunked one none, its rows start at `addend row` of the fp32
-     * addend and are covered by chunks. */
+     * -1) has one slot for each adapter in it, at most 32, of which at most 8 without chunks of their own; a chunked one
+     * none, its rows start at `addend row` of the fp32 addend and are covered by chunks. */
     const int32_t* tiles;
     const int32_t* slots;       /* [][12]: adapter, 1 if chunks do its down projection (else 0), 0, 0, then 256 bits: the rows of
                                    the tile that use it */

@@ -101,6 +101,10 @@ LINEAR = [
     ([100, 60, 40], [0, -1, 1], 64, 24576, 16, torch.bfloat16),
     ([2000, 1, 559], [0, 1, 0], 16, 2049, 8, torch.bfloat16),
     ([256], [0], 4224, 64, 128, torch.bfloat16),
+    # sixteen adapters in a tile, some with a few rows: on wide tiles, on narrow ones, without a full tile of rows
+    ([1] * 10 + [240, 3, 8, 9, 700], [*range(10), 10, 11, 12, 13, 14], 512, 12288, 72, torch.bfloat16),
+    ([20] * 8 + [8] * 8 + [40], [*range(16), -1], 320, 336, 16, torch.float16),
+    ([9, 8] * 8 + [1300], [*range(16), 3], 256, 4104, 136, torch.float16),
 ]
 
 

@@ -24,7 +24,9 @@ def tables(rows):
 @pytest.mark.parametrize("lengths,adapters", [
     ([1], None), ([1], [3]), ([0, 5, 0], [0, 1, 2]), ([1] * 9, [0, 0, 0, 0, 0, 1, -1, -1, 1]), ([257, 3, 0, 255], [2, -1, 5, 2]),
     ([4, 4, 1, 300], [1, 1, 1, 0]), ([0, 0], [0, 0]), ([1000], [-1]), ([1] * 400, [i % 9 for i in range(400)]), ([255], [0]), ([256], [0]),
-    ([1] * 300 + [500] + [1] * 100, [i % 20 for i in range(401)]), ([600] + [1] * 50, [0] * 51), ([130, 2, 700], [1048575, -1, 7]),
+    ([1] * 300 + [500] + [1] * 100, [i % 20 for i in range(401)]), ([600] + [1] * 50, [0] * 51),
+    ([1] * 14 + [400], [*range(15)]), ([1] * 15 + [400], [*range(16)]), ([1] * 16 + [400], [*range(17)]),
+    ([20] * 8 + [8] * 8 + [300], [*range(16)] + [-1]), ([20] * 9 + [300], [*range(9)] + [-1]), ([130, 2, 700], [1048575, -1, 7]),
 ])
 def test_row_plan_describes_every_row_once(pkg, lengths, adapters):
     rows = pkg.adapters.RequestRows(lengths, adapters, device="cpu")
@@ -45,9 +47,10 @@ def test_row_plan_describes_every_row_once(pkg, lengths, adapters):
             assert count == 0
             addend_at.update({m: addend + m - 256 * i for m in tile_rows})
             continue
-        assert addend == -1 and 0 <= count <= 8 and begin == next_slot
+        assert addend == -1 and 0 <= count <= 16 and begin == next_slot
         next_slot += count
         mine = slots[begin:begin + count]
+        assert (mine[:, 1] == 0).sum() <= 8
         assert sorted(mine[:, 0].tolist()) == sorted({want_adapter[m] for m in tile_rows} - {-1})
         for slot in mine:
             bits = np.unpackbits(slot[4:].view(np.uint8), bitorder="little")
