@@ -4,9 +4,9 @@
 //   x' = c * x + g(m) * P(y)                 h = N(x') * (1 + s(m)) + t(m)
 //
 // m: the request of the row.  P (after the branch) and N (before the next) are an RMS norm, v / sqrt(mean(v^2) + eps), a
-// LayerNorm, (v - mean) / sqrt(mean((v - mean)^2) + eps), or (P only) nothing; each may carry a weight vector; g may be
-// the tanh of what is given.  h leaves in the branch's 16-bit type, as per-token int8, or both: q = rint(h * (1 / a)),
-// a = max(absmax(h) / 127, 1e-30).
+// LayerNorm, (v - mean) / sqrt(mean((v - mean)^2) + eps), or (P only) nothing, P(y) = y; each may carry a weight vector (without
+// a norm too: a layer scale); g may be the tanh of what is given.  h leaves in the branch's 16-bit type, as per-token int8,
+// or both: q = rint(h * (1 / a)), a = max(absmax(h) / 127, 1e-30).
 //
 // r = 1 / sqrt(...) is the device's rsqrtf (two units in the last place).  Everything between the loads and the stores is
 // fp32: h and its int8 form come from the unrounded x', so each output is
@@ -851,7 +851,7 @@ extern "C" int i8f_gated_residual_norm(const void* x, int x_dtype, int64_t ldx, 
     a.gate = gate;
     a.scale = scale;
     a.shift = shift;
-    a.post_weight = post_norm == I8F_NORM_NONE ? nullptr : post_weight;
+    a.post_weight = post_weight;
     a.weight = weight;
     a.row_request = row_request;
     a.x_out = x_out;

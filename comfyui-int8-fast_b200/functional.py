@@ -686,10 +686,11 @@ def gated_residual_norm(x: Tensor, y: Tensor, gate: Tensor | None = None, *, row
         x_new = residual_scale * x + g * post_norm(y) * post_weight          g = gate, or tanh(gate) with `gate_tanh`
         h     = norm(x_new) * weight * (1 + scale) + shift
 
-    post_norm: None, "rms" or "layer" (without affine part); norm: "rms" or "layer".  gate, scale and shift are [K] for all
-    rows or [requests, K] with the row plan `rows` (row slices of a wider matrix are read in place); they and the weights
-    [K] are taken in y's dtype (bf16 or fp16).  x is in y's dtype or fp32.  Everything in between is fp32 and h comes from
-    the unrounded x_new.  Returns (x_new, h); `x_out` (it may be x) receives x_new.  At most 16384 columns."""
+    post_norm: None (y itself, post_weight is then a layer scale), "rms" or "layer" (without affine part); norm: "rms" or
+    "layer".  gate, scale and shift are [K] for all rows or [requests, K] with the row plan `rows` (row slices of a wider
+    matrix are read in place); they and the weights [K] are taken in y's dtype (bf16 or fp16).  x is in y's dtype or fp32.
+    Everything in between is fp32 and h comes from the unrounded x_new.  Returns (x_new, h); `x_out` (it may be x) receives
+    x_new.  At most 16384 columns."""
     x_new, h, _, _ = _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm, post_weight, norm, weight, scale,
                                           shift, eps, x_out, True, False)
     return x_new, h

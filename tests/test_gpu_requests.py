@@ -374,6 +374,32 @@ def test_gated_residual_norm_shared_vectors(cuda_pkg):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("M,K,dt,xdt", [(6, 512, torch.bfloat16, torch.bfloat16), (5, 2305, torch.float16, torch.float32), (300, 256, torch.bfloat16, torch.float32),
+                                        (300, 4096, torch.bfloat16, torch.bfloat16), (300, 2305, torch.float16, torch.float16),
+                                        (260, 16384, torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("with_gate", [True, False])
+def test_gated_residual_norm_weight_without_post_norm(cuda_pkg, M, K, dt, xdt, with_gate):
+    """A weight behind the branch that no norm precedes (a layer scale): x' = c x + g y w, by every kernel."""
+    F = cuda_pkg.functional
+    g = gen(K)
+    x, y = (torch.randn(M, K, generator=g, device=DEV) * 3).to(xdt), torch.randn(M, K, generator=g, device=DEV).to(dt)
+    w, weight = ((torch.randn(K, generator=g, device=DEV) + 1).to(dt) for _ in range(2))
+    lengths = [M // 2, M - M // 2]
+    rows = cuda_pkg.adapters.RequestRows(lengths, None, DEV)
+    gate = torch.randn(2, K, generator=g, device=DEV).to(dt) if with_gate else None
+    x_new, h = F.gated_residual_norm(x, y, gate, rows=rows, residual_scale=0.5, post_weight=w, norm="layer", weight=weight, eps=1e-5)
+    at = torch.repeat_interleave(torch.arange(2, device=DEV), torch.tensor(lengths, device=DEV))
+    term = y.to(F64) * w.to(F64) * (gate.to(F64)[at] if with_gate else 1.0)
+    xn = 0.5 * x.to(F64) + term
+    xn_off = E32 * (2 * term.abs() + xn.abs())          # two products (0.5 x is exact) and their sum, in fp32
+    check(x_new, xn, xn_off + u_of(xdt) * (xn.abs() + xn_off) + TINY[xdt])
+    hn, hn_off = ref_norm(xn, xn_off, "layer", weight, 1e-5)
+    check(h, hn, hn_off + u_of(dt) * (hn.abs() + hn_off) + TINY[dt])
+    x_q, q, qs = F.quantize_rowwise_gated_residual_norm(x, y, gate, rows=rows, residual_scale=0.5, post_weight=w, norm="layer", weight=weight,
+                                                        eps=1e-5)
+    assert torch.equal(x_q, x_new)
+
+
 def test_gated_residual_norm_special_rows(cuda_pkg):
     """Constant and zero rows are what eps makes of them; a NaN or an infinity stays in its row and shows in its scale."""
     F = cuda_pkg.functional
