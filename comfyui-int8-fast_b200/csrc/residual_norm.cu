@@ -175,9 +175,10 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][V], int kind, float ep
         for (int j = 0; j < V; ++j) v[i][j] *= r;
 }
 
-// Quantisation step of a row from its absolute maximum; a NaN stays: the row is marked by its scale.
+// Quantisation step of a row from its absolute maximum, divided as i8f_quant_rowwise does (a product with 1 / 127 is off by a unit
+// in the last place for some of them); a NaN stays: the row is marked by its scale.
 __device__ __forceinline__ float row_step(float amax) {
-    const float step = amax * (1.0f / 127.0f);
+    const float step = __fdiv_rn(amax, 127.0f);
     return step < kScaleFloor ? kScaleFloor : step;
 }
 template <int V>

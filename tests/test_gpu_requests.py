@@ -400,6 +400,29 @@ def test_gated_residual_norm_weight_without_post_norm(cuda_pkg, M, K, dt, xdt, w
     assert torch.equal(x_q, x_new)
 
 
+@pytest.mark.parametrize("M,K,dt", [(40, 512, torch.bfloat16), (40, 509, torch.float16), (600, 256, torch.float16), (600, 4096, torch.bfloat16),
+                                    (600, 2305, torch.bfloat16)])
+def test_int8_rows_of_the_residual_norm_are_the_quantisers(cuda_pkg, M, K, dt):
+    """A scale of -1 leaves h = shift, exactly: its int8 form has the bits that the quantiser gives the same rows, a step of
+    absmax / 127 rounded once."""
+    F = cuda_pkg.functional
+    g = gen(K + M)
+    x, y, shift = (torch.randn(M, K, generator=g, device=DEV).to(dt) for _ in range(3))
+    rows = cuda_pkg.adapters.RequestRows([1] * M, None, DEV)
+    shared = cuda_pkg.adapters.RequestRows([M // 4] * 4, None, DEV)
+    one = torch.full((K,), -1.0, dtype=dt, device=DEV)
+    for plan, t, at in ((rows, shift, torch.arange(M, device=DEV)), (shared, shift[:4], torch.arange(M, device=DEV) // (M // 4))):
+        _, q, qs, h = F.quantize_rowwise_gated_residual_norm(x, y, rows=plan, scale=one, shift=t, return_h=True)
+        assert torch.equal(h, t[at])
+        amax = h.float().abs().amax(1, keepdim=True)
+        step = torch.div(amax, torch.full_like(amax, 127.0))       # by a tensor: a division, not a product with 1 / 127
+        assert torch.equal(qs, step)
+        assert torch.equal(q, torch.round(h.float() * torch.div(torch.ones_like(step), step)).to(torch.int8))
+        if K % 16 == 0:
+            want_q, want_s = F.quantize_rowwise(h)
+            assert torch.equal(q, want_q) and torch.equal(qs, want_s)
+
+
 def test_gated_residual_norm_special_rows(cuda_pkg):
     """Constant and zero rows are what eps makes of them; a NaN or an infinity stays in its row and shows in its scale."""
     F = cuda_pkg.functional
