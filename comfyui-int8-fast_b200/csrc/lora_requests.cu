@@ -84,7 +84,8 @@ down_chunks_kernel(const void* __restrict__ x, int64_t ldx, const void* __restri
             for (int w = 1; w < kChunkWarps; ++w) big = max(big, s_max[w]);
             __syncthreads();      // before the next row's
             const float amax = DT == I8F_BF16 ? __uint_as_float(big << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(big)));
-            const float step = fmaxf(__fdiv_rn(amax, 127.0f), 1e-30f);
+            float step = __fdiv_rn(amax, 127.0f);
+            if (step < 1e-30f) step = 1e-30f;      // not by fmaxf: a NaN stays in the step and makes the row NaN
             const float inv = __fdiv_rn(1.0f, step);
             const int64_t row = static_cast<int64_t>(c.x) + m;
             if (threadIdx.x == 0) out.scale[row] = step;

@@ -177,6 +177,28 @@ def test_nothing_leaks_between_requests(cuda_pkg, lengths, N):
     assert torch.equal(y[1:], clean[1:]) and not y[0].isfinite().any()
 
 
+@pytest.mark.parametrize("lengths,N,hadamard,rotated", [
+    ([3, 1, 40, 9], 320, False, True),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_nan_activations_stay_nan(cuda_pkg, lengths, N, hadamard, rotated, dtype):
+    """A NaN in a row's activations makes that row NaN, with an adapter and without one, and no other."""
+    F, nat = cuda_pkg.functional, cuda_pkg._native
+    rows = cuda_pkg.adapters.RequestRows(lengths, [-1, 0, 1, -1], DEV)
+    w, ws, b, la, lb = layer(256, N, 16, 2, dtype, 57)
+    x = torch.randn(rows.total, 256, generator=gen(58), device=DEV).to(dtype)
+    bad = torch.zeros(rows.total, dtype=torch.bool, device=DEV)
+    x2 = x.clone()
+    for m, k in ((1, 7), (lengths[0] + lengths[1] + 3, 255), (rows.total - 1, 128)):
+        x2[m, k] = float("nan")
+        bad[m] = True
+    for order in (nat.EPI_SINGLE, nat.EPI_PYTORCH):
+        clean, y = (F.linear_lora_requests(v, w, ws, b, la, lb, rows, dtype, hadamard=hadamard, rotated_lora_input=rotated, order=order)
+                    for v in (x, x2))
+        assert y[bad].isnan().all()
+        assert torch.equal(y[~bad], clean[~bad])
+
+
 @pytest.mark.parametrize("rotated", [True, False])
 def test_linear_lora_requests_rotated(cuda_pkg, rotated):
     F = cuda_pkg.functional
