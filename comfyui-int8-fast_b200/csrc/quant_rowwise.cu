@@ -26,6 +26,13 @@ constexpr float kScaleFloor = 1e-30f;
 
 enum Mode : int { kRowwise = 0, kAbsmaxOnly = 1, kGlobalScale = 2 };
 
+// Larger of two values, a NaN if either is one: a NaN in a row reaches the row's scale, and by it everything made of the row.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 template <int DT>
 __device__ __forceinline__ void load8(const void* base, int64_t elem_off, float (&v)[8]) {
     if constexpr (DT == I8F_BF16) {
@@ -432,20 +439,20 @@ quant_rows_kernel(const void* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
 #pragma unroll
             for (int i = 0; i < VPT; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) amax = fmaxf(fmaxf(amax, fabsf(v[i][j])), fabsf(v[i][j + 1]));
+                for (int j = 0; j < 8; j += 2) amax = max_nan(max_nan(amax, fabsf(v[i][j])), fabsf(v[i][j + 1]));
         }
         // reduce over the lanes of this row that share a warp
         // (the whole warp when only the tensor-wide maximum is wanted)
         const int span = (MODE == kAbsmaxOnly || tpr > 32) ? 32 : tpr;
-        for (int d = 1; d < span; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
+        for (int d = 1; d < span; d <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
         if (tpr > 32 || MODE == kAbsmaxOnly) {
             if (lane == 0) s_part[threadIdx.x >> 5] = amax;
             __syncthreads();
             if constexpr (MODE == kAbsmaxOnly) {
                 if (threadIdx.x == 0) {
                     float m = 0.f;
-                    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) m = fmaxf(m, s_part[w]);
-                    // non-negative floats order like their bit patterns
+                    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) m = max_nan(m, s_part[w]);
+                    // non-negative floats order like their bit patterns, a NaN behind them
                     atomicMax(reinterpret_cast<int*>(gmax), __float_as_int(m));
                 }
                 return;
@@ -453,7 +460,7 @@ quant_rows_kernel(const void* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
                 const int warps_per_row = tpr >> 5;
                 const int first = (threadIdx.x >> tpr_log2) * warps_per_row;
                 float m = 0.f;
-                for (int w = 0; w < warps_per_row; ++w) m = fmaxf(m, s_part[first + w]);
+                for (int w = 0; w < warps_per_row; ++w) m = max_nan(m, s_part[first + w]);
                 amax = m;
             }
         }
@@ -461,7 +468,8 @@ quant_rows_kernel(const void* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
         amax = *gmax;
     }
 
-    const float sc = fmaxf(__fdiv_rn(amax, 127.0f), kScaleFloor);
+    float sc = __fdiv_rn(amax, 127.0f);
+    if (sc < kScaleFloor) sc = kScaleFloor;      // a NaN stays
     const float inv = __fdiv_rn(1.0f, sc);
     if constexpr (MODE == kRowwise) {
         if (row_ok && t == 0) scale[row] = sc;

@@ -642,3 +642,25 @@ def test_launch_counter_counts_kernels(cuda_pkg):
     before = lib.i8f_launch_count()
     F.linear_small_batch(x[:4], wq, ws, None)
     assert lib.i8f_launch_count() - before == 1
+
+
+@pytest.mark.parametrize("K", [128, 272, 1024, 4096, 12288])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("hadamard", [False, True])
+def test_quantiser_marks_rows_with_nan(cuda_pkg, K, dtype, hadamard):
+    """A NaN anywhere in a row is its scale, as max(absmax / 127, 1e-30) has it; the other rows are as they were."""
+    if hadamard and K % 128:
+        pytest.skip("the rotation takes rows of whole blocks of 128")
+    F = cuda_pkg.functional
+    x = torch.randn(70, K, generator=torch.Generator(device=DEV).manual_seed(K), device=DEV).to(dtype)
+    x2 = x.clone()
+    bad = torch.zeros(70, dtype=torch.bool, device=DEV)
+    for m, k in ((0, 0), (5, K - 1), (6, K // 2), (33, 17), (69, K // 3)):
+        x2[m, k] = float("nan") if m != 6 else -float("nan")
+        bad[m] = True
+    q, s = F.quantize_rowwise(x, hadamard=hadamard)
+    q2, s2 = F.quantize_rowwise(x2, hadamard=hadamard)
+    assert s2[bad].isnan().all()
+    assert torch.equal(q2[~bad], q[~bad]) and torch.equal(s2[~bad], s[~bad])
+    qt, st = F.quantize_tensorwise(x2, hadamard=hadamard)
+    assert st.isnan().all() and not F.quantize_tensorwise(x, hadamard=hadamard)[1].isnan().any()

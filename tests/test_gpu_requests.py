@@ -178,7 +178,9 @@ def test_nothing_leaks_between_requests(cuda_pkg, lengths, N):
 
 
 @pytest.mark.parametrize("lengths,N,hadamard,rotated", [
-    ([3, 1, 40, 9], 320, False, True),
+    ([3, 1, 40, 9], 320, False, True), ([300, 5, 40, 200], 320, False, True), ([300, 500, 40, 900], 4096, False, True),
+    ([3, 1, 40, 9], 320, True, True), ([3, 1, 40, 9], 320, True, False), ([300, 5, 40, 200], 320, True, True),
+    ([300, 500, 40, 900], 4096, True, True), ([300, 500, 40, 900], 4096, True, False),
 ])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_nan_activations_stay_nan(cuda_pkg, lengths, N, hadamard, rotated, dtype):
