@@ -127,13 +127,13 @@ __device__ __forceinline__ float row_sum(float v, float* s_part, int row_in_cta)
 }
 __device__ __forceinline__ float row_max(float v, float* s_part, int row_in_cta) {
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+    for (int d = 1; d < 32; d <<= 1) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
     const int warp = threadIdx.x >> 5;
     row_barrier(row_in_cta);
     if ((threadIdx.x & 31) == 0) s_part[warp] = v;
     row_barrier(row_in_cta);
     const float* w = s_part + row_in_cta * 4;
-    return fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+    return max_nan(max_nan(w[0], w[1]), max_nan(w[2], w[3]));
 }
 
 __device__ __forceinline__ float seq_sum8(const float (&f)[8]) {
@@ -162,7 +162,8 @@ __device__ __forceinline__ float packed_absmax(const uint4 (&raw)[VPT]) {
 template <int DT, int VPT>
 __device__ __forceinline__ void quantise_and_store(const uint4 (&raw)[VPT], float amax, bool row_ok, int64_t row, int t, int nvec,
                                                    int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
-    const float sc = fmaxf(__fdiv_rn(amax, 127.0f), kScaleFloor);
+    float sc = __fdiv_rn(amax, 127.0f);
+    if (sc < kScaleFloor) sc = kScaleFloor;      // a NaN stays
     const float inv = __fdiv_rn(1.0f, sc);
     if (row_ok && t == 0) scale[row] = sc;
 #pragma unroll
@@ -373,8 +374,9 @@ ln_modulate_quant_warp_kernel(const void* __restrict__ x, int64_t M, int64_t K, 
     if constexpr (DT == I8F_BF16) amax = __uint_as_float(m16 << 16);
     else amax = __half2float(__ushort_as_half(static_cast<unsigned short>(m16)));
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-    const float sc = fmaxf(__fdiv_rn(amax, 127.0f), kScaleFloor);
+    for (int d = 1; d < 32; d <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
+    float sc = __fdiv_rn(amax, 127.0f);
+    if (sc < kScaleFloor) sc = kScaleFloor;      // a NaN stays
     const float inv = __fdiv_rn(1.0f, sc);
     if (lane == 0) scale[row] = sc;
 #pragma unroll

@@ -26,13 +26,6 @@ constexpr float kScaleFloor = 1e-30f;
 
 enum Mode : int { kRowwise = 0, kAbsmaxOnly = 1, kGlobalScale = 2 };
 
-// Larger of two values, a NaN if either is one: a NaN in a row reaches the row's scale, and by it everything made of the row.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 template <int DT>
 __device__ __forceinline__ void load8(const void* base, int64_t elem_off, float (&v)[8]) {
     if constexpr (DT == I8F_BF16) {

@@ -664,3 +664,24 @@ def test_quantiser_marks_rows_with_nan(cuda_pkg, K, dtype, hadamard):
     assert torch.equal(q2[~bad], q[~bad]) and torch.equal(s2[~bad], s[~bad])
     qt, st = F.quantize_tensorwise(x2, hadamard=hadamard)
     assert st.isnan().all() and not F.quantize_tensorwise(x, hadamard=hadamard)[1].isnan().any()
+
+
+@pytest.mark.parametrize("M,K", [(70, 1024), (70, 8192), (600, 4096)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_fused_quantisers_mark_rows_with_nan(cuda_pkg, M, K, dtype):
+    """The quantisers behind LayerNorm and GELU keep a NaN as the plain one does (short and long rows, direct and by table)."""
+    F = cuda_pkg.functional
+    g = torch.Generator(device=DEV).manual_seed(K)
+    x = torch.randn(M, K, generator=g, device=DEV).to(dtype)
+    shift, scale = (torch.randn(K, generator=g, device=DEV).to(dtype) * 0.1 for _ in range(2))
+    x2 = x.clone()
+    bad = torch.zeros(M, dtype=torch.bool, device=DEV)
+    for m, k in ((0, 0), (5, K - 1), (33, 17), (M - 1, K // 3)):
+        x2[m, k] = float("nan")
+        bad[m] = True
+    plain = torch.randn(M, 512, generator=g, device=DEV).to(dtype)
+    for call in (lambda v: F.quantize_rowwise_ln_modulate(v, shift, scale), lambda v: F.quantize_rowwise_gelu(v),
+                 lambda v: F.quantize_rowwise_gelu(v, plain)):
+        (q, s), (q2, s2) = call(x)[:2], call(x2)[:2]
+        assert s2[bad].isnan().all()
+        assert torch.equal(q2[~bad], q[~bad]) and torch.equal(s2[~bad], s[~bad])
