@@ -142,7 +142,7 @@ class RequestLoras:
 
     @property
     def samples(self) -> int | None:
-        """Samples of the model's current batch, where the model's hook has left word."""
+        """Samples of the model's current batch, where the model's hook has left word and could see it."""
         return self._plans.get("samples")
 
     def bank(self, device: torch.device, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
@@ -150,6 +150,29 @@ class RequestLoras:
         if self._converted is None or self._converted[0].device != device or self._converted[0].dtype != dtype:
             self._converted = (self.lora_a.to(device=device, dtype=dtype).contiguous(), self.lora_b.to(device=device, dtype=dtype).contiguous())
         return self._converted
+
+    def plan(self, rows: int, leading: int | None, device: torch.device) -> RequestRows:
+        """The plan of an input of `rows` rows, equal runs of them one per sample of the batch.  `leading` is the first of the
+        input's three or more dimensions, None for fewer.
+
+        The samples are as many as the model's batch has where its hook has said so and the rows divide by it, else `leading`.
+        An input of two dimensions is one run of rows per request where no hook speaks for the model; where one does but could
+        not see the batch, such an input is refused: which rows are whose cannot be known."""
+        known, n = self.samples, len(self.entries)
+        if not rows:
+            samples = n
+        elif known and rows % known == 0 and known % n == 0:
+            samples = known
+        elif leading is not None:
+            samples = leading
+        elif known is None and "samples" in self._plans:
+            raise ValueError(f"the batch of the model's call is not known (its first argument is no tensor), {rows} rows in two "
+                             "dimensions cannot be told apart by request")
+        else:
+            samples = n
+        if not samples or rows % samples:
+            raise ValueError(f"{rows} rows are not {samples} samples of equal length")
+        return self.rows(samples, rows // samples, device)
 
     def rows(self, samples: int, rows_per_sample: int, device: torch.device) -> RequestRows:
         n = len(self.entries)

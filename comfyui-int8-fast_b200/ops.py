@@ -7,6 +7,7 @@ of libi8f.so and raises if they are unavailable.
 """
 from __future__ import annotations
 
+import inspect
 import logging
 
 import torch
@@ -334,9 +335,15 @@ class DynamicLoRAHook:
             self._held = [d["patches"] for r in ([loras] + list(requests)) for d in r]
         if requests:
             # the samples of this call's batch: a layer that gets one row per sample, or all rows flattened, goes by it
-            x = input_args[0] if input_args else None
+            x = input_args[0] if input_args else input_kwargs.get(self._first_argument(module))
             self._plans["samples"] = x.shape[0] if isinstance(x, Tensor) and x.dim() > 0 else None
         return None
+
+    @staticmethod
+    def _first_argument(module) -> str:
+        """Name of the first parameter of the model's forward (the batch, which may be passed by keyword)."""
+        first = next(iter(inspect.signature(module.forward).parameters.values()), None)
+        return first.name if first is not None and first.kind is first.POSITIONAL_OR_KEYWORD else "x"
 
     @staticmethod
     def _factors(patches):
@@ -446,19 +453,11 @@ def _prepare_lora(module, device: torch.device, dtype: torch.dtype):
 
 
 @torch.compiler.disable
-def _request_forward(loras, x: Tensor, samples: int | None, weight: Tensor, w_scale, bias: Tensor | None, dtype: torch.dtype, hadamard: bool,
+def _request_forward(loras, x: Tensor, leading: int | None, weight: Tensor, w_scale, bias: Tensor | None, dtype: torch.dtype, hadamard: bool,
                      rotated_lora_input: bool) -> Tensor:
     """The Linear's forward for a batch with one adapter per request.  x [rows, K] holds equal runs of rows, one per sample of the
-    batch: as many as the model's batch has where the hook has said so, else `samples` (the first of three or more
-    dimensions), else one per request."""
-    known = loras.samples
-    if known and x.shape[0] % known == 0 and known % len(loras.entries) == 0:
-        samples = known
-    elif samples is None:
-        samples = len(loras.entries)
-    if x.shape[0] % samples:
-        raise ValueError(f"{x.shape[0]} rows are not {samples} samples of equal length")
-    plan = loras.rows(samples, x.shape[0] // samples, x.device)
+    batch; `leading` is the first of the input's three or more dimensions (RequestLoras.plan says which run is whose)."""
+    plan = loras.plan(x.shape[0], leading, x.device)
     lora_a, lora_b = loras.bank(x.device, dtype)
     if x.shape[0] > SMALL_BATCH_ROWS:
         return F.linear_lora_requests(x, weight, w_scale, bias, lora_a, lora_b, plan, dtype, hadamard=hadamard,

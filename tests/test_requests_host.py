@@ -267,3 +267,56 @@ def test_request_loras_refuse(pkg):
     for args in ((a[0], b, [0]), (a, b[:1], [0]), (a, b[:, :, :4], [0]), (a, b, []), (a, b, [2]), (a, b, [-2])):
         with pytest.raises(ValueError):
             A(*args)
+
+
+def linear_plan(pkg, monkeypatch, loras, shape):
+    """Lengths and adapters of the rows that the Linear's forward hands to the kernels for an input of this shape."""
+    seen = []
+
+    def take(x, weight, w_scale, bias, lora_a, lora_b, rows, *args, **kw):
+        seen.append(rows)
+        return x
+
+    monkeypatch.setattr(pkg.ops.F, "linear_lora_requests", take)
+    monkeypatch.setattr(pkg.ops.F, "linear_small_batch_lora_requests", take)
+    x = torch.zeros(shape)
+    pkg.ops._request_forward(loras, x.reshape(-1, shape[-1]), shape[0] if len(shape) > 2 else None, None, None, None, x.dtype, False, True)
+    return [a for n, a in zip(seen[0].lengths, seen[0].adapters) for _ in range(n)]
+
+
+class _Model(torch.nn.Module):
+    def __init__(self, forward):
+        super().__init__()
+        self.layer = _Layer(24, 32)
+        self._run = forward
+
+    def forward(self, latent, t=None, transformer_options={}):
+        return self._run(latent)
+
+
+def two_requests(pkg, *input_args, **input_kwargs):
+    """The first layer's RequestLoras and the hook's model after a call of two requests with one LoRA each."""
+    model = _Model(lambda latent: latent)
+    one, two = ({"patches": {"layer.weight": _Adapter(torch.ones(24, 4), torch.ones(4, 32))}, "strength": 1.0} for _ in range(2))
+    pkg.ops.DynamicLoRAHook.register(model)
+    model(*input_args, transformer_options={"request_loras": [[one], [two]]}, **input_kwargs)
+    return model.layer.request_loras
+
+
+def test_hook_sees_a_batch_that_is_passed_by_keyword(pkg, monkeypatch):
+    """Two requests under guidance, four samples: row j of a two-dimensional input is request j modulo 2, however the batch is
+    passed; where the hook cannot see the batch, such an input is refused, never cut by guess."""
+    for loras in (two_requests(pkg, torch.zeros(4, 3)), two_requests(pkg, latent=torch.zeros(4, 3))):
+        assert loras.samples == 4
+        assert linear_plan(pkg, monkeypatch, loras, (4, 32)) == [0, 1, 0, 1]
+        assert linear_plan(pkg, monkeypatch, loras, (4, 2, 32)) == [0, 0, 1, 1, 0, 0, 1, 1]
+    unseen = two_requests(pkg, [torch.zeros(4, 3)])
+    assert unseen.samples is None
+    with pytest.raises(ValueError, match="batch"):
+        linear_plan(pkg, monkeypatch, unseen, (4, 32))
+    assert linear_plan(pkg, monkeypatch, unseen, (4, 1, 32)) == [0, 1, 0, 1]       # the leading dimension says it
+    # a layer whose model has no hook: two dimensions are one run of rows per request, as it is told
+    alone = pkg.adapters.RequestLoras(unseen.lora_a, unseen.lora_b, [0, 1])
+    assert linear_plan(pkg, monkeypatch, alone, (4, 32)) == [0, 0, 1, 1]
+    for shape in ((0, 32), (0, 5, 32), (2, 0, 32)):
+        assert linear_plan(pkg, monkeypatch, alone, shape) == linear_plan(pkg, monkeypatch, unseen, shape) == []
