@@ -155,17 +155,20 @@ class RequestLoras:
         """The plan of an input of `rows` rows, equal runs of them one per sample of the batch.  `leading` is the first of the
         input's three or more dimensions, None for fewer.
 
-        The samples are as many as the model's batch has where its hook has said so and the rows divide by it, else `leading`.
-        An input of two dimensions is one run of rows per request where no hook speaks for the model; where one does but could
-        not see the batch, such an input is refused: which rows are whose cannot be known."""
+        Where the requests differ, the samples are as many as the model's batch has where its hook has said so and the rows
+        divide by it, else `leading`; rows that are not equal runs for every request are refused.  An input of two dimensions
+        goes by the hook's word alone: where the hook could not see the batch it is refused, and only where no hook speaks for
+        the model it is one run of rows per request."""
         known, n = self.samples, len(self.entries)
         if not rows:
             samples = n
-        elif known and rows % known == 0 and known % n == 0:
-            samples = known
+        elif len(set(self.entries)) == 1:      # one composition for all: nothing to tell apart
+            return self._planned([rows], self.entries[:1], device)
+        elif known is not None:
+            samples = known if leading is None or (known and rows % known == 0) else leading
         elif leading is not None:
             samples = leading
-        elif known is None and "samples" in self._plans:
+        elif "samples" in self._plans:
             raise ValueError(f"the batch of the model's call is not known (its first argument is no tensor), {rows} rows in two "
                              "dimensions cannot be told apart by request")
         else:
@@ -178,10 +181,13 @@ class RequestLoras:
         n = len(self.entries)
         if samples % n:
             raise ValueError(f"a batch of {samples} samples for {n} requests")
-        key = (self.entries, samples, rows_per_sample, device)
+        return self._planned([rows_per_sample] * samples, self.entries * (samples // n), device)
+
+    def _planned(self, lengths: list[int], entries: tuple[int, ...], device: torch.device) -> RequestRows:
+        key = (entries, len(lengths), lengths[0] if lengths else 0, device)
         plan = self._plans.get(key)
         if plan is None:
-            plan = self._plans[key] = RequestRows([rows_per_sample] * samples, [self.entries[j % n] for j in range(samples)], device)
+            plan = self._plans[key] = RequestRows(lengths, entries, device)
         return plan
 
 

@@ -320,3 +320,19 @@ def test_hook_sees_a_batch_that_is_passed_by_keyword(pkg, monkeypatch):
     assert linear_plan(pkg, monkeypatch, alone, (4, 32)) == [0, 0, 1, 1]
     for shape in ((0, 32), (0, 5, 32), (2, 0, 32)):
         assert linear_plan(pkg, monkeypatch, alone, shape) == linear_plan(pkg, monkeypatch, unseen, shape) == []
+
+
+def test_batch_that_is_no_multiple_of_the_requests_is_refused(pkg, monkeypatch):
+    loras = two_requests(pkg, torch.zeros(3, 3))
+    for shape in ((6, 32), (2, 32), (3, 2, 32), (6, 2, 32)):
+        with pytest.raises(ValueError):
+            linear_plan(pkg, monkeypatch, loras, shape)
+    loras = two_requests(pkg, torch.zeros(4, 3))
+    for shape in ((6, 32), (2, 32)):               # rows that are not four samples, in two dimensions
+        with pytest.raises(ValueError):
+            linear_plan(pkg, monkeypatch, loras, shape)
+    # where all requests have one composition there is nothing to tell apart
+    for entries, known in (([0], 3), ([1, 1], 3), ([-1, -1, -1], 4), ([0], None)):
+        same = pkg.adapters.RequestLoras(loras.lora_a, loras.lora_b, entries, {"samples": known})
+        for shape in ((6, 32), (7, 32), (1, 5, 32), (5, 3, 32)):
+            assert linear_plan(pkg, monkeypatch, same, shape) == [entries[0]] * int(np.prod(shape[:-1]))
