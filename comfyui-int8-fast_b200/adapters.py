@@ -155,17 +155,21 @@ class RequestLoras:
         """The plan of an input of `rows` rows, equal runs of them one per sample of the batch.  `leading` is the first of the
         input's three or more dimensions, None for fewer.
 
-        Where the requests differ, the samples are as many as the model's batch has where its hook has said so and the rows
-        divide by it, else `leading`; rows that are not equal runs for every request are refused.  An input of two dimensions
-        goes by the hook's word alone: where the hook could not see the batch it is refused, and only where no hook speaks for
-        the model it is one run of rows per request."""
+        Where the requests differ, the samples are as many as the model's batch has where its hook has said so: the input's
+        leading dimension has to be that many, or 1 with the rows of all samples behind it (rows that the samples share have no
+        adapter of their own).  Another leading dimension is refused, since it does not say whether its rows
+        repeat the samples one after the other or cut each of them in pieces.  Where the hook could not see the batch `leading`
+        counts and an input of two dimensions is refused; where no hook speaks for the model such an input is one run of rows
+        per request.  Rows that are not equal runs for every request are refused."""
         known, n = self.samples, len(self.entries)
         if not rows:
             samples = n
         elif len(set(self.entries)) == 1:      # one composition for all: nothing to tell apart
             return self._planned([rows], self.entries[:1], device)
         elif known is not None:
-            samples = known if leading is None or (known and rows % known == 0) else leading
+            if leading not in (None, 1, known):
+                raise ValueError(f"a leading dimension of {leading} for a batch of {known} samples: which rows are whose cannot be known")
+            samples = known
         elif leading is not None:
             samples = leading
         elif "samples" in self._plans:

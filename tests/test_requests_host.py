@@ -336,3 +336,18 @@ def test_batch_that_is_no_multiple_of_the_requests_is_refused(pkg, monkeypatch):
         same = pkg.adapters.RequestLoras(loras.lora_a, loras.lora_b, entries, {"samples": known})
         for shape in ((6, 32), (7, 32), (1, 5, 32), (5, 3, 32)):
             assert linear_plan(pkg, monkeypatch, same, shape) == [entries[0]] * int(np.prod(shape[:-1]))
+
+
+def test_leading_dimension_that_is_not_the_batch_is_refused(pkg, monkeypatch):
+    """[2 B, T, K] may be the batch twice (0, 1, 0, 1) or two pieces of every sample (0, 0, 1, 1)."""
+    for batch in (2, 4):
+        loras = two_requests(pkg, torch.zeros(batch, 3))
+        assert loras.samples == batch
+        for leading in (2 * batch, 3 * batch, batch + 1, 6 - batch):
+            with pytest.raises(ValueError, match="leading"):
+                linear_plan(pkg, monkeypatch, loras, (leading, 12, 32))
+        want = [j % 2 for j in range(batch) for _ in range(12)]
+        for shape in ((batch, 12, 32), (batch, 3, 4, 32), (1, 12 * batch, 32), (12 * batch, 32)):
+            assert linear_plan(pkg, monkeypatch, loras, shape) == want
+        with pytest.raises(ValueError):
+            linear_plan(pkg, monkeypatch, loras, (1, 12 * batch + 1, 32))
