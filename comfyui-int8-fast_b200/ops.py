@@ -7,6 +7,7 @@ of libi8f.so and raises if they are unavailable.
 """
 from __future__ import annotations
 
+import functools
 import inspect
 import logging
 
@@ -386,7 +387,9 @@ class DynamicLoRAHook:
             K, N = some[0].flatten(1).shape[1], some[1].flatten(1).shape[0]
             empty = (some[0].new_zeros(0, K), some[1].new_zeros(N, 0))
             device = getattr(module, "weight", torch.tensor(0)).device
-            bank = adapters.stack_adapters([p if p is not None else empty for p in pairs], some[0].dtype, device)
+            # a type that holds the factors of all requests: what one request uses may not cost another's bits
+            dtype = functools.reduce(torch.promote_types, (f.dtype for p in pairs if p is not None for f in p))
+            bank = adapters.stack_adapters([p if p is not None else empty for p in pairs], dtype, device)
             module.request_loras = adapters.RequestLoras(*bank, entries, plans)
 
     def apply_composition(self, diffusion_model, dynamic_loras):

@@ -351,3 +351,23 @@ def test_leading_dimension_that_is_not_the_batch_is_refused(pkg, monkeypatch):
             assert linear_plan(pkg, monkeypatch, loras, shape) == want
         with pytest.raises(ValueError):
             linear_plan(pkg, monkeypatch, loras, (1, 12 * batch + 1, 32))
+
+
+@pytest.mark.parametrize("types", [(torch.bfloat16, torch.float32), (torch.float16, torch.bfloat16), (torch.float16, torch.float32),
+                                   (torch.bfloat16, torch.bfloat16)])
+def test_bank_holds_every_requests_factors_in_full(pkg, types):
+    """LoRAs of several types in one batch, in either order: each entry of the bank has its own LoRA's values to the bit."""
+    g = torch.Generator().manual_seed(5)
+    factors = {t: (torch.randn(24, 4, generator=g) * 1e5 if t is not torch.float16 else torch.randn(24, 4, generator=g),
+                   torch.randn(4, 32, generator=g) * 1e-9 if t is not torch.float16 else torch.randn(4, 32, generator=g)) for t in set(types)}
+    for order in (types, types[::-1]):
+        model = _Model(lambda latent: latent)
+        pkg.ops.DynamicLoRAHook.register(model)
+        entries = [{"patches": {"layer.weight": _Adapter(*(f.to(t) for f in factors[t]), alpha=4.0)}, "strength": 1.0} for t in order]
+        model(torch.zeros(2, 3), transformer_options={"request_loras": [[e] for e in entries]})
+        bank = model.layer.request_loras
+        for i, t in enumerate(order):
+            up, down = (f.to(t) for f in factors[t])
+            assert torch.equal(bank.lora_a[bank.entries[i], :4].float(), down.float())
+            assert torch.equal(bank.lora_b[bank.entries[i], :, :4].float(), up.float())
+    assert types[0] is not types[1] or bank.lora_a.dtype is types[0]
