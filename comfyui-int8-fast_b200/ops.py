@@ -312,6 +312,7 @@ class DynamicLoRAHook:
     `request_loras` in transformer_options gives a batch one composition per request: a list with, for every request, a list
     of entries like those of `dynamic_loras` (which all requests share on top).  Each quantised layer then holds a bank of the
     distinct compositions (`request_loras`) in place of lora_A / lora_B."""
+    _HALF_SET = object()        # no composition's id: one that was refused half way is not taken for the one before
 
     def __init__(self):
         self.current_lora_id = None
@@ -328,6 +329,7 @@ class DynamicLoRAHook:
         if requests:
             lora_id = (lora_id, tuple(tuple((id(d["patches"]), d["strength"]) for d in r) for r in requests))
         if lora_id != self.current_lora_id:
+            self.current_lora_id = self._HALF_SET
             if requests:
                 self.apply_requests(module, loras, requests)
             else:

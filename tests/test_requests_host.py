@@ -371,3 +371,22 @@ def test_bank_holds_every_requests_factors_in_full(pkg, types):
             assert torch.equal(bank.lora_a[bank.entries[i], :4].float(), down.float())
             assert torch.equal(bank.lora_b[bank.entries[i], :, :4].float(), up.float())
     assert types[0] is not types[1] or bank.lora_a.dtype is types[0]
+
+
+def test_refused_composition_does_not_pass_for_the_one_before(pkg):
+    """A composition that does not fit a layer raises; the next call sets every layer up again, whatever it asks for."""
+    model = torch.nn.ModuleDict({"a": _Layer(24, 32), "b": _Layer(16, 32)})
+    hook = pkg.ops.DynamicLoRAHook()
+
+    def entry(n_b):
+        return {"patches": {"a.weight": _Adapter(torch.ones(24, 4), torch.ones(4, 32)), "b.weight": _Adapter(torch.ones(n_b, 4), torch.ones(5, 32))},
+                "strength": 1.0}
+
+    good = {"patches": {k + ".weight": _Adapter(torch.ones(n, 4), torch.ones(4, 32)) for k, n in (("a", 24), ("b", 16))}, "strength": 1.0}
+    for opts in ({"request_loras": [[good], []]}, {"dynamic_loras": [good]}, {}):
+        hook.pre_forward(model, (), {"transformer_options": opts})
+        want = [(m.request_loras is not None, m.lora_A is not None) for m in model.values()]
+        with pytest.raises(ValueError):
+            hook.pre_forward(model, (), {"transformer_options": {"request_loras": [[entry(16)]]}})
+        hook.pre_forward(model, (), {"transformer_options": opts})
+        assert [(m.request_loras is not None, m.lora_A is not None) for m in model.values()] == want
