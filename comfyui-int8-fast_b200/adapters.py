@@ -20,6 +20,7 @@ TILE_SLOTS = 8      # adapters with more than a few rows that a tile may have to
 TILE_ADAPTERS = 16  # adapters in all that it may have (an up-projection MMA each; the few rows' down projection is chunked)
 DENSE_ROWS = 256    # batches of fewer rows are chunked throughout
 FEW_ROWS = 8        # rows of a tile up to which an adapter's down projection is left to chunks where the tile has others
+MAX_RANK = 1024     # ranks of an adapter that the projections take
 CHUNK_ROWS = 4      # rows of one adapter that a small work item of the kernels takes together
 
 

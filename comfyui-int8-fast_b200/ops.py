@@ -391,6 +391,9 @@ class DynamicLoRAHook:
             device = getattr(module, "weight", torch.tensor(0)).device
             # a type that holds the factors of all requests: what one request uses may not cost another's bits
             dtype = functools.reduce(torch.promote_types, (f.dtype for p in pairs if p is not None for f in p))
+            rank = max(p[0].shape[0] for p in pairs if p is not None)
+            if rank > adapters.MAX_RANK:
+                raise ValueError(f"{name}: the LoRAs of a request have {rank} ranks together, at most {adapters.MAX_RANK} beside one another")
             bank = adapters.stack_adapters([p if p is not None else empty for p in pairs], dtype, device)
             module.request_loras = adapters.RequestLoras(*bank, entries, plans)
 

@@ -390,3 +390,18 @@ def test_refused_composition_does_not_pass_for_the_one_before(pkg):
             hook.pre_forward(model, (), {"transformer_options": {"request_loras": [[entry(16)]]}})
         hook.pre_forward(model, (), {"transformer_options": opts})
         assert [(m.request_loras is not None, m.lora_A is not None) for m in model.values()] == want
+
+
+def test_hook_refuses_ranks_that_the_layers_would(pkg):
+    """A request's LoRAs add up to more ranks than the projections take: refused by name when the banks are made."""
+    model = torch.nn.ModuleDict({"a": _Layer(24, 32)})
+    hook = pkg.ops.DynamicLoRAHook()
+
+    def entry(r):
+        return {"patches": {"a.weight": _Adapter(torch.zeros(24, r), torch.zeros(r, 32))}, "strength": 1.0}
+
+    hook.pre_forward(model, (), {"transformer_options": {"request_loras": [[entry(1000), entry(24)], [entry(8)]]}})
+    assert model["a"].request_loras.lora_a.shape == (2, 1024, 32)
+    with pytest.raises(ValueError, match="^a: .* 1025 ranks"):
+        hook.pre_forward(model, (), {"transformer_options": {"request_loras": [[entry(8)], [entry(1000), entry(25)]]}})
+    assert pkg.adapters.MAX_RANK == 1024      # what the library refuses beyond (test_abi_refuses_bad_adapter_calls)
