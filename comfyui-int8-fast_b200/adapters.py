@@ -28,9 +28,9 @@ class RequestRows:
     """The rows of a batch: `lengths[i]` consecutive rows belong to request i (0 is allowed), which uses entry `adapters[i]`
     of the bank of adapters, or none (-1, also without `adapters`).  Rows that pad a batch are a request without an adapter.
 
-    The tables are copied to `device` here (the host waits for the copy, so they may be used on any stream afterwards);
-    make the plan outside a graph capture.  A captured call keeps the plan that it was captured with, which has to outlive
-    the graph.
+    The tables are copied to `device` here (the host waits for the copy, so they may be used on any stream afterwards, and the
+    plan may be dropped while calls with it are under way); make the plan outside a graph capture.  A captured call keeps
+    the tables that it was captured with: the plan has to outlive the graph.
     """
 
     def __init__(self, lengths: Sequence[int], adapters: Sequence[int] | None = None,
@@ -63,9 +63,17 @@ class RequestRows:
         self.native = nat.RequestRowsStruct(rows=self.total, row_adapter=at[0], row_request=at[1], tiles=at[2], slots=at[3], chunks=at[4],
                                             n_dense=int((tiles[:, 2] < 0).sum()), n_chunks=chunks.shape[0], addend_rows=addend_rows,
                                             max_adapter=self.max_adapter)
+        # streams whose calls the allocator waits for before it hands the tables' memory on
+        self.streams = {nat.stream_handle(self.device)} if self.device.type == "cuda" else set()
         self.native_ptr = ctypes.byref(self.native)
         self.row_request_ptr = at[1]
         self.workspace_bytes: dict = {}      # sizes the library asks for, by layer shape
+
+    def use_on(self, stream: int) -> None:
+        """A call on `stream` (the handle of the device's current one, not in `streams` yet) is about to read the tables."""
+        if not torch.cuda.is_current_stream_capturing():
+            self._tables.record_stream(torch.cuda.current_stream(self.device))
+            self.streams.add(stream)
 
     @staticmethod
     def _plan(row_adapter: np.ndarray, lengths: Sequence[int], adapters: Sequence[int]):

@@ -459,6 +459,14 @@ def _check_requests(rows: RequestRows, x: Tensor, lora_a: Tensor | None, lora_b:
     return n, r
 
 
+def _stream_for(rows: RequestRows, device: torch.device) -> int:
+    """The device's current stream, on which a call is about to read the plan's tables."""
+    stream = nat.stream_handle(device)
+    if stream not in rows.streams:
+        rows.use_on(stream)
+    return stream
+
+
 def lora_down_requests(x: Tensor, lora_a: Tensor, rows: RequestRows) -> Tensor:
     """t [M,r]: row m of x (bf16 or fp16) times the transposed lora_a [adapters, r, K] of the row's adapter, in x's dtype;
     zeros on rows without an adapter."""
@@ -469,7 +477,7 @@ def lora_down_requests(x: Tensor, lora_a: Tensor, rows: RequestRows) -> Tensor:
         t = torch.empty((M, r), dtype=x.dtype, device=x.device)
         if M:
             nat.check(nat.load().i8f_lora_down_requests(x.data_ptr(), _ld(x), lora_a.data_ptr(), n, r, rows.native_ptr, t.data_ptr(), r,
-                                                        _code(x.dtype), M, K, nat.current_stream(x.device)),
+                                                        _code(x.dtype), M, K, _stream_for(rows, x.device)),
                       "i8f_lora_down_requests")
         return t
 
@@ -506,7 +514,7 @@ def linear_w8a8_lora_requests(q: Tensor, q_scale: Tensor, w: Tensor, w_scale, bi
                                                         _code(bias.dtype) if bias is not None else 0, t.data_ptr(), _ld(t),
                                                         lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(), _code(out_dtype), N, M,
                                                         N, K, order, workspace.data_ptr() if need else None, need,
-                                                        nat.current_stream(q.device)), "i8f_linear_w8a8_lora_requests")
+                                                        _stream_for(rows, q.device)), "i8f_linear_w8a8_lora_requests")
         return out
 
 
@@ -545,7 +553,7 @@ def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lor
                                               ws.data_ptr(), mode, bias.data_ptr() if bias is not None else None,
                                               _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(), lora_b.data_ptr(), n, r,
                                               rows.native_ptr, out.data_ptr(), N, M, N, K, order, workspace.data_ptr(), need,
-                                              nat.stream_handle(device))
+                                              _stream_for(rows, device))
             if rc:
                 nat.check(rc, "i8f_linear_lora_requests")
         return out
@@ -576,7 +584,7 @@ def linear_small_batch_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor
                                                           bias.data_ptr() if bias is not None else None,
                                                           _code(bias.dtype) if bias is not None else 0, lora_a.data_ptr(),
                                                           lora_b.data_ptr(), n, r, rows.native_ptr, out.data_ptr(), N, M, N, K,
-                                                          workspace.data_ptr(), need, nat.stream_handle(device))
+                                                          workspace.data_ptr(), need, _stream_for(rows, device))
             if rc:
                 nat.check(rc, "i8f_linear_w8a16_small_lora_requests")
         return out
@@ -671,7 +679,7 @@ def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm,
                 x.data_ptr(), _code(x.dtype), ldx, y.data_ptr(), _code(dtype), ldy, M, K, row_request, requests if row_request is not None else 1, g, ldg, 1 if gate_tanh else 0,
                 residual_scale, nat.NORM_CODE[post_norm], pw, nat.NORM_CODE[norm], nw, s, lds, t, ldt, eps, x_out.data_ptr(), ldo,
                 h.data_ptr() if want_h else None, K, q.data_ptr() if want_q else None, K, q_scale.data_ptr() if want_q else None,
-                nat.stream_handle(device))
+                nat.stream_handle(device) if row_request is None else _stream_for(rows, device))
             if rc:
                 nat.check(rc, "i8f_gated_residual_norm")
         return x_out, h, q, q_scale

@@ -594,6 +594,38 @@ def test_two_calls_at_once_on_two_streams(cuda_pkg):
         assert all(torch.equal(o[0], want[i][0]) and torch.equal(o[1], want[i][1]) for o in outs[i])
 
 
+def test_plan_dropped_while_another_stream_reads_it(cuda_pkg):
+    """The tables' memory is not handed on before the calls on other streams are done, whichever entry point made them."""
+    F = cuda_pkg.functional
+    Rows = cuda_pkg.adapters.RequestRows
+    w, ws, b, la, lb = layer(512, 640, 16, 3, torch.bfloat16, 95)
+    x = torch.randn(600, 512, generator=gen(96), device=DEV).bfloat16()
+    y = torch.randn(600, 512, generator=gen(97), device=DEV).bfloat16()
+    gate = torch.randn(3, 512, generator=gen(98), device=DEV).bfloat16()
+    q, qs = F.quantize_rowwise(x)
+    t = F.lora_down_requests(x, la, Rows([300, 100, 200], [0, -1, 2], DEV))
+    calls = [lambda p: F.linear_lora_requests(x, w, ws, b, la, lb, p, x.dtype), lambda p: F.lora_down_requests(x, la, p),
+             lambda p: F.linear_w8a8_lora_requests(q, qs, w, ws, b, t, lb, p, x.dtype),
+             lambda p: F.gated_residual_norm(x, y, gate, rows=p)[1],
+             lambda p: F.linear_small_batch_lora_requests(x[:9], w, ws, b, la, lb, p)]
+    side = torch.cuda.Stream()
+    for i, call in enumerate(calls):
+        plan = Rows([3, 1, 5] if i == 4 else [300, 100, 200], [0, -1, 2], DEV)
+        want = call(plan)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(50_000_000)        # some 30 ms
+            got = call(plan)
+        at, n = plan._tables.data_ptr(), plan._tables.numel()
+        assert not side.query()
+        del plan
+        later = [torch.full((n,), 1 << 20, dtype=torch.int32, device=DEV) for _ in range(8)]
+        assert all(v.data_ptr() != at for v in later)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del later
+
+
 def test_offsets_past_32_bits(cuda_pkg):
     """Rows that lie further apart than 32 bits can count: 20 rows with a pitch of 2^27 elements."""
     F = cuda_pkg.functional

@@ -405,3 +405,30 @@ def test_hook_refuses_ranks_that_the_layers_would(pkg):
     with pytest.raises(ValueError, match="^a: .* 1025 ranks"):
         hook.pre_forward(model, (), {"transformer_options": {"request_loras": [[entry(8)], [entry(1000), entry(25)]]}})
     assert pkg.adapters.MAX_RANK == 1024      # what the library refuses beyond (test_abi_refuses_bad_adapter_calls)
+
+
+def test_plan_is_held_for_the_streams_that_read_it(pkg, monkeypatch):
+    """Every entry point that hands the tables to the library reports its stream; the first report of a stream is recorded with the
+    allocator, but not within a graph capture, whose plan the caller holds."""
+    rows = pkg.adapters.RequestRows([3, 2], [0, -1], device="cpu")
+    recorded, capturing = [], [False]
+
+    class Tables:
+        def record_stream(self, stream):
+            recorded.append(stream)
+
+    rows._tables = Tables()
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: ("stream", handle[0]))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    handle = [5]
+    monkeypatch.setattr(pkg.functional.nat, "stream_handle", lambda device: handle[0])
+    stream_for = pkg.functional._stream_for
+    assert rows.streams == set()
+    for h in (5, 5, 7, 5):
+        handle[0] = h
+        assert stream_for(rows, rows.device) == h
+    assert recorded == [("stream", 5), ("stream", 7)]
+    capturing[0], handle[0] = True, 9
+    assert stream_for(rows, rows.device) == 9 and len(recorded) == 2
+    capturing[0] = False
+    assert stream_for(rows, rows.device) == 9 and recorded[2:] == [("stream", 9)]
