@@ -148,6 +148,8 @@ class RequestLoras:
         self.entries = tuple(int(e) for e in entries)
         self._plans = {} if plans is None else plans
         self._converted = None
+        self._streams: set = set()      # those that have waited for the conversion
+        self._ready = None
 
     @property
     def samples(self) -> int | None:
@@ -155,10 +157,27 @@ class RequestLoras:
         return self._plans.get("samples")
 
     def bank(self, device: torch.device, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
-        """The bank in the compute type on the compute device, converted once."""
-        if self._converted is None or self._converted[0].device != device or self._converted[0].dtype != dtype:
-            self._converted = (self.lora_a.to(device=device, dtype=dtype).contiguous(), self.lora_b.to(device=device, dtype=dtype).contiguous())
-        return self._converted
+        """The bank in the compute type on the compute device, converted once: another stream than the first waits for that, and
+        the allocator for it.  Within a graph capture nothing is kept, since the conversion only runs with the graph."""
+        held = self._converted
+        fits = held is not None and held[0].device == device and held[0].dtype == dtype
+        if not fits:
+            held = (self.lora_a.to(device=device, dtype=dtype).contiguous(), self.lora_b.to(device=device, dtype=dtype).contiguous())
+        if device.type == "cuda":
+            handle = nat.stream_handle(device)
+            if (fits and handle in self._streams) or torch.cuda.is_current_stream_capturing():
+                return held
+            stream = torch.cuda.current_stream(device)
+            if fits:
+                stream.wait_event(self._ready)
+            else:
+                self._ready = stream.record_event()
+                self._streams = set()
+            self._streams.add(handle)
+            for t in held:
+                t.record_stream(stream)
+        self._converted = held
+        return held
 
     def plan(self, rows: int, leading: int | None, device: torch.device) -> RequestRows:
         """The plan of an input of `rows` rows, equal runs of them one per sample of the batch.  `leading` is the first of the

@@ -704,6 +704,40 @@ def test_linear_module_with_request_loras(cuda_pkg, tokens, quarot):
     assert torch.equal(lin(x.reshape(1, -1, K)).reshape(y.shape), y)
 
 
+def test_linear_module_on_two_streams_and_captured_first(cuda_pkg):
+    """A bank of another type than the activations is converted by the first call: a second stream waits for that, and a first call
+    within a graph capture leaves nothing that later calls would take for converted."""
+    K, N = 256, 320
+    w, ws, b, la, lb = layer(K, N, 16, 3, torch.bfloat16, 45)
+    lin = cuda_pkg.ops.StandaloneInt8Ops.Linear(K, N, bias=True, device="meta")
+    lin._load_from_state_dict({"weight": w, "weight_scale": ws, "bias": b}, "", {}, True, [], [], [])
+    x = torch.randn(4, 50, K, generator=gen(46), device=DEV).bfloat16()
+    wide = la.float(), lb.float()
+    plans: dict = {}
+
+    def loras():
+        return cuda_pkg.adapters.RequestLoras(*wide, [1, -1], plans)
+
+    lin.request_loras = loras()
+    want = lin(x)
+    torch.cuda.synchronize()
+    lin.request_loras = loras()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        first = lin(x)
+    second = lin(x)                        # the conversion is still to come, on the other stream
+    torch.cuda.synchronize()
+    assert torch.equal(first, want) and torch.equal(second, want)
+    lin.request_loras = loras()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = lin(x)
+    assert torch.equal(lin(x), want)       # before the graph has run
+    graph.replay()
+    assert torch.equal(captured, want)
+
+
 def test_dit_batch_of_samples_fused(cuda_pkg):
     """A batch of samples through the fused block code against the same model in element-wise steps: the differences are 16-bit
     roundings that the fused pass leaves out, and the int8 steps they move."""

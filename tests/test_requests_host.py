@@ -432,3 +432,60 @@ def test_plan_is_held_for_the_streams_that_read_it(pkg, monkeypatch):
     assert stream_for(rows, rows.device) == 9 and len(recorded) == 2
     capturing[0] = False
     assert stream_for(rows, rows.device) == 9 and recorded[2:] == [("stream", 9)]
+
+
+class _FakeTensor:
+    """A factor bank on a pretended device, which notes the streams that it is recorded for."""
+
+    def __init__(self, shape, device, dtype, made):
+        self.shape, self.device, self.dtype, self.made, self.streams = shape, device, dtype, made, []
+        made.append(self)
+
+    def dim(self):
+        return len(self.shape)
+
+    def to(self, device, dtype):
+        return _FakeTensor(self.shape, device, dtype, self.made)
+
+    def contiguous(self):
+        return self
+
+    def record_stream(self, stream):
+        self.streams.append(stream.name)
+
+
+def test_converted_bank_on_other_streams_and_in_captures(pkg, monkeypatch):
+    """A second stream waits for the conversion that the first one made, and holds its memory; a conversion within a capture is not
+    kept for calls outside of it."""
+    log, state = [], dict(stream="a", capturing=False)
+
+    class Stream:
+        name = property(lambda self: state["stream"])
+
+        def record_event(self):
+            log.append(("record", self.name))
+            return "event of " + self.name
+
+        def wait_event(self, event):
+            log.append(("wait", self.name, event))
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    monkeypatch.setattr(pkg.adapters.nat, "stream_handle", lambda device: state["stream"])
+    made, device = [], torch.device("cuda", 0)
+    loras = pkg.adapters.RequestLoras(_FakeTensor((2, 8, 32), device, torch.float32, made), _FakeTensor((2, 24, 8), device, torch.float32, made), [0, 1])
+    state["capturing"] = True
+    captured = loras.bank(device, torch.bfloat16)
+    state["capturing"] = False
+    first = loras.bank(device, torch.bfloat16)
+    assert first[0] is not captured[0] and log == [("record", "a")]
+    assert loras.bank(device, torch.bfloat16) is first and len(log) == 1
+    state["stream"] = "b"
+    assert loras.bank(device, torch.bfloat16) is first and loras.bank(device, torch.bfloat16) is first
+    assert log[1:] == [("wait", "b", "event of a")] and [t.streams for t in first] == [["a", "b"]] * 2
+    state["capturing"], state["stream"] = True, "c"
+    assert loras.bank(device, torch.bfloat16) is first and len(log) == 2
+    state["capturing"] = False
+    other = loras.bank(device, torch.float16)              # another type: converted anew, on the stream that asks
+    assert other is not first and log[2:] == [("record", "c")] and [t.streams for t in other] == [["c"]] * 2
+    assert len(made) == 2 + 2 * 3
