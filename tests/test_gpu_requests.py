@@ -213,6 +213,23 @@ def test_linear_lora_requests_rotated(cuda_pkg, rotated):
     assert torch.equal(y, F.linear_w8a8_lora_requests(q, qs, w, ws, b, t, lb, rows, torch.bfloat16))
 
 
+@pytest.mark.parametrize("lengths,adapters", [([9, 8], [0, 1]), ([1] * 30 + [70, 100], [i % 3 - 1 for i in range(30)] + [0, 2]), ([255], [1])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_lora_requests_plain_adapter_input_beside_rotated_rows(cuda_pkg, lengths, adapters, dtype):
+    """17 to 255 rows whose quantiser rotates while the adapters see the activations as they came."""
+    F = cuda_pkg.functional
+    rows = cuda_pkg.adapters.RequestRows(lengths, adapters, DEV)
+    w, ws, b, la, lb = layer(640, 328, 24, 3, dtype, 29)
+    x = torch.randn(rows.total, 640, generator=gen(30), device=DEV).to(dtype)
+    y = F.linear_lora_requests(x, w, ws, b, la, lb, rows, dtype, hadamard=True, rotated_lora_input=False)
+    q, qs = F.quantize_rowwise(x, hadamard=True)
+    assert torch.equal(y, F.linear_w8a8_lora_requests(q, qs, w, ws, b, F.lora_down_requests(x, la, rows), lb, rows, dtype))
+    base, base_tol = base_quantised(q, qs, w, ws, b)
+    term, term_tol = low_rank(x, la, lb, adapter_rows(rows), dtype)
+    want, off = base + term, base_tol + term_tol + 2 * 3 * E32 * (base.abs() + term.abs())      # two additions of sixteen ranks, one more
+    check(y, want, off + u_of(dtype) * (want.abs() + off) + TINY[dtype])
+
+
 SMALL = [
     ([1], [0], 64, 16, 8, torch.bfloat16), ([1], [-1], 64, 24, 8, torch.bfloat16), ([16], [1], 1040, 333, 24, torch.float16),
     ([1] * 16, [i % 7 - 1 for i in range(16)], 4096, 1000, 32, torch.bfloat16), ([3, 0, 5, 1], [0, 1, -1, 2], 256, 77, 128, torch.float16),
@@ -592,6 +609,68 @@ def test_two_calls_at_once_on_two_streams(cuda_pkg):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o[0], want[i][0]) and torch.equal(o[1], want[i][1]) for o in outs[i])
+
+
+CHAINS = [
+    # rows, K = N, rank, whether the form for at most 16 rows
+    ([1] * 9, [0, 1, 2, -1, 0, 1, 2, 0, 1], 512, 24, True),
+    ([1] * 40 + [20], [i % 3 for i in range(40)] + [2], 512, 16, False),
+    ([200, 30, 100], [0, -1, 1], 512, 64, False),
+    ([600, 1, 3, 900], [0, 1, 2, 2], 2048, 32, False),
+]
+
+
+@pytest.mark.parametrize("case", range(len(CHAINS)))
+@pytest.mark.parametrize("hadamard,rotated", [(False, True), (True, True), (True, False)])
+def test_whole_forwards_behind_one_another(cuda_pkg, case, hadamard, rotated):
+    """The whole-forward calls overlap their kernels' tails: chained layers, each behind the kernel that makes its input and in the
+    workspace of the one before, on two streams at once and as two captured graphs, give the bits of calls that wait for all else."""
+    F = cuda_pkg.functional
+    lengths, adapters, K, r, small = CHAINS[case]
+    if small and hadamard:
+        pytest.skip("the form for at most 16 rows takes rotated activations as they come")
+    rows = cuda_pkg.adapters.RequestRows(lengths, adapters, DEV)
+
+    def chain(state, wait):
+        x = state["x"]
+        for i, (w, ws, b, la, lb) in enumerate(state["layers"]):
+            if i % 2 == 0:
+                x = torch.nn.functional.rms_norm(x, (K,))
+            if wait:
+                torch.cuda.synchronize()
+            if small:
+                x = F.linear_small_batch_lora_requests(x, w, ws, b, la, lb, rows)
+            else:
+                x = F.linear_lora_requests(x, w, ws, b, la, lb, rows, x.dtype, hadamard=hadamard, rotated_lora_input=rotated)
+        return x
+
+    states = [dict(x=torch.randn(rows.total, K, generator=gen(900 + i), device=DEV).bfloat16(),
+                   layers=[layer(K, K, r, 3, torch.bfloat16, 910 + 10 * i + j) for j in range(6)]) for i in range(2)]
+    want = [chain(s, True) for s in states]
+    assert all(w.isfinite().all() for w in want) and not torch.equal(*want)
+    torch.cuda.synchronize()
+    for s, w in zip(states, want):
+        assert torch.equal(chain(s, False), w)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for _ in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(chain(states[i], False))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+    graphs, captured = [], []
+    for s in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            captured.append(chain(s, False))
+        graphs.append(g)
+    for i in (0, 1, 1, 0):
+        graphs[i].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(c, w) for c, w in zip(captured, want))
 
 
 def test_plan_dropped_while_another_stream_reads_it(cuda_pkg):
