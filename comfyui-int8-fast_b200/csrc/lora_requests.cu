@@ -671,7 +671,8 @@ int i8f_linear_w8a8_lora_requests(const int8_t* a, int64_t lda, const float* a_s
     return I8F_OK;
 }
 
-// Workspace of the whole forward: int8 rows, their scales, the rotated rows (where the adapters see them), t, the addend.
+// Workspace of the whole forward: int8 rows, their scales, the rotated rows (where the adapters see them), t, the addend (where
+// the product reads one).
 struct ForwardLayout {
     size_t scales, rotated, t, addend, total;
     ForwardLayout(const i8f_request_rows* rows, int64_t M, int64_t N, int64_t K, int64_t r, bool keep_rotated) {
@@ -679,7 +680,7 @@ struct ForwardLayout {
         rotated = scales + padded(static_cast<size_t>(M) * sizeof(float));
         t = rotated + (keep_rotated ? padded(static_cast<size_t>(M) * K * 2) : 0);
         addend = t + padded(static_cast<size_t>(M) * r * 2);
-        total = addend + addend_bytes(rows, N);
+        total = addend + (requests_need_addend(M, N, K) ? addend_bytes(rows, N) : 0);
     }
 };
 

@@ -489,3 +489,21 @@ def test_converted_bank_on_other_streams_and_in_captures(pkg, monkeypatch):
     other = loras.bank(device, torch.float16)              # another type: converted anew, on the stream that asks
     assert other is not first and log[2:] == [("record", "c")] and [t.streams for t in other] == [["c"]] * 2
     assert len(made) == 2 + 2 * 3
+
+
+def test_workspace_of_the_whole_forward(pkg):
+    """The fp32 addend is asked for only where the product reads it: chunked rows on 256-wide tiles (gemm_plan)."""
+    lib = pkg._native.load()
+
+    def padded(n):
+        return -(-n // 256) * 256
+
+    for lengths, N, K, r in (([1] * 64, 4096, 4096, 16), ([77], 4096, 4096, 64), ([1] * 400, 512, 1024, 8), ([1] * 5000, 12288, 4096, 16),
+                             ([1] * 300 + [5000], 12288, 4096, 16), ([5000], 12288, 4096, 16)):
+        rows = pkg.adapters.RequestRows(lengths, [i % 40 for i in range(len(lengths))], device="cpu")
+        M = rows.total
+        wide = pkg.functional.gemm_plan(M, N, K)["tile"][1] == 256
+        base = padded(M * K) + padded(4 * M) + padded(2 * M * r)
+        for rotated in (0, 1):
+            want = base + rotated * padded(2 * M * K) + (rows.native.addend_rows * N * 4 if wide else 0)
+            assert lib.i8f_linear_lora_requests_workspace_bytes(rows.native_ptr, N, K, r, rotated, rotated) == want
