@@ -817,6 +817,19 @@ def test_linear_module_on_two_streams_and_captured_first(cuda_pkg):
     assert torch.equal(captured, want)
 
 
+@pytest.mark.parametrize("tokens", [2, 50])
+def test_compiled_linear_with_request_loras(cuda_pkg, tokens):
+    """A compiled layer runs the adapters outside of its graph, with the same bits, and follows the adapters that it is given."""
+    w, ws, b, la, lb = layer(256, 320, 16, 3, torch.bfloat16, 47)
+    lin = cuda_pkg.ops.StandaloneInt8Ops.Linear(256, 320, bias=True, device="meta")
+    lin._load_from_state_dict({"weight": w, "weight_scale": ws, "bias": b}, "", {}, True, [], [], [])
+    x = torch.randn(4, tokens, 256, generator=gen(48), device=DEV).bfloat16()
+    compiled = torch.compile(lin, backend="eager")
+    for loras in (None, cuda_pkg.adapters.RequestLoras(la, lb, [1, -1]), cuda_pkg.adapters.RequestLoras(la, lb, [2, 0, 1, 1]), None):
+        lin.request_loras = loras
+        assert torch.equal(compiled(x), lin(x))
+
+
 def test_dit_batch_of_samples_fused(cuda_pkg):
     """A batch of samples through the fused block code against the same model in element-wise steps: the differences are 16-bit
     roundings that the fused pass leaves out, and the int8 steps they move."""
