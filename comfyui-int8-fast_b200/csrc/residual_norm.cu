@@ -12,9 +12,10 @@
 // fp32: h and its int8 form come from the unrounded x', so each output is
 // rounded once.  Row sums are per-thread sums, a shuffle tree, then the warps in order: the same order every time.
 //
-// Bound by the bytes of x, y, x' and h.  Measured, inputs from HBM: 4608 x 4096 bf16 36.6 us = 4.1 TB/s (63 % of the copy rate;
-// some 8 us of it pass before the first rows leave, the rest streams at 6.7 TB/s), 18432 x 4096 with an fp32 residual
-// 157 us = 5.8 TB/s (88 %), 777 rows of 2305 in 11 requests 17.9 us, one row 4.4 us.
+// Bound by the bytes of x, y, x' and h.  Measured, inputs from HBM: 4608 x 4096 bf16 in four equal requests 32.3 us = 4.7 TB/s
+// (71 % of the copy rate; some 8 us of it pass before the first rows leave, the rest streams at 6.7 TB/s), in four requests
+// of 46 to 3936 rows 36.6 us (a CTA whose rows cross a border works the columns of another request out), 18432 x 4096 with an
+// fp32 residual 157 us = 5.8 TB/s (88 %), 777 rows of 2305 in 11 requests 18.6 us, one row 4.3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -285,9 +286,9 @@ gated_residual_norm_kernel(const NormArgs a) {
 // pieces that contain the row; a row that starts `o` elements behind a boundary is handled in the vectors of its memory,
 // elements 8 v - o ... 8 v - o + 7, so that all but the first and the last are read and written in 16-byte pieces.  x, y
 // and the outputs must lie alike (o is the same for all of them), as contiguous tensors of one shape do.
-// Threads that take rows.  Five groups hide a row's chain of reductions better than four (4608 x 4096 bf16: 32.3 us against 34.5,
-// with int8 rows 30.0 against 32.6); fp32 rows leave room for seven slots only, and four groups serve them better (18432 x
-// 4096: 162 us against 166).
+// Threads that take rows.  Five groups hide a row's chain of reductions better than four (4608 x 4096 bf16 in four equal requests:
+// 32.3 us against 34.7, with int8 rows 30.8 against 33.9); fp32 rows leave room for seven slots only, and four groups serve
+// them better (18432 x 4096: 162 us against 166).
 template <int XDT, int GT>
 constexpr int workers() { return GT == 512 ? 512 : (XDT == I8F_F32 ? 4 : 5) * GT; }
 constexpr int kMaxSlots = 16;

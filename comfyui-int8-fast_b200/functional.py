@@ -525,7 +525,8 @@ def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lor
     adapter of each row's request (lora_a [adapters, r, K], lora_b [adapters, N, r], see adapters.stack_adapters) beside it.
 
     x [M,K] bf16 or fp16, out_dtype the same type.  With `hadamard` the adapters see the rotated activations unless
-    `rotated_lora_input` is false, as in the single-adapter forward."""
+    `rotated_lora_input` is false, as in the single-adapter forward.  Between the two low-rank products x @ lora_a^T is rounded
+    to x's type, as there (in fp16 its values may not pass 65504)."""
     device = x.device
     with _on(device):
         x, ldx = _pitched(x)
@@ -562,7 +563,7 @@ def linear_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lor
 def linear_small_batch_lora_requests(x: Tensor, w: Tensor, w_scale, bias: Tensor | None, lora_a: Tensor, lora_b: Tensor,
                                      rows: RequestRows) -> Tensor:
     """M <= 16 rows (single tokens) of several requests: y = x @ (w * w_scale)^T + bias + (x @ lora_a[a]^T) @ lora_b[a]^T with
-    the adapter a of each row, activations not quantised, one rounding to x's dtype (bf16 or fp16)."""
+    the adapter a of each row, activations not quantised, one rounding to x's dtype (bf16 or fp16) besides that of x @ lora_a^T."""
     device = x.device
     with _on(device):
         x, ldx = _pitched(x)

@@ -311,7 +311,10 @@ class DynamicLoRAHook:
 
     `request_loras` in transformer_options gives a batch one composition per request: a list with, for every request, a list
     of entries like those of `dynamic_loras` (which all requests share on top).  Each quantised layer then holds a bank of the
-    distinct compositions (`request_loras`) in place of lora_A / lora_B."""
+    distinct compositions (`request_loras`) in place of lora_A / lora_B.  Sample j of the batch, the model's first argument, is
+    request j modulo the number of requests; adapters.RequestLoras.plan says which inputs of a layer are refused because
+    their rows cannot be told apart.  A captured graph holds the factors and plans of its composition: another composition
+    replaces them, so it is not replayed after that.  Under torch.compile a layer with request_loras runs outside of the graph."""
     _HALF_SET = object()        # no composition's id: one that was refused half way is not taken for the one before
 
     def __init__(self):

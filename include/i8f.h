@@ -307,8 +307,8 @@ typedef struct i8f_request_rows {
     const int32_t* row_adapter; /* [rows]: index into the bank of adapters, -1: none */
     const int32_t* row_request; /* [rows]: request of the row (gated_residual_norm) */
     /* The batch in tiles of 256 rows: [ceil(rows / 256)][4] = first slot, slots, addend row, 0.  A dense tile (addend row
-     * -1) has one slot for each adapter in it, at most 32, of which at most 8 without chunks of their own; a chunked one
-     * none, its rows start at `addend row` of the fp32 addend and are covered by chunks. */
+     * -1) has one slot for each adapter in it, at most 32 (the package's plans make at most 16), of which at most 8
+     * without chunks of their own; a chunked one none, its rows start at `addend row` of the fp32 addend and are covered by chunks. */
     const int32_t* tiles;
     const int32_t* slots;       /* [][12]: adapter, 1 if chunks do its down projection (else 0), 0, 0, then 256 bits: the rows of
                                    the tile that use it */
@@ -372,10 +372,11 @@ int i8f_linear_w8a16_small_lora_requests(const void* x, int x_dtype, int64_t ldx
  * of them, 1 with NULL):
  *   x_out = residual_scale * x + g * post_norm(y) * post_weight       g = gate[q] or, with gate_tanh, tanh(gate[q])
  *   h     = norm(x_out) * weight * (1 + scale[q]) + shift[q]
+ * (with I8F_NORM_NONE post_norm(y) is y, and post_weight a layer scale.)
  * fp32 throughout; h comes from the unrounded x_out, so each output is rounded once.  x, x_out [M,K] in x_dtype
  * (y_dtype or I8F_F32); y, h and all vectors in y_dtype (I8F_BF16 or I8F_F16).  gate, scale, shift: [requests, K] with
  * pitches ldg, lds, ldt (0: one row for every request), each may be NULL (1, 0, 0), as may the weights [K].  h [M,K] and the per-token int8 form of h
- * (q [M,K], row_scale [M] as in i8f_quant_rowwise) may be asked for separately or both; NULL: not wanted.  x_out may be x.
+ * (q [M,K], row_scale [M] as in i8f_quant_rowwise, a NaN of a row being its scale) may be asked for separately or both; NULL: not wanted.  x_out may be x.
  * K at most 16384; rows of any length, pitch and alignment (16-byte aligned rows of a multiple of 8 elements are read
  * and written in 16-byte pieces). */
 int i8f_gated_residual_norm(const void* x, int x_dtype, int64_t ldx, const void* y, int y_dtype, int64_t ldy,
