@@ -35,6 +35,9 @@ class RequestRows:
 
     def __init__(self, lengths: Sequence[int], adapters: Sequence[int] | None = None,
                  device: torch.device | str = "cuda"):
+        device = torch.device(device)
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a row plan is made outside of a graph capture: its tables are copied from the host")
         n = np.asarray(lengths, dtype=np.int64).reshape(-1)
         a = np.full(n.shape, -1, dtype=np.int64) if adapters is None else np.asarray(adapters, dtype=np.int64).reshape(-1)
         if n.size == 0 or (n < 0).any():

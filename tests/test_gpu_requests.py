@@ -673,6 +673,18 @@ def test_whole_forwards_behind_one_another(cuda_pkg, case, hadamard, rotated):
     assert all(torch.equal(c, w) for c, w in zip(captured, want))
 
 
+def test_plan_within_a_capture_leaves_the_capture_whole(cuda_pkg):
+    """A plan is refused before anything reaches the device, so the capture goes on."""
+    x = torch.ones(4, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="outside of a graph capture"):
+            cuda_pkg.adapters.RequestRows([4], [0], DEV)
+        y = x + 1
+    graph.replay()
+    assert (y == 2).all()
+
+
 def test_plan_dropped_while_another_stream_reads_it(cuda_pkg):
     """The tables' memory is not handed on before the calls on other streams are done, whichever entry point made them."""
     F = cuda_pkg.functional

@@ -507,3 +507,10 @@ def test_workspace_of_the_whole_forward(pkg):
         for rotated in (0, 1):
             want = base + rotated * padded(2 * M * K) + (rows.native.addend_rows * N * 4 if wide else 0)
             assert lib.i8f_linear_lora_requests_workspace_bytes(rows.native_ptr, N, K, r, rotated, rotated) == want
+
+
+def test_plan_within_a_capture_is_refused(pkg, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="outside of a graph capture"):
+        pkg.adapters.RequestRows([4], [0], device="cuda")
+    assert pkg.adapters.RequestRows([4], [0], device="cpu").total == 4
