@@ -632,6 +632,19 @@ def _weight_vector(v: Tensor | None, name: str, y: Tensor):
     return v, v.data_ptr()
 
 
+def _rows_overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether rows of two 2-D tensors with unit inner stride share memory other than by being the same rows, element for element."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    (M, K), ea, eb = a.shape, a.element_size(), b.element_size()
+    lda, ldb = _ld(a) * ea, _ld(b) * eb
+    if pa == pb and ea == eb and (lda == ldb or M == 1):
+        return False
+    if not M or pa >= pb + (M - 1) * ldb + K * eb or pb >= pa + (M - 1) * lda + K * ea:
+        return False
+    d = (pb - pa) % lda
+    return lda != ldb or d < K * ea or lda - d < K * eb      # of one pitch: column blocks of one buffer may lie side by side
+
+
 def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm, post_weight, norm, weight, scale, shift, eps,
                          x_out, want_h, want_q):
     device = y.device
@@ -666,6 +679,8 @@ def _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm,
                 raise ValueError("x_out must have x's shape, type and device, rows of unit inner stride that do not overlap")
             if x_out is given:
                 x = x_out
+            if _rows_overlap(x_out, x) or _rows_overlap(x_out, y):
+                raise ValueError("x_out may be x or y themselves, but may not share memory with them otherwise")
             ldo = _ld(x_out)
         h = None if not want_h else torch.empty_like(y) if y.is_contiguous() else y.new_empty(shape)
         q = y.new_empty(shape, dtype=torch.int8) if want_q else None
@@ -698,8 +713,8 @@ def gated_residual_norm(x: Tensor, y: Tensor, gate: Tensor | None = None, *, row
     post_norm: None (y itself, post_weight is then a layer scale), "rms" or "layer" (without affine part); norm: "rms" or
     "layer".  gate, scale and shift are [K] for all rows or [requests, K] with the row plan `rows` (row slices of a wider
     matrix are read in place); they and the weights [K] are taken in y's dtype (bf16 or fp16).  x is in y's dtype or fp32.
-    Everything in between is fp32 and h comes from the unrounded x_new.  Returns (x_new, h); `x_out` (it may be x) receives
-    x_new.  At most 16384 columns."""
+    Everything in between is fp32 and h comes from the unrounded x_new.  Returns (x_new, h); `x_out` (it may be x, but may not
+    overlap it otherwise) receives x_new.  At most 16384 columns."""
     x_new, h, _, _ = _gated_residual_norm(x, y, gate, rows, gate_tanh, residual_scale, post_norm, post_weight, norm, weight, scale,
                                           shift, eps, x_out, True, False)
     return x_new, h

@@ -522,6 +522,33 @@ def test_gated_residual_norm_refuses(cuda_pkg):
         assert x_new.shape == h.shape == (M, K)
 
 
+def test_gated_residual_norm_into_shared_memory(cuda_pkg):
+    """x_out as y, as another view of x, as the columns beside x: the bits of a call into memory of its own.  Rows that overlap
+    otherwise are refused."""
+    F = cuda_pkg.functional
+    for M, K in ((9, 264), (700, 2048), (700, 1001)):
+        g = gen(M + K)
+        x, y = (torch.randn(M, K, generator=g, device=DEV).bfloat16() for _ in range(2))
+        want = F.gated_residual_norm(x, y, post_norm="rms")
+        y2 = y.clone()
+        got = F.gated_residual_norm(x, y2, post_norm="rms", x_out=y2)
+        assert torch.equal(y2, want[0]) and torch.equal(got[1], want[1])
+        wide = torch.zeros(M + 1, 2 * K, dtype=torch.bfloat16, device=DEV)
+        left, right = wide[:M, :K], wide[:M, K:]
+        left.copy_(x)
+        # the same rows at the same places: rows that lie otherwise to one another may be another kernel's, with sums in another order
+        want = F.gated_residual_norm(left, y, post_norm="rms")
+        got = F.gated_residual_norm(left, y, post_norm="rms", x_out=right)
+        assert torch.equal(right, want[0]) and torch.equal(got[1], want[1]) and torch.equal(left, x)
+        got = F.gated_residual_norm(left, y, post_norm="rms", x_out=wide[:M, :K])
+        assert torch.equal(left, want[0]) and torch.equal(got[1], want[1])
+        for out in (wide[1:, :K], wide[:M, 1:K + 1]):
+            with pytest.raises(ValueError, match="share memory"):
+                F.gated_residual_norm(left, y, x_out=out)
+            with pytest.raises(ValueError, match="share memory"):
+                F.gated_residual_norm(x, left, x_out=out)
+
+
 # ------------------------------------------------------------------ together, streams, graphs, long offsets
 def block_step(pkg, s):
     """A residual update with its int8 output and the quantised projection with adapters that follows it, as a block runs them."""

@@ -514,3 +514,21 @@ def test_plan_within_a_capture_is_refused(pkg, monkeypatch):
     with pytest.raises(RuntimeError, match="outside of a graph capture"):
         pkg.adapters.RequestRows([4], [0], device="cuda")
     assert pkg.adapters.RequestRows([4], [0], device="cpu").total == 4
+
+
+def test_output_rows_that_overlap_the_input_are_seen(pkg):
+    """The rows of x_out may be those of x, or lie beside them in one buffer; anything else that shares memory would be read and
+    written at once."""
+    overlap = pkg.functional._rows_overlap
+    buf = torch.zeros(4000)
+    wide = buf[:3000].view(30, 100)
+    x = wide[2:12, 8:40]
+    for other in (x, x[:], wide[2:12, 40:72], wide[2:12, 68:100], wide[12:22, 8:40], torch.zeros(10, 32), buf[3000:3320].view(10, 32)):
+        assert not overlap(x, other) and not overlap(other, x)
+    assert not overlap(x[:, :24], wide[1:11, 76:]) and not overlap(x[:1], buf[208:240].view(1, 32))
+    for other in (wide[3:13, 8:40], wide[1:11, 8:40], wide[2:12, 9:41], wide[2:12, 0:32], wide[3:13, 39:71], wide[1:11, 68:100].as_strided((10, 32), (100, 1), 180),
+                  buf[208:528].view(10, 32), buf[:2000].view(10, 200)[:, :32]):
+        assert overlap(x, other) and overlap(other, x)
+    half = buf.view(torch.bfloat16)
+    assert overlap(x, half[416:416 + 320].view(10, 32)) and overlap(half.view(40, 200)[2:12, 16:48], x)
+    assert not overlap(half.view(40, 200)[2:12, 80:112], x) and not overlap(x[:0], x[:0])
