@@ -188,10 +188,10 @@ class RequestLoras:
 
         Where the requests differ, the samples are as many as the model's batch has where its hook has said so: the input's
         leading dimension has to be that many, or 1 with the rows of all samples behind it (rows that the samples share have no
-        adapter of their own).  Another leading dimension is refused, since it does not say whether its rows
-        repeat the samples one after the other or cut each of them in pieces.  Where the hook could not see the batch `leading`
-        counts and an input of two dimensions is refused; where no hook speaks for the model such an input is one run of rows
-        per request.  Rows that are not equal runs for every request are refused."""
+        adapter of their own).  Another leading dimension is refused, since it does not say whether it repeats the batch or cuts
+        every sample in pieces.  Where the hook could not see the batch `leading` counts and an input of two dimensions is
+        refused; where no hook speaks for the model such an input is one run of rows per request.  Rows that are not equal
+        runs for every request are refused."""
         known, n = self.samples, len(self.entries)
         if not rows:
             samples = n
@@ -199,7 +199,8 @@ class RequestLoras:
             return self._planned([rows], self.entries[:1], device)
         elif known is not None:
             if leading not in (None, 1, known):
-                raise ValueError(f"a leading dimension of {leading} for a batch of {known} samples: which rows are whose cannot be known")
+                raise ValueError(f"a leading dimension of {leading} for a batch of {known} samples: which rows are whose cannot be known "
+                                 "(an input of two dimensions holds the samples' rows one sample after the other)")
             samples = known
         elif leading is not None:
             samples = leading
